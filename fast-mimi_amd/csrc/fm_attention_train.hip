@@ -1,0 +1,819 @@
+// Causal sliding-window attention for training: forward with the row's
+// log-sum-exp, and the backward pass, which forms the probabilities again from
+// it.  FP32, bfloat16 and float16; grouped query heads; padded batches.
+//
+// A key head's queries are rows r = t * G + g (position t, head g of its group
+// of G), so grouped heads share every key tile that is loaded and the key and
+// value gradients sum over them without atomics.  Query t stands at position
+// p = S - T + t; key j is visible iff p - window < j <= p and p < length.
+//
+//   forward   S = Q K^T c, P = exp2(S - max), O = P V / sum P      (c = scale log2 e)
+//   backward  P = exp2(S - lse), D = rowsum(dO O), dS = P (dO V^T - D)
+//             dQ = dS K scale                     (one block: some rows, all their keys)
+//             dV = P^T dO, dK = dS^T Q scale      (one block: some keys, all their rows)
+//
+// All products run on 32x32 MFMA tiles and are arranged so that what a lane
+// holds of one is its operand of the next: S^T (keys x rows) leaves lane l with
+// row l % 32 and sixteen keys of it, which is the B operand of O^T = V^T P^T
+// once V^T is read in the same order of keys; no probability crosses lanes.
+// FP32 inputs use the FP32 MFMA throughout; 16-bit ones round P and dS (in
+// [0, 1], or a product with it) to the inputs' type for the second product, as
+// the operands of the 16-bit MFMA are; every sum, maximum and gradient is FP32.
+
+#include "fm_common.h"
+
+namespace {
+
+typedef __bf16 bf16x2_v __attribute__((ext_vector_type(2)));
+typedef _Float16 halfx2_v __attribute__((ext_vector_type(2)));
+typedef float floatx2_v __attribute__((ext_vector_type(2)));
+typedef unsigned uintx2_v __attribute__((ext_vector_type(2)));
+typedef unsigned uintx4_v __attribute__((ext_vector_type(4)));
+
+constexpr float LOG2E = 1.44269504088896341f;
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+  typedef floatx4 Frag;
+  static constexpr int STEP = 8;  // contraction elements of one fragment pair (two lane halves of 16 bytes)
+  static FM_DEVICE floatx16 mma(Frag a, Frag b, floatx16 c) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c = fm_mfma32(a[e], b[e], c);
+    return c;
+  }
+  // Accumulator elements STEP / 2 * s .. of a lane as an operand.
+  static FM_DEVICE Frag pack(const floatx16& p, int s) { return Frag{p[4 * s], p[4 * s + 1], p[4 * s + 2], p[4 * s + 3]}; }
+  static FM_DEVICE float dot(Frag a, Frag b, float s) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s = fmaf(a[e], b[e], s);
+    return s;
+  }
+  static FM_DEVICE void store4(float* p, float a, float b, float c, float d) {
+    *reinterpret_cast<floatx4*>(p) = floatx4{a, b, c, d};
+  }
+};
+template <> struct Elem<__bf16> {
+  typedef bf16x8 Frag;
+  static constexpr int STEP = 16;
+  static FM_DEVICE floatx16 mma(Frag a, Frag b, floatx16 c) { return fm_mfma32_bf16(a, b, c); }
+  static FM_DEVICE unsigned two(float a, float b) {
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((floatx2_v{a, b}), bf16x2_v));
+  }
+  static FM_DEVICE Frag pack(const floatx16& p, int s) {
+    uintx4_v u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = two(p[8 * s + 2 * e], p[8 * s + 2 * e + 1]);
+    return __builtin_bit_cast(Frag, u);
+  }
+  static FM_DEVICE float dot(Frag a, Frag b, float s) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf((float)a[e], (float)b[e], s);
+    return s;
+  }
+  static FM_DEVICE void store4(__bf16* p, float a, float b, float c, float d) {
+    *reinterpret_cast<uintx2_v*>(p) = uintx2_v{two(a, b), two(c, d)};
+  }
+};
+template <> struct Elem<_Float16> {
+  typedef halfx8 Frag;
+  static constexpr int STEP = 16;
+  static FM_DEVICE floatx16 mma(Frag a, Frag b, floatx16 c) { return fm_mfma32_f16(a, b, c); }
+  static FM_DEVICE unsigned two(float a, float b) {
+    return __builtin_bit_cast(unsigned, __builtin_convertvector((floatx2_v{a, b}), halfx2_v));
+  }
+  static FM_DEVICE Frag pack(const floatx16& p, int s) {
+    uintx4_v u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = two(p[8 * s + 2 * e], p[8 * s + 2 * e + 1]);
+    return __builtin_bit_cast(Frag, u);
+  }
+  static FM_DEVICE float dot(Frag a, Frag b, float s) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf((float)a[e], (float)b[e], s);
+    return s;
+  }
+  static FM_DEVICE void store4(_Float16* p, float a, float b, float c, float d) {
+    *reinterpret_cast<uintx2_v*>(p) = uintx2_v{two(a, b), two(c, d)};
+  }
+};
+
+// A strided [batch][rows][heads][head_dim] input; strides in elements.
+struct View {
+  const void* p;
+  long batch, row, head;
+};
+
+struct Attn {
+  View q, k, v, dout;
+  const void* o;  // backward: the forward's output, contiguous
+  void *out, *dk, *dv;  // forward: O; backward: dQ in out
+  float* lse;      // [B][T][H], log2 of the row's sum of exponentials
+  float* delta;    // [B][T][H], rowsum(dO O)
+  float *part_o, *part_ml;  // split forward: unnormalised O [split][B][KV][R][DT], then (max, sum)
+  const int* lengths;
+  int B, T, S, H, KV, G, D, window, splits;
+  FmDivisor by_g;
+  float scale, scale2;
+};
+
+// Tiles in LDS keep 16-byte chunk c of row r at chunk c ^ swz(r): eight rows
+// of one chunk (a fragment read) then lie in eight different chunk positions,
+// and four rows of a 64-byte column block (a transposed read) in all of them.
+FM_DEVICE int swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+
+// 32 rows of an LDS tile as the A operand of a product over its columns:
+// lane l holds row l % 32, bytes 32 s + 16 (l / 32) .. + 15.
+template <typename T, int DT>
+FM_DEVICE typename Elem<T>::Frag row_frag(const unsigned char* tile, int row, int s, int lane) {
+  constexpr int PITCH = DT * (int)sizeof(T);
+  const int r = row + (lane & 31);
+  const int chunk = (2 * s + (lane >> 5)) ^ swz(r);
+  return __builtin_bit_cast(typename Elem<T>::Frag, *reinterpret_cast<const uintx4_v*>(tile + r * PITCH + chunk * 16));
+}
+
+// Columns 0 .. DT - 1 of STEP rows as A operands (one per 32 columns) of a
+// product over the rows, in the order in which a lane holds a 32x32 result:
+// lane l holds column l % 32 of rows row + 8 i + 4 (l / 32) + 0..3.  16-bit
+// tiles use the LDS transpose read: each group of 16 lanes reads 4 rows x 16
+// columns, lane i gets column i.  Its builtin makes the compiler wait for the
+// next tile's copies too, so the reads and their wait are one asm block.  FP32
+// tiles read single values.
+template <typename T, int DT>
+FM_DEVICE void col_frags(const unsigned char* tile, int row, int lane, typename Elem<T>::Frag (&f)[DT / 32]) {
+  constexpr int PITCH = DT * (int)sizeof(T);
+  if constexpr (sizeof(T) == 4) {
+    const int col = lane & 31;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = row + 4 * (lane >> 5) + e;
+      const unsigned char* at = tile + r * PITCH + (((col >> 2) ^ swz(r)) << 4) + (col & 3) * 4;
+#pragma unroll
+      for (int dt = 0; dt < DT / 32; ++dt) f[dt][e] = *reinterpret_cast<const float*>(at + 128 * dt);
+    }
+  } else {
+    const int r = row + 4 * (lane >> 5) + ((lane >> 2) & 3), low = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+    // Column blocks 2 i and 2 i + 1 lie 64 bytes apart, in the order that the swizzle gives.
+    const unsigned char* base = tile + r * PITCH + (lane & 1) * 8;
+    const unsigned at0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)(base + ((low ^ swz(r)) << 4));
+    const unsigned at1 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)(base + (((4 + low) ^ swz(r)) << 4));
+    uintx2_v u[DT / 32][2];
+    if constexpr (DT == 64)
+      asm volatile(
+          "ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
+          "ds_read_b64_tr_b16 %2, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(u[0][0]), "=&v"(u[0][1]), "=&v"(u[1][0]), "=&v"(u[1][1])
+          : "v"(at0), "v"(at1), "n"(8 * PITCH));
+    else
+      asm volatile(
+          "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%10\n\t"
+          "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%10\n\t"
+          "ds_read_b64_tr_b16 %4, %8 offset:128\n\tds_read_b64_tr_b16 %5, %8 offset:%11\n\t"
+          "ds_read_b64_tr_b16 %6, %9 offset:128\n\tds_read_b64_tr_b16 %7, %9 offset:%11\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(u[0][0]), "=&v"(u[0][1]), "=&v"(u[1][0]), "=&v"(u[1][1]), "=&v"(u[2][0]), "=&v"(u[2][1]),
+            "=&v"(u[3][0]), "=&v"(u[3][1])
+          : "v"(at0), "v"(at1), "n"(8 * PITCH), "n"(8 * PITCH + 128));
+#pragma unroll
+    for (int dt = 0; dt < DT / 32; ++dt)
+      f[dt] = __builtin_bit_cast(typename Elem<T>::Frag, (uintx4_v{u[dt][0][0], u[dt][0][1], u[dt][1][0], u[dt][1][1]}));
+  }
+}
+
+// The B operand of one row straight from memory: chunk s of the lane's half,
+// zeros where the row is not live or the chunk lies past the head's width.
+template <typename T, int DT>
+FM_DEVICE void load_row(const T* row, bool live, int D, int lane, typename Elem<T>::Frag (&f)[DT / Elem<T>::STEP]) {
+  constexpr int N = DT / Elem<T>::STEP, E = 16 / (int)sizeof(T);
+#pragma unroll
+  for (int s = 0; s < N; ++s) {
+    const int d = (2 * s + (lane >> 5)) * E;
+    uintx4_v u{0, 0, 0, 0};
+    if (live && d < D) u = *reinterpret_cast<const uintx4_v*>(row + d);
+    f[s] = __builtin_bit_cast(typename Elem<T>::Frag, u);
+  }
+}
+
+// Starts the copy of ROWS rows into LDS (global -> LDS, 16 bytes a lane).
+// offset(r) is the byte offset of tile row r from `base`, or negative for a
+// row that is not there (zeros).
+template <typename T, int DT, int ROWS, int WAVES, typename Offset>
+FM_DEVICE void load_tile(const void* base, unsigned char* tile, int D, int wave, int lane, Offset offset) {
+  constexpr int PITCH = DT * (int)sizeof(T), CPR = PITCH / 16, INSTR = ROWS * PITCH / 1024;
+  static_assert(INSTR % WAVES == 0, "whole instructions per wave");
+  const __amdgpu_buffer_rsrc_t buf = fm_buffer(base, INT_MAX);
+#pragma unroll
+  for (int u = 0; u < INSTR / WAVES; ++u) {
+    const int i = wave * (INSTR / WAVES) + u;
+    const int slot = i * 64 + lane, r = slot / CPR, chunk = (slot % CPR) ^ swz(r);
+    const int off = offset(r);
+    const bool ok = off >= 0 && chunk * 16 < D * (int)sizeof(T);
+    fm_buf_load_lds16(buf, tile + i * 1024, ok ? off + chunk * 16 : INT_MIN, 0);
+  }
+}
+
+// The sum or maximum of the two lane halves, in both.
+FM_DEVICE float other_half(float v) { return __shfl_xor(v, 32, 64); }
+
+FM_DEVICE void tile_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// What the row kernels (forward, dQ) share: the rows of a block and wave and
+// the keys they see.
+template <int WQ>
+struct Rows {
+  int b, kh, len, R, r, t, p, p_lo, p_hi, k_lo, k_hi;
+  bool live;
+  long row_index;  // into [B][T][H]
+  FM_DEVICE Rows(const Attn& a, int wq, int lane) {
+    b = blockIdx.x / a.KV, kh = blockIdx.x - b * a.KV;
+    len = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S;
+    R = a.T * a.G;
+    const int r0 = blockIdx.y * 32 * WQ, past = a.S - a.T;
+    const int w0 = min(r0 + 32 * wq, R - 1), w1 = min(r0 + 32 * wq + 31, R - 1);
+    p_lo = past + (int)fm_div(w0, a.by_g);  // the wave's positions
+    p_hi = min(past + (int)fm_div(w1, a.by_g), len - 1);
+    r = r0 + 32 * wq + (lane & 31);
+    t = (int)fm_div(min(r, R - 1), a.by_g);
+    p = past + t;
+    live = r < R && p < len;
+    row_index = ((long)b * a.T + t) * a.H + kh * a.G + (min(r, R - 1) - t * a.G);
+    // The block's keys.
+    const int b_lo = past + (int)fm_div(r0, a.by_g);
+    const int b_hi = past + (int)fm_div(min(r0 + 32 * WQ, R) - 1, a.by_g);
+    k_lo = max(0, b_lo - a.window + 1);
+    k_hi = min(b_hi, len - 1);
+  }
+  template <typename T> FM_DEVICE const T* of(const View& v) const {
+    return static_cast<const T*>(v.p) + b * v.batch;
+  }
+};
+
+// O^T or dQ^T of four waves that each took a quarter of the keys, summed into
+// wave w's quarter of the registers; weight: the wave's own factor of its part.
+template <int DT, int WK>
+FM_DEVICE void merge(float* lds, floatx16 (&acc)[DT / 32], int wk, int lane, float (&mine)[DT / 2 / WK]) {
+  constexpr int N = DT / 2;
+#pragma unroll
+  for (int i = 0; i < N; ++i) lds[(wk * N + i) * 64 + lane] = acc[i / 16][i % 16];
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N / WK; ++i) {
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WK; ++w) s += lds[(w * N + wk * (N / WK) + i) * 64 + lane];
+    mine[i] = s;
+  }
+}
+
+template <typename T, int DT, int WQ, int WK>
+struct Tiling {
+  static constexpr int NB = WK > 1 || sizeof(T) == 4 ? 1 : 2;  // 32-key tiles of a wave
+  static constexpr int KEYS = 32 * NB * WK;
+  static constexpr int TILE = KEYS * DT * (int)sizeof(T);
+  static constexpr int STAGES = 4 * TILE <= 131072 ? 2 : 1;
+  static constexpr int LDS = 2 * STAGES * TILE;
+  // Blocks per CU that the registers are held to.  At two (256 a lane) all of
+  // them are vector registers and no result passes through accumulation
+  // registers; the kernels that need more (HEAVY) run one block.
+  template <bool HEAVY> static constexpr int blocks() { return LDS > 81920 || HEAVY ? 1 : 2; }
+};
+
+// Forward.  WQ waves take 32 rows each and share the key tiles (many rows), or
+// WK waves take the same 32 rows and a quarter of each key tile (few rows).
+template <typename T, int DT, int WQ, int WK>
+__global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<false>())) void attention_forward_kernel(Attn a) {
+  typedef Elem<T> E;
+  typedef Tiling<T, DT, WQ, WK> L;
+  constexpr int NS = DT / E::STEP, ND = DT / 32;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[L::LDS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave % WQ, wk = wave / WQ, half = lane >> 5;
+  const Rows<WQ> w(a, wq, lane);
+
+  typename E::Frag qf[NS];
+  load_row<T, DT>(w.template of<T>(a.q) + w.t * a.q.row + (w.kh * a.G + (min(w.r, w.R - 1) - w.t * a.G)) * a.q.head, w.live,
+                  a.D, lane, qf);
+  floatx16 acc[ND] = {};
+  float m = -INFINITY, l = 0.0f;  // l: of this lane's keys only
+
+  int tiles = w.k_hi >= w.k_lo ? (w.k_hi - w.k_lo) / L::KEYS + 1 : 0, first = 0;
+  if (a.splits > 1) {
+    const int per = (tiles + a.splits - 1) / a.splits;
+    first = blockIdx.z * per;
+    tiles = min(tiles, first + per);
+  }
+  const T* kp = w.template of<T>(a.k) + w.kh * a.k.head;
+  const T* vp = w.template of<T>(a.v) + w.kh * a.v.head;
+  auto load = [&](int i) {
+    const int k0 = w.k_lo + i * L::KEYS, n = w.k_hi - k0;
+    unsigned char* at = lds + (i - first) % L::STAGES * 2 * L::TILE;
+    const int ks = (int)(a.k.row * (long)sizeof(T)), vs = (int)(a.v.row * (long)sizeof(T));
+    load_tile<T, DT, L::KEYS, 4>(kp + k0 * a.k.row, at, a.D, wave, lane, [&](int r) { return r <= n ? r * ks : -1; });
+    load_tile<T, DT, L::KEYS, 4>(vp + k0 * a.v.row, at + L::TILE, a.D, wave, lane,
+                                 [&](int r) { return r <= n ? r * vs : -1; });
+  };
+  if (first < tiles) load(first);
+  for (int i = first; i < tiles; ++i) {
+    tile_barrier();  // tile i is there, and every wave is past tile i - 1
+    if (L::STAGES == 2 && i + 1 < tiles) load(i + 1);
+    const unsigned char* kt = lds + (i - first) % L::STAGES * 2 * L::TILE;
+    const unsigned char* vt = kt + L::TILE;
+#pragma unroll
+    for (int nb = 0; nb < L::NB; ++nb) {
+      const int row = (wk * L::NB + nb) * 32, k0 = w.k_lo + i * L::KEYS + row;
+      if (k0 > w.p_hi || k0 + 31 <= w.p_lo - a.window) continue;  // nothing that this wave sees
+      floatx16 s = {};
+#pragma unroll
+      for (int c = 0; c < NS; ++c) s = E::mma(row_frag<T, DT>(kt, row, c, lane), qf[c], s);
+      if (k0 + 31 > w.p_lo || k0 <= w.p_hi - a.window || k0 + 31 > w.k_hi) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int key = k0 + 8 * (e >> 2) + 4 * half + (e & 3);
+          s[e] = key <= w.p && key > w.p - a.window && key <= w.k_hi ? s[e] : -INFINITY;
+        }
+      }
+      float top = s[0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
+      top = fmaxf(top, other_half(top)) * a.scale2;
+      if (__any(top > m)) {
+        const float up = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - (up == -INFINITY ? 0.0f : up));
+        m = up;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[d][e] *= f;
+      }
+      const float sub = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -sub));
+        l += s[e];
+      }
+#pragma unroll
+      for (int c = 0; c < 32 / E::STEP; ++c) {
+        const typename E::Frag p = E::pack(s, c);
+        typename E::Frag f[ND];
+        col_frags<T, DT>(vt, row + c * E::STEP, lane, f);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[d] = E::mma(f[d], p, acc[d]);
+      }
+    }
+    if (L::STAGES == 1 && i + 1 < tiles) {
+      tile_barrier();
+      load(i + 1);
+    }
+  }
+  l += other_half(l);
+
+  constexpr int MINE = DT / 2 / WK;
+  float mine[MINE];
+  if constexpr (WK > 1) {
+    __shared__ float ml[2][WK][32];
+    __syncthreads();
+    if (half == 0) ml[0][wk][lane] = m, ml[1][wk][lane] = l;
+    __syncthreads();
+    const float own = m;
+    m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int u = 0; u < WK; ++u) m = fmaxf(m, ml[0][u][lane & 31]);
+    const float sub = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int u = 0; u < WK; ++u) l += ml[1][u][lane & 31] * __builtin_amdgcn_exp2f(ml[0][u][lane & 31] - sub);
+    const float f = __builtin_amdgcn_exp2f(own - sub);
+#pragma unroll
+    for (int d = 0; d < ND; ++d)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[d][e] *= f;
+    merge<DT, WK>(reinterpret_cast<float*>(lds), acc, wk, lane, mine);
+  } else {
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) mine[i] = acc[i / 16][i % 16];
+  }
+  if (w.r >= w.R) return;
+  const bool writes = half == 0 && wk == 0;
+  if (a.splits > 1) {
+    const long at = ((long)blockIdx.z * gridDim.x + blockIdx.x) * w.R + w.r;
+    if (writes) *reinterpret_cast<floatx2_v*>(a.part_ml + 2 * at) = floatx2_v{m, l};
+    float* o = a.part_o + at * DT;
+#pragma unroll
+    for (int i = 0; i < MINE; i += 4) {
+      const int e = wk * MINE + i;
+      *reinterpret_cast<floatx4*>(o + 32 * (e / 16) + 8 * (e % 16 / 4) + 4 * half) =
+          floatx4{mine[i], mine[i + 1], mine[i + 2], mine[i + 3]};
+    }
+    return;
+  }
+  // A row that sees nothing (padding) gives zeros.
+  const float inv = w.live && l > 0.0f ? 1.0f / l : (w.live && l != l ? l : 0.0f);
+  if (writes) a.lse[w.row_index] = w.live && l != 0.0f ? m + log2f(l) : -INFINITY;
+  T* o = static_cast<T*>(a.out) + w.row_index * a.D;
+#pragma unroll
+  for (int i = 0; i < MINE; i += 4) {
+    const int e = wk * MINE + i, d = 32 * (e / 16) + 8 * (e % 16 / 4) + 4 * half;
+    if (d < a.D)
+      E::store4(o + d, w.live ? mine[i] * inv : 0.0f, w.live ? mine[i + 1] * inv : 0.0f, w.live ? mine[i + 2] * inv : 0.0f,
+                w.live ? mine[i + 3] * inv : 0.0f);
+  }
+}
+
+// Joins the parts of a split forward: one wave per row, lane d of DT columns.
+template <typename T, int DT>
+__global__ __launch_bounds__(256) void attention_join_kernel(Attn a) {
+  const int lane = threadIdx.x & 63, R = a.T * a.G;
+  const long rows = (long)a.B * a.KV * R, at = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= rows) return;
+  const int seq = (int)(at / R), r = (int)(at - (long)seq * R), b = seq / a.KV, kh = seq - b * a.KV;
+  const int t = (int)fm_div(r, a.by_g);
+  const int len = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S;
+  const bool live = a.S - a.T + t < len;
+  float m = -INFINITY, l = 0.0f, o[DT / 64] = {};
+  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * rows + at)]);
+  const float sub = m == -INFINITY ? 0.0f : m;
+  for (int s = 0; s < a.splits; ++s) {
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * (s * rows + at)] - sub);
+    l = fmaf(a.part_ml[2 * (s * rows + at) + 1], f, l);
+#pragma unroll
+    for (int u = 0; u < DT / 64; ++u) o[u] = fmaf(a.part_o[(s * rows + at) * DT + 64 * u + lane], f, o[u]);
+  }
+  const long row = ((long)b * a.T + t) * a.H + kh * a.G + (r - t * a.G);
+  if (lane == 0) a.lse[row] = live && l != 0.0f ? m + log2f(l) : -INFINITY;
+  T* out = static_cast<T*>(a.out) + row * a.D;
+#pragma unroll
+  for (int u = 0; u < DT / 64; ++u)
+    if (64 * u + lane < a.D) out[64 * u + lane] = (T)(live && l != 0.0f ? o[u] / l : 0.0f);
+}
+
+// dQ, and rowsum(dO O) for the dK / dV kernel: rows and keys as the forward.
+template <typename T, int DT, int WQ, int WK>
+__global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<sizeof(T) == 4 && DT == 128>())) void attention_dq_kernel(Attn a) {
+  typedef Elem<T> E;
+  typedef Tiling<T, DT, WQ, WK> L;
+  constexpr int NS = DT / E::STEP, ND = DT / 32;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[L::LDS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave % WQ, wk = wave / WQ, half = lane >> 5;
+  const Rows<WQ> w(a, wq, lane);
+
+  const T* kp = w.template of<T>(a.k) + w.kh * a.k.head;
+  const T* vp = w.template of<T>(a.v) + w.kh * a.v.head;
+  const int tiles = w.k_hi >= w.k_lo ? (w.k_hi - w.k_lo) / L::KEYS + 1 : 0;
+  auto load = [&](int i) {
+    const int k0 = w.k_lo + i * L::KEYS, n = w.k_hi - k0;
+    unsigned char* at = lds + i % L::STAGES * 2 * L::TILE;
+    const int ks = (int)(a.k.row * (long)sizeof(T)), vs = (int)(a.v.row * (long)sizeof(T));
+    load_tile<T, DT, L::KEYS, 4>(kp + k0 * a.k.row, at, a.D, wave, lane, [&](int r) { return r <= n ? r * ks : -1; });
+    load_tile<T, DT, L::KEYS, 4>(vp + k0 * a.v.row, at + L::TILE, a.D, wave, lane,
+                                 [&](int r) { return r <= n ? r * vs : -1; });
+  };
+  if (tiles) load(0);
+
+  typename E::Frag qf[NS], gf[NS];
+  const int head = w.kh * a.G + (min(w.r, w.R - 1) - w.t * a.G);
+  load_row<T, DT>(w.template of<T>(a.dout) + w.t * a.dout.row + head * a.dout.head, w.live, a.D, lane, gf);
+  load_row<T, DT>(static_cast<const T*>(a.o) + w.row_index * a.D, w.live, a.D, lane, qf);
+  float delta = 0.0f;
+#pragma unroll
+  for (int c = 0; c < NS; ++c) delta = E::dot(gf[c], qf[c], delta);
+  delta += other_half(delta);
+  load_row<T, DT>(w.template of<T>(a.q) + w.t * a.q.row + head * a.q.head, w.live, a.D, lane, qf);
+  if (w.r < w.R && half == 0 && wk == 0) a.delta[w.row_index] = delta;
+  // A row without keys takes every probability as zero.
+  float lse = w.live ? a.lse[w.row_index] : INFINITY;
+  lse = lse == -INFINITY ? INFINITY : lse;
+
+  floatx16 acc[ND] = {};
+  for (int i = 0; i < tiles; ++i) {
+    tile_barrier();
+    if (L::STAGES == 2 && i + 1 < tiles) load(i + 1);
+    const unsigned char* kt = lds + i % L::STAGES * 2 * L::TILE;
+    const unsigned char* vt = kt + L::TILE;
+#pragma unroll
+    for (int nb = 0; nb < L::NB; ++nb) {
+      const int row = (wk * L::NB + nb) * 32, k0 = w.k_lo + i * L::KEYS + row;
+      if (k0 > w.p_hi || k0 + 31 <= w.p_lo - a.window) continue;
+      floatx16 s = {}, dp = {};
+#pragma unroll
+      for (int c = 0; c < NS; ++c) s = E::mma(row_frag<T, DT>(kt, row, c, lane), qf[c], s);
+#pragma unroll
+      for (int c = 0; c < NS; ++c) dp = E::mma(row_frag<T, DT>(vt, row, c, lane), gf[c], dp);
+      const bool edge = k0 + 31 > w.p_lo || k0 <= w.p_hi - a.window || k0 + 31 > w.k_hi;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -lse));
+        s[e] = p * (dp[e] - delta);
+      }
+      if (edge) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int key = k0 + 8 * (e >> 2) + 4 * half + (e & 3);
+          s[e] = key <= w.p && key > w.p - a.window && key <= w.k_hi && w.live ? s[e] : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 32 / E::STEP; ++c) {
+        const typename E::Frag ds = E::pack(s, c);
+        typename E::Frag f[ND];
+        col_frags<T, DT>(kt, row + c * E::STEP, lane, f);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[d] = E::mma(f[d], ds, acc[d]);
+      }
+    }
+    if (L::STAGES == 1 && i + 1 < tiles) {
+      tile_barrier();
+      load(i + 1);
+    }
+  }
+  constexpr int MINE = DT / 2 / WK;
+  float mine[MINE];
+  if constexpr (WK > 1) {
+    __syncthreads();
+    merge<DT, WK>(reinterpret_cast<float*>(lds), acc, wk, lane, mine);
+  } else {
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) mine[i] = acc[i / 16][i % 16];
+  }
+  if (w.r >= w.R) return;
+  T* o = static_cast<T*>(a.out) + w.row_index * a.D;
+#pragma unroll
+  for (int i = 0; i < MINE; i += 4) {
+    const int e = wk * MINE + i, d = 32 * (e / 16) + 8 * (e % 16 / 4) + 4 * half;
+    const float f = a.scale;
+    if (d < a.D)
+      E::store4(o + d, w.live ? mine[i] * f : 0.0f, w.live ? mine[i + 1] * f : 0.0f, w.live ? mine[i + 2] * f : 0.0f,
+                w.live ? mine[i + 3] * f : 0.0f);
+  }
+}
+
+// dK and dV of 32 keys a wave over every row that sees them.  WK waves take 32
+// keys each and share the row tiles (many keys), or WR waves take the same 32
+// keys and a quarter of each row tile.
+template <typename T, int DT, int WK, int WR>
+__global__ __launch_bounds__(256, (Tiling<T, DT, WK, WR>::template blocks<DT == 128>())) void attention_dkv_kernel(Attn a) {
+  typedef Elem<T> E;
+  typedef Tiling<T, DT, WK, WR> L;  // rows in the place of keys
+  constexpr int NS = DT / E::STEP, ND = DT / 32, ROWS = L::KEYS;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[L::LDS];
+  __shared__ __attribute__((aligned(16))) float stat[L::STAGES][3][ROWS];  // lse, delta, position (as an int)
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wk = wave % WK, wr = wave / WK, half = lane >> 5;
+  const int b = blockIdx.x / a.KV, kh = blockIdx.x - b * a.KV;
+  const int len = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S, past = a.S - a.T;
+  const int k0 = blockIdx.y * 32 * WK, w0 = k0 + 32 * wk, key = w0 + (lane & 31);
+  const bool live = key < len;
+  // Rows of the positions that see any of the block's keys.
+  const int p_lo = max(k0, past);
+  const int p_hi = min((long)min(k0 + 32 * WK, len) - 1 + a.window - 1, (long)len - 1);
+  const int r_lo = (p_lo - past) * a.G, r_hi = (p_hi - past + 1) * a.G - 1;
+  const int tiles = k0 < len && p_hi >= p_lo ? (r_hi - r_lo) / ROWS + 1 : 0;
+
+  const T* qp = static_cast<const T*>(a.q.p) + b * a.q.batch + kh * a.G * a.q.head;
+  const T* gp = static_cast<const T*>(a.dout.p) + b * a.dout.batch + kh * a.G * a.dout.head;
+  auto load = [&](int i) {
+    const int r0 = r_lo + i * ROWS, t0 = (int)fm_div(r0, a.by_g), stage = i % L::STAGES;
+    unsigned char* at = lds + stage * 2 * L::TILE;
+    auto offset = [&](const View& v) {
+      return [&, rs = (int)(v.row * (long)sizeof(T)), hs = (int)(v.head * (long)sizeof(T))](int u) {
+        const int r = r0 + u;
+        if (r > r_hi) return -1;
+        const int t = (int)fm_div(r, a.by_g);
+        return (t - t0) * rs + (r - t * a.G) * hs;
+      };
+    };
+    load_tile<T, DT, ROWS, 4>(qp + t0 * a.q.row, at, a.D, wave, lane, offset(a.q));
+    load_tile<T, DT, ROWS, 4>(gp + t0 * a.dout.row, at + L::TILE, a.D, wave, lane, offset(a.dout));
+    for (int u = threadIdx.x; u < ROWS; u += 256) {
+      const int r = min(r0 + u, r_hi), t = (int)fm_div(r, a.by_g);
+      const long at = ((long)b * a.T + t) * a.H + kh * a.G + (r - t * a.G);
+      const float lse = a.lse[at];
+      // Rows past the last, and rows without keys, take every probability as zero.
+      stat[stage][0][u] = r0 + u > r_hi || lse == -INFINITY ? INFINITY : lse;
+      stat[stage][1][u] = a.delta[at];
+      stat[stage][2][u] = __builtin_bit_cast(float, past + t);
+    }
+  };
+  if (tiles) load(0);
+  typename E::Frag kf[NS], vf[NS];
+  const int at_key = min(key, a.S - 1);
+  load_row<T, DT>(static_cast<const T*>(a.k.p) + b * a.k.batch + kh * a.k.head + at_key * a.k.row, live, a.D, lane, kf);
+  load_row<T, DT>(static_cast<const T*>(a.v.p) + b * a.v.batch + kh * a.v.head + at_key * a.v.row, live, a.D, lane, vf);
+
+  floatx16 ak[ND] = {}, av[ND] = {};
+  for (int i = 0; i < tiles; ++i) {
+    tile_barrier();
+    if (L::STAGES == 2 && i + 1 < tiles) load(i + 1);
+    const int stage = i % L::STAGES;
+    const unsigned char* qt = lds + stage * 2 * L::TILE;
+    const unsigned char* gt = qt + L::TILE;
+#pragma unroll
+    for (int nb = 0; nb < L::NB; ++nb) {
+      const int row = (wr * L::NB + nb) * 32, r0 = r_lo + i * ROWS + row;
+      if (r0 > r_hi) continue;
+      const int lo = past + (int)fm_div(r0, a.by_g), hi = past + (int)fm_div(min(r0 + 31, r_hi), a.by_g);
+      if (w0 > hi || w0 + 31 <= lo - a.window) continue;  // no row here sees these keys
+      floatx16 s = {}, dp = {};
+#pragma unroll
+      for (int c = 0; c < NS; ++c) s = E::mma(row_frag<T, DT>(qt, row, c, lane), kf[c], s);
+#pragma unroll
+      for (int c = 0; c < NS; ++c) dp = E::mma(row_frag<T, DT>(gt, row, c, lane), vf[c], dp);
+      const bool edge = w0 + 31 > lo || w0 <= hi - a.window;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const floatx4 lse = *reinterpret_cast<const floatx4*>(&stat[stage][0][row + 8 * g + 4 * half]);
+        const floatx4 delta = *reinterpret_cast<const floatx4*>(&stat[stage][1][row + 8 * g + 4 * half]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], a.scale2, -lse[e]));
+          s[4 * g + e] = p;
+          dp[4 * g + e] = p * (dp[4 * g + e] - delta[e]);
+        }
+      }
+      if (edge) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int p = __builtin_bit_cast(int, stat[stage][2][row + 8 * (e >> 2) + 4 * half + (e & 3)]);
+          const bool ok = key <= p && key > p - a.window;
+          s[e] = ok ? s[e] : 0.0f;
+          dp[e] = ok ? dp[e] : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 32 / E::STEP; ++c) {
+        const typename E::Frag p = E::pack(s, c), ds = E::pack(dp, c);
+        typename E::Frag f[ND];
+        col_frags<T, DT>(gt, row + c * E::STEP, lane, f);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) av[d] = E::mma(f[d], p, av[d]);
+        col_frags<T, DT>(qt, row + c * E::STEP, lane, f);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) ak[d] = E::mma(f[d], ds, ak[d]);
+      }
+    }
+    if (L::STAGES == 1 && i + 1 < tiles) {
+      tile_barrier();
+      load(i + 1);
+    }
+  }
+  constexpr int MINE = DT / 2 / WR;
+  const long row_index = ((long)b * a.S + key) * a.KV + kh;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    floatx16(&acc)[ND] = which ? av : ak;
+    float mine[MINE];
+    if constexpr (WR > 1) {
+      __syncthreads();
+      merge<DT, WR>(reinterpret_cast<float*>(lds), acc, wr, lane, mine);
+    } else {
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) mine[i] = acc[i / 16][i % 16];
+    }
+    if (key >= a.S) continue;
+    T* o = static_cast<T*>(which ? a.dv : a.dk) + row_index * a.D;
+    const float f = which ? 1.0f : a.scale;
+#pragma unroll
+    for (int i = 0; i < MINE; i += 4) {
+      const int e = wr * MINE + i, d = 32 * (e / 16) + 8 * (e % 16 / 4) + 4 * half;
+      if (d < a.D)  // padding takes no gradient
+        E::store4(o + d, live ? mine[i] * f : 0.0f, live ? mine[i + 1] * f : 0.0f, live ? mine[i + 2] * f : 0.0f,
+                  live ? mine[i + 3] * f : 0.0f);
+    }
+  }
+}
+
+enum { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };
+
+int check(const Attn& a, int dtype) {
+  if (a.B < 0 || a.T < 0 || a.S < 0 || a.H <= 0 || a.KV <= 0 || a.D <= 0 || a.window <= 0 || !(a.scale > 0.0f) ||
+      a.scale == INFINITY || a.H % a.KV || a.T > a.S || dtype < DT_F32 || dtype > DT_F16)
+    return FM_BAD_ARGUMENT;
+  const int unit = dtype == DT_F32 ? 4 : 8, size = dtype == DT_F32 ? 4 : 2;
+  if (a.D > 128 || a.D % unit) return FM_UNSUPPORTED;
+  if ((long)a.T * a.G >= INT_MAX - 256 || a.S >= INT_MAX - 256 || (long)a.B * a.KV >= INT_MAX) return FM_UNSUPPORTED;
+  if (((long)a.T * a.G + 31) / 32 > 65535 || (a.S + 31) / 32 > 65535) return FM_UNSUPPORTED;
+  for (const View* v : {&a.q, &a.k, &a.v, &a.dout}) {
+    if (!v->p) continue;
+    // 16-byte rows, and a tile's rows within reach of 32-bit offsets.
+    if ((reinterpret_cast<uintptr_t>(v->p) & 15) || v->batch % unit || v->row % unit || v->head % unit) return FM_UNSUPPORTED;
+    if (v->batch < 0 || v->row < 0 || v->head < 0) return FM_UNSUPPORTED;
+    if (v->row > INT_MAX / size / 256 || v->head > INT_MAX / size / 2 / a.G) return FM_UNSUPPORTED;
+  }
+  return FM_OK;
+}
+
+// Key splits of the forward: a call of few rows over many keys (single tokens)
+// has one block per 32 rows and key head; its keys are cut until some 512
+// blocks run, at least four tiles (of 128 keys) each.
+int forward_splits(const Attn& a) {
+  const long blocks = (long)a.B * a.KV * fm_ceil_div((long)a.T * a.G, 32);
+  const int tiles = fm_ceil_div(std::min<long>(a.S, (long)a.window + a.T - 1), 128);
+  return (int)std::max<long>(1, std::min<long>({tiles / 4, 512 / std::max<long>(blocks, 1), 64}));
+}
+
+// Whether the waves of a block take rows (or keys) of their own: enough blocks
+// of four times 32 to give every CU one.
+bool wide(const Attn& a, long rows) { return (long)a.B * a.KV * fm_ceil_div(rows, 128) >= 256; }
+
+size_t workspace_floats(const Attn& a, int splits) {
+  return splits > 1 ? (size_t)splits * a.B * a.KV * a.T * a.G * ((a.D > 64 ? 128 : 64) + 2) : 0;
+}
+
+template <typename T, int DT>
+int forward(const Attn& a, hipStream_t stream) {
+  const long rows = (long)a.T * a.G;
+  const unsigned seqs = (unsigned)(a.B * a.KV);
+  if (a.splits == 1 && wide(a, rows))
+    hipLaunchKernelGGL((attention_forward_kernel<T, DT, 4, 1>), dim3(seqs, fm_ceil_div(rows, 128)), dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((attention_forward_kernel<T, DT, 1, 4>), dim3(seqs, fm_ceil_div(rows, 32), a.splits), dim3(256), 0,
+                       stream, a);
+  if (a.splits > 1)
+    hipLaunchKernelGGL((attention_join_kernel<T, DT>), dim3(fm_ceil_div(seqs * rows, 4)), dim3(256), 0, stream, a);
+  return (int)hipGetLastError();
+}
+
+template <typename T, int DT>
+int backward(const Attn& a, hipStream_t stream) {
+  const long rows = (long)a.T * a.G;
+  const unsigned seqs = (unsigned)(a.B * a.KV);
+  if (rows > 0) {
+    if (wide(a, rows))
+      hipLaunchKernelGGL((attention_dq_kernel<T, DT, 4, 1>), dim3(seqs, fm_ceil_div(rows, 128)), dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL((attention_dq_kernel<T, DT, 1, 4>), dim3(seqs, fm_ceil_div(rows, 32)), dim3(256), 0, stream, a);
+  }
+  if (wide(a, a.S))
+    hipLaunchKernelGGL((attention_dkv_kernel<T, DT, 4, 1>), dim3(seqs, fm_ceil_div(a.S, 128)), dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((attention_dkv_kernel<T, DT, 1, 4>), dim3(seqs, fm_ceil_div(a.S, 32)), dim3(256), 0, stream, a);
+  return (int)hipGetLastError();
+}
+
+#define FM_ATTENTION_TYPES(run)                                            \
+  (dtype == DT_F32    ? (a.D > 64 ? run<float, 128>(a, stream) : run<float, 64>(a, stream))   \
+   : dtype == DT_BF16 ? (a.D > 64 ? run<__bf16, 128>(a, stream) : run<__bf16, 64>(a, stream)) \
+                      : (a.D > 64 ? run<_Float16, 128>(a, stream) : run<_Float16, 64>(a, stream)))
+
+Attn sizes(int batch, int queries, int keys, int heads, int kv_heads, int head_dim, int window, float scale) {
+  Attn a{};
+  a.B = batch, a.T = queries, a.S = keys, a.H = heads, a.KV = kv_heads, a.D = head_dim;
+  a.G = kv_heads > 0 && heads > 0 ? heads / kv_heads : 1;
+  a.window = window, a.scale = scale, a.scale2 = scale * LOG2E;
+  a.by_g = fm_divisor((unsigned)std::max(a.G, 1));
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fm_attention_forward_workspace_bytes(int batch, int queries, int keys, int heads, int kv_heads, int head_dim,
+                                            int window) {
+  const Attn a = sizes(batch, queries, keys, heads, kv_heads, head_dim, window, 1.0f);
+  if (check(a, DT_F32) != FM_OK && check(a, DT_BF16) != FM_OK) return 0;
+  if (batch == 0 || queries == 0) return 0;
+  return workspace_floats(a, forward_splits(a)) * sizeof(float);
+}
+
+int fm_attention_forward(const void* q, long q_batch, long q_row, long q_head, const void* k, long k_batch, long k_row,
+                         long k_head, const void* v, long v_batch, long v_row, long v_head, const int* lengths, int batch,
+                         int queries, int keys, int heads, int kv_heads, int head_dim, int window, float scale, int dtype,
+                         void* out, float* lse, float* workspace, size_t workspace_bytes, hipStream_t stream) {
+  Attn a = sizes(batch, queries, keys, heads, kv_heads, head_dim, window, scale);
+  a.q = View{q, q_batch, q_row, q_head}, a.k = View{k, k_batch, k_row, k_head}, a.v = View{v, v_batch, v_row, v_head};
+  a.lengths = lengths, a.out = out, a.lse = lse;
+  if (const int status = check(a, dtype)) return status;
+  if (batch == 0 || queries == 0) return FM_OK;
+  if (!q || !k || !v || !out || !lse) return FM_BAD_ARGUMENT;
+  if (reinterpret_cast<uintptr_t>(out) & 15) return FM_UNSUPPORTED;
+  a.splits = forward_splits(a);
+  if (a.splits > 1) {
+    const size_t need = workspace_floats(a, a.splits) * sizeof(float);
+    if (!workspace || workspace_bytes < need) return FM_WORKSPACE_TOO_SMALL;
+    if (reinterpret_cast<uintptr_t>(workspace) & 15) return FM_UNSUPPORTED;
+    a.part_o = workspace;
+    a.part_ml = workspace + (size_t)a.splits * a.B * a.KV * a.T * a.G * (a.D > 64 ? 128 : 64);
+  }
+  return FM_ATTENTION_TYPES(forward);
+}
+
+int fm_attention_backward(const void* dout, long dout_batch, long dout_row, long dout_head, const void* q, long q_batch,
+                          long q_row, long q_head, const void* k, long k_batch, long k_row, long k_head, const void* v,
+                          long v_batch, long v_row, long v_head, const void* out, const float* lse, const int* lengths,
+                          int batch, int queries, int keys, int heads, int kv_heads, int head_dim, int window, float scale,
+                          int dtype, void* dq, void* dk, void* dv, float* delta, hipStream_t stream) {
+  Attn a = sizes(batch, queries, keys, heads, kv_heads, head_dim, window, scale);
+  a.q = View{q, q_batch, q_row, q_head}, a.k = View{k, k_batch, k_row, k_head}, a.v = View{v, v_batch, v_row, v_head};
+  a.dout = View{dout, dout_batch, dout_row, dout_head};
+  a.o = out, a.lengths = lengths, a.lse = const_cast<float*>(lse);
+  a.out = dq, a.dk = dk, a.dv = dv, a.delta = delta, a.splits = 1;
+  if (const int status = check(a, dtype)) return status;
+  if (batch == 0 || keys == 0) return FM_OK;
+  if (!k || !v || !dk || !dv || (queries > 0 && (!dout || !q || !out || !lse || !dq || !delta))) return FM_BAD_ARGUMENT;
+  for (const void* p : {out, (const void*)dq, (const void*)dk, (const void*)dv})
+    if (reinterpret_cast<uintptr_t>(p) & 15) return FM_UNSUPPORTED;
+  return FM_ATTENTION_TYPES(backward);
+}
+
+}  // extern "C"

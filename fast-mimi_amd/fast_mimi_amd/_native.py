@@ -29,6 +29,9 @@ WEIGHTS_X6 = 64
 ACT_EXP = 128  # residual blocks: ELU as e^x - 1 (decoder-side calls)
 WEIGHTS_H3 = 512  # fp16 planes after the bf16 ones (decoder-side layers)
 
+# Element types of the training entry points (FM_DTYPE_*).
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+
 _STATUS = {1000: "bad argument", 1001: "workspace too small", 1002: "unsupported shape",
            1003: "input larger than the fixed scratch of an allocation-free entry point"}
 
@@ -91,6 +94,15 @@ _SIGNATURES = {
     "fm_conv_resblock64": ([_P, _I, _I, _P, _P, _P, _P, _P, _P, _I, _P, _P], _I),
     "fm_resblock64_conv_workspace_bytes": ([_I, _I], _S),
     "fm_resblock64_conv": ([_P, _I, _I, _P, _P, _P, _P, _I, _P, _P, _I, _P, _P, _S, _P], _I),
+    "fm_layer_norm_forward": ([_P, _L, _P, _P, _L, _I, _F, _I, _I, _P, _P, _P, _P], _I),
+    "fm_layer_norm_backward_workspace_bytes": ([_L, _I], _S),
+    "fm_layer_norm_backward": ([_P, _L, _P, _L, _P, _P, _P, _L, _I, _I, _I, _P, _P, _P, _P, _S, _P], _I),
+    "fm_attention_forward_workspace_bytes": ([_I, _I, _I, _I, _I, _I, _I], _S),
+    "fm_attention_forward": ([_P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P, _S, _P], _I),
+    "fm_attention_backward": ([_P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P, _P, _P], _I),
+    "fm_code_embedding": ([_P, _L, _L, _I, _I, _I, _P, _I, _I, _F, _I, _P, _P], _I),
+    "fm_code_embedding_backward_workspace_bytes": ([_I, _I, _I, _I, _I], _S),
+    "fm_code_embedding_backward": ([_P, _L, _P, _L, _L, _I, _I, _I, _I, _I, _F, _I, _P, _P, _S, _P], _I),
 }
 
 _lock = threading.Lock()

@@ -536,6 +536,111 @@ int fm_window_attention_stream(const float* qkv, int batch, int length, int head
 int fm_copy_buffers(const void* src0, void* dst0, size_t bytes0, const void* src1, void* dst1,
                     size_t bytes1, hipStream_t stream);
 
+/*
+ * Training.  These entry points take FP32, bfloat16 or float16 activations
+ * (dtype: FM_DTYPE_*); sums, statistics and softmax states are FP32, and each
+ * output is rounded once to its type.  No result depends on the order of
+ * atomics: the same call gives the same bits.
+ */
+enum { FM_DTYPE_F32 = 0, FM_DTYPE_BF16 = 1, FM_DTYPE_F16 = 2 };
+
+/*
+ * LayerNorm over the last dimension with the statistics its gradient needs:
+ * y = (x - mean) rstd gamma + beta, rstd = 1 / sqrt(biased variance + eps).
+ * x has rows of `channels` elements at a pitch of ld_x elements; y is
+ * contiguous; mean and rstd are [rows].  gamma / beta may be NULL (one /
+ * zero); weight_dtype is theirs: dtype, or FP32.
+ * Replaces nn.LayerNorm in MimiTransformerLayer (model.py:2028-2061) where
+ * the layer is trained.
+ */
+int fm_layer_norm_forward(const void* x, long ld_x, const void* gamma, const void* beta, long rows,
+                          int channels, float eps, int dtype, int weight_dtype, void* y,
+                          float* mean, float* rstd, hipStream_t stream);
+
+/*
+ * The gradients of fm_layer_norm_forward: with xh = (x - mean) rstd and
+ * g = dy gamma, dx = rstd (g - mean(g) - xh mean(g xh)), dgamma = the sum over
+ * rows of dy xh, dbeta = that of dy (both weight_dtype; NULL to leave them).
+ * dx is contiguous.  The workspace holds the row blocks' partial sums and is
+ * needed where dgamma or dbeta is given.
+ */
+size_t fm_layer_norm_backward_workspace_bytes(long rows, int channels);
+int fm_layer_norm_backward(const void* dy, long ld_dy, const void* x, long ld_x, const void* gamma,
+                           const float* mean, const float* rstd, long rows, int channels, int dtype,
+                           int weight_dtype, void* dx, void* dgamma, void* dbeta, float* workspace,
+                           size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * Causal sliding-window attention of queries [batch][queries][heads][head_dim]
+ * over keys and values [batch][keys][kv_heads][head_dim] (rotated already).
+ * Query t stands at position p = keys - queries + t (queries <= keys: those
+ * before are a cache) and sees key j iff p - window < j <= p and, with lengths
+ * (int [batch], NULL for whole sequences), p < lengths[b]: positions from
+ * lengths[b] on are padding, whose values are not used; padded queries give
+ * zeros.  heads is a multiple of kv_heads; query head h reads key head
+ * h / (heads / kv_heads).  q / k / v are strided (strides in elements of the
+ * batch, position and head dimensions; a packed projection is such a view);
+ * rows must be 16-byte aligned, head_dim <= 128 a multiple of 8 (FP32: 4),
+ * scale positive.  out [batch][queries][heads][head_dim] and lse
+ * [batch][queries][heads] (log2 of the row's sum of exponentials, -inf for a
+ * row without keys) are contiguous.  A visible key or value row that holds an
+ * infinity or NaN may reach other rows of its 32-row tiles.
+ * The workspace holds the parts of calls whose keys are split over blocks (few
+ * queries over many keys); NULL where its size is 0.
+ * Replaces F.scaled_dot_product_attention in MimiAttention.forward
+ * (model.py:1870-1961) with _attention_mask (model.py:1627-1688), padded
+ * batches and 16-bit types added.
+ */
+size_t fm_attention_forward_workspace_bytes(int batch, int queries, int keys, int heads,
+                                            int kv_heads, int head_dim, int window);
+int fm_attention_forward(const void* q, long q_batch, long q_row, long q_head, const void* k,
+                         long k_batch, long k_row, long k_head, const void* v, long v_batch,
+                         long v_row, long v_head, const int* lengths, int batch, int queries,
+                         int keys, int heads, int kv_heads, int head_dim, int window, float scale,
+                         int dtype, void* out, float* lse, float* workspace,
+                         size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * The gradients of fm_attention_forward (its arguments, out and lse), which
+ * forms the probabilities again.  dout is strided as q; dq, dk and dv are
+ * contiguous; delta [batch][queries][heads] is scratch (the rows' dout . out).
+ * Padding takes no gradient (zeros), and its dout is not used.
+ */
+int fm_attention_backward(const void* dout, long dout_batch, long dout_row, long dout_head,
+                          const void* q, long q_batch, long q_row, long q_head, const void* k,
+                          long k_batch, long k_row, long k_head, const void* v, long v_batch,
+                          long v_row, long v_head, const void* out, const float* lse,
+                          const int* lengths, int batch, int queries, int keys, int heads,
+                          int kv_heads, int head_dim, int window, float scale, int dtype, void* dq,
+                          void* dk, void* dv, float* delta, hipStream_t stream);
+
+/*
+ * Codebook embedding: out[b][t] = scale * sum over q of table[q][codes[b][q][t]],
+ * summed in the order of q.  codes are int64 at strides codes_batch and
+ * codes_book (elements; frames adjacent), table [books][entries][dim] and out
+ * [batch][frames][dim] contiguous, of dtype.  Code -1 is absent (adds
+ * nothing); any other code outside [0, entries) gives NaN, as in
+ * fm_rvq_decode.  At most 32768 entries.
+ * Replaces the codebook sum of MimiResidualVectorQuantizer.decode
+ * (model.py:2430-2444) where the codebooks are trained.
+ */
+int fm_code_embedding(const int64_t* codes, long codes_batch, long codes_book, int batch, int books,
+                      int frames, const void* table, int entries, int dim, float scale, int dtype,
+                      void* out, hipStream_t stream);
+
+/*
+ * Its gradient, by sorted codes: dtable[q][e] = scale * the sum, in order, of
+ * the rows (b, t) of dout whose code q is e (zero where there is none); codes
+ * outside [0, entries) take none.  dout has rows of dim elements at a pitch of
+ * ld_dout elements.
+ */
+size_t fm_code_embedding_backward_workspace_bytes(int batch, int books, int frames, int entries,
+                                                  int dim);
+int fm_code_embedding_backward(const void* dout, long ld_dout, const int64_t* codes,
+                               long codes_batch, long codes_book, int batch, int books, int frames,
+                               int entries, int dim, float scale, int dtype, void* dtable,
+                               void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
