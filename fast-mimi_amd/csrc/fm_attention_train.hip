@@ -31,6 +31,7 @@ typedef unsigned uintx2_v __attribute__((ext_vector_type(2)));
 typedef unsigned uintx4_v __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.44269504088896341f;
+constexpr float SLACK = 8.0f;
 
 template <typename T> struct Elem;
 template <> struct Elem<float> {
@@ -65,6 +66,13 @@ template <> struct Elem<__bf16> {
     for (int e = 0; e < 4; ++e) u[e] = two(p[8 * s + 2 * e], p[8 * s + 2 * e + 1]);
     return __builtin_bit_cast(Frag, u);
   }
+  // What pack(p, s) = f left of each value, rounded in its turn.
+  static FM_DEVICE Frag pack_rest(const floatx16& p, Frag f, int s) {
+    uintx4_v u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = two(p[8 * s + 2 * e] - (float)f[2 * e], p[8 * s + 2 * e + 1] - (float)f[2 * e + 1]);
+    return __builtin_bit_cast(Frag, u);
+  }
   static FM_DEVICE float dot(Frag a, Frag b, float s) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) s = fmaf((float)a[e], (float)b[e], s);
@@ -85,6 +93,13 @@ template <> struct Elem<_Float16> {
     uintx4_v u;
 #pragma unroll
     for (int e = 0; e < 4; ++e) u[e] = two(p[8 * s + 2 * e], p[8 * s + 2 * e + 1]);
+    return __builtin_bit_cast(Frag, u);
+  }
+  // What pack(p, s) = f left of each value, rounded in its turn.
+  static FM_DEVICE Frag pack_rest(const floatx16& p, Frag f, int s) {
+    uintx4_v u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = two(p[8 * s + 2 * e] - (float)f[2 * e], p[8 * s + 2 * e + 1] - (float)f[2 * e + 1]);
     return __builtin_bit_cast(Frag, u);
   }
   static FM_DEVICE float dot(Frag a, Frag b, float s) {
@@ -108,7 +123,7 @@ struct Attn {
   const void* o;  // backward: the forward's output, contiguous
   void *out, *dk, *dv;  // forward: O; backward: dQ in out
   float* lse;      // [B][T][H], log2 of the row's sum of exponentials
-  float* delta;    // [B][T][H], rowsum(dO O)
+  float* stats;    // [2][B][T][H]: lse, infinite for a row without keys; rowsum(dO O)
   float *part_o, *part_ml;  // split forward: unnormalised O [split][B][KV][R][DT], then (max, sum)
   const int* lengths;
   int B, T, S, H, KV, G, D, window, splits;
@@ -116,69 +131,93 @@ struct Attn {
   float scale, scale2;
 };
 
-// Tiles in LDS keep 16-byte chunk c of row r at chunk c ^ swz(r): eight rows
-// of one chunk (a fragment read) then lie in eight different chunk positions,
-// and four rows of a 64-byte column block (a transposed read) in all of them.
-FM_DEVICE int swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
-
-// 32 rows of an LDS tile as the A operand of a product over its columns:
-// lane l holds row l % 32, bytes 32 s + 16 (l / 32) .. + 15.
+// Tiles in LDS keep 16-byte chunk c of row r at chunk c ^ swz(r), such that both
+// reads below spread over all 64 banks (256 bytes): a fragment read takes the
+// same chunk of 16 rows at a time, a transposed 16-bit read 64 bytes of 4 rows,
+// an FP32 column read 128 bytes of two rows that lie 4 apart.
 template <typename T, int DT>
-FM_DEVICE typename Elem<T>::Frag row_frag(const unsigned char* tile, int row, int s, int lane) {
-  constexpr int PITCH = DT * (int)sizeof(T);
-  const int r = row + (lane & 31);
-  const int chunk = (2 * s + (lane >> 5)) ^ swz(r);
-  return __builtin_bit_cast(typename Elem<T>::Frag, *reinterpret_cast<const uintx4_v*>(tile + r * PITCH + chunk * 16));
+FM_DEVICE int swz(int row) {
+  if constexpr (sizeof(T) == 4) return ((row & 4) << 1) | ((row & 8) >> 1) | (row & 3);
+  else if constexpr (DT == 128) return ((row & 3) << 2) | ((row >> 2) & 3);
+  else return ((row & 2) << 1) | ((row & 4) >> 1) | ((row & 8) >> 3);  // two rows are 256 bytes
 }
 
-// Columns 0 .. DT - 1 of STEP rows as A operands (one per 32 columns) of a
-// product over the rows, in the order in which a lane holds a 32x32 result:
-// lane l holds column l % 32 of rows row + 8 i + 4 (l / 32) + 0..3.  16-bit
-// tiles use the LDS transpose read: each group of 16 lanes reads 4 rows x 16
-// columns, lane i gets column i.  Its builtin makes the compiler wait for the
-// next tile's copies too, so the reads and their wait are one asm block.  FP32
-// tiles read single values.
+// How lanes read a tile's operands.  With the swizzle an exclusive-or, every
+// address is one lane constant plus the tile's place, changed by constant bits:
+// the kernels keep two registers of addresses, not one per read (`fresh` keeps
+// the compiler from computing them all before the loop and holding them there).
 template <typename T, int DT>
-FM_DEVICE void col_frags(const unsigned char* tile, int row, int lane, typename Elem<T>::Frag (&f)[DT / 32]) {
-  constexpr int PITCH = DT * (int)sizeof(T);
-  if constexpr (sizeof(T) == 4) {
-    const int col = lane & 31;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = row + 4 * (lane >> 5) + e;
-      const unsigned char* at = tile + r * PITCH + (((col >> 2) ^ swz(r)) << 4) + (col & 3) * 4;
-#pragma unroll
-      for (int dt = 0; dt < DT / 32; ++dt) f[dt][e] = *reinterpret_cast<const float*>(at + 128 * dt);
-    }
-  } else {
-    const int r = row + 4 * (lane >> 5) + ((lane >> 2) & 3), low = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
-    // Column blocks 2 i and 2 i + 1 lie 64 bytes apart, in the order that the swizzle gives.
-    const unsigned char* base = tile + r * PITCH + (lane & 1) * 8;
-    const unsigned at0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)(base + ((low ^ swz(r)) << 4));
-    const unsigned at1 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)(base + (((4 + low) ^ swz(r)) << 4));
-    uintx2_v u[DT / 32][2];
-    if constexpr (DT == 64)
-      asm volatile(
-          "ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
-          "ds_read_b64_tr_b16 %2, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
-          "s_waitcnt lgkmcnt(0)"
-          : "=&v"(u[0][0]), "=&v"(u[0][1]), "=&v"(u[1][0]), "=&v"(u[1][1])
-          : "v"(at0), "v"(at1), "n"(8 * PITCH));
-    else
-      asm volatile(
-          "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%10\n\t"
-          "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%10\n\t"
-          "ds_read_b64_tr_b16 %4, %8 offset:128\n\tds_read_b64_tr_b16 %5, %8 offset:%11\n\t"
-          "ds_read_b64_tr_b16 %6, %9 offset:128\n\tds_read_b64_tr_b16 %7, %9 offset:%11\n\t"
-          "s_waitcnt lgkmcnt(0)"
-          : "=&v"(u[0][0]), "=&v"(u[0][1]), "=&v"(u[1][0]), "=&v"(u[1][1]), "=&v"(u[2][0]), "=&v"(u[2][1]),
-            "=&v"(u[3][0]), "=&v"(u[3][1])
-          : "v"(at0), "v"(at1), "n"(8 * PITCH), "n"(8 * PITCH + 128));
-#pragma unroll
-    for (int dt = 0; dt < DT / 32; ++dt)
-      f[dt] = __builtin_bit_cast(typename Elem<T>::Frag, (uintx4_v{u[dt][0][0], u[dt][0][1], u[dt][1][0], u[dt][1][1]}));
+struct Reads {
+  typedef typename Elem<T>::Frag Frag;
+  static constexpr int PITCH = DT * (int)sizeof(T);
+
+  static FM_DEVICE unsigned lds(const unsigned char* p) {
+    return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const unsigned char*)p;
   }
-}
+  static FM_DEVICE unsigned fresh(unsigned a) {
+    asm volatile("" : "+v"(a));
+    return a;
+  }
+
+  // 32 rows as the A or B operand of a product over their columns: lane l holds
+  // row l % 32, bytes 32 s + 16 (l / 32) .. + 15.
+  static FM_DEVICE unsigned row_lane(int lane) {
+    return (lane & 31) * PITCH + (((lane >> 5) ^ swz<T, DT>(lane & 31)) << 4);
+  }
+  static FM_DEVICE Frag row(unsigned a, int s) {
+    return __builtin_bit_cast(Frag, *(const __attribute__((address_space(3))) uintx4_v*)(a ^ (32 * s)));
+  }
+
+  // Columns 0 .. DT - 1 of STEP rows as A operands (one per 32 columns) of a
+  // product over the rows, in the order in which a lane holds a 32x32 result:
+  // lane l holds column l % 32 of rows 8 i + 4 (l / 32) + 0..3.  16-bit tiles use
+  // the LDS transpose read: each group of 16 lanes reads 4 rows x 16 columns,
+  // lane i gets column i.  Its builtin makes the compiler wait for the next
+  // tile's copies too, so the reads and their wait are one asm block.  FP32 tiles
+  // read single values.
+  static FM_DEVICE unsigned col_lane(int lane) {
+    const int half = lane >> 5;
+    if constexpr (sizeof(T) == 4)
+      return 4 * half * PITCH + ((((lane & 31) >> 2) ^ swz<T, DT>(4 * half)) << 4) + (lane & 3) * 4;
+    const int r = 4 * half + ((lane >> 2) & 3), chunk = 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+    return r * PITCH + ((chunk ^ swz<T, DT>(r)) << 4) + (lane & 1) * 8;
+  }
+  static FM_DEVICE void cols(unsigned a, int step, Frag (&f)[DT / 32]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int dt = 0; dt < DT / 32; ++dt)
+          f[dt][e] = *(const __attribute__((address_space(3))) float*)((a ^ ((swz<T, DT>(8 * step + e) ^ (8 * dt)) << 4)) +
+                                                                       (8 * step + e) * PITCH);
+    } else {
+      a += 16 * step * PITCH;
+      constexpr unsigned EIGHT = (DT == 128 ? 2 : 1) << 4;  // the swizzle of row r + 8 against row r's
+      uintx2_v u[DT / 32][2];
+      if constexpr (DT == 64)
+        asm volatile(
+            "ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %5 offset:%8\n\t"
+            "ds_read_b64_tr_b16 %2, %6\n\tds_read_b64_tr_b16 %3, %7 offset:%8\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(u[0][0]), "=&v"(u[0][1]), "=&v"(u[1][0]), "=&v"(u[1][1])
+            : "v"(a), "v"(a ^ EIGHT), "v"(a ^ 64), "v"(a ^ 64 ^ EIGHT), "n"(8 * PITCH));
+      else
+        asm volatile(
+            "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %9 offset:%16\n\t"
+            "ds_read_b64_tr_b16 %2, %10\n\tds_read_b64_tr_b16 %3, %11 offset:%16\n\t"
+            "ds_read_b64_tr_b16 %4, %12\n\tds_read_b64_tr_b16 %5, %13 offset:%16\n\t"
+            "ds_read_b64_tr_b16 %6, %14\n\tds_read_b64_tr_b16 %7, %15 offset:%16\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(u[0][0]), "=&v"(u[0][1]), "=&v"(u[1][0]), "=&v"(u[1][1]), "=&v"(u[2][0]), "=&v"(u[2][1]),
+              "=&v"(u[3][0]), "=&v"(u[3][1])
+            : "v"(a), "v"(a ^ EIGHT), "v"(a ^ 64), "v"(a ^ 64 ^ EIGHT), "v"(a ^ 128), "v"(a ^ 128 ^ EIGHT), "v"(a ^ 192),
+              "v"(a ^ 192 ^ EIGHT), "n"(8 * PITCH));
+#pragma unroll
+      for (int dt = 0; dt < DT / 32; ++dt)
+        f[dt] = __builtin_bit_cast(Frag, (uintx4_v{u[dt][0][0], u[dt][0][1], u[dt][1][0], u[dt][1][1]}));
+    }
+  }
+};
 
 // The B operand of one row straight from memory: chunk s of the lane's half,
 // zeros where the row is not live or the chunk lies past the head's width.
@@ -188,9 +227,51 @@ FM_DEVICE void load_row(const T* row, bool live, int D, int lane, typename Elem<
 #pragma unroll
   for (int s = 0; s < N; ++s) {
     const int d = (2 * s + (lane >> 5)) * E;
-    uintx4_v u{0, 0, 0, 0};
-    if (live && d < D) u = *reinterpret_cast<const uintx4_v*>(row + d);
+    const bool ok = live && d < D;  // the row itself is always one of the tensor's
+    uintx4_v u = *reinterpret_cast<const uintx4_v*>(row + (d < D ? d : 0));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u[e] = ok ? u[e] : 0;
     f[s] = __builtin_bit_cast(typename Elem<T>::Frag, u);
+  }
+}
+
+// Has the compiler wait for these loads here.  Where their first use is inside
+// a loop it would wait there in every turn, for the next tile's copies as well.
+template <typename F, int N>
+FM_DEVICE void arrive(F (&f)[N]) {
+#pragma unroll
+  for (int s = 0; s < N; ++s) asm volatile("" : "+v"(f[s]));
+}
+
+// s += 32 rows of a tile (lane address a) times B: a product over the head's
+// width.  The 16-bit forms read four steps' fragments before their products, so
+// that a wave does not wait for LDS at each (32 cycles do not cover a read);
+// FP32 products do.
+template <typename T, int DT, int N>
+FM_DEVICE void products(unsigned a, const typename Elem<T>::Frag (&b)[N], floatx16& s) {
+  typename Elem<T>::Frag f[N];
+  constexpr int AHEAD = 4;
+#pragma unroll
+  for (int c0 = 0; c0 < N; c0 += AHEAD) {
+#pragma unroll
+    for (int c = c0; c < c0 + AHEAD; ++c) f[c] = Reads<T, DT>::row(a, c);
+    if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int c = c0; c < c0 + AHEAD; ++c) s = Elem<T>::mma(f[c], b[c], s);
+  }
+}
+// The same with B in LDS as well.
+template <typename T, int DT, int N>
+FM_DEVICE void products(unsigned a, unsigned b, floatx16& s) {
+  typename Elem<T>::Frag f[N], g[N];
+  constexpr int AHEAD = 4;
+#pragma unroll
+  for (int c0 = 0; c0 < N; c0 += AHEAD) {
+#pragma unroll
+    for (int c = c0; c < c0 + AHEAD; ++c) f[c] = Reads<T, DT>::row(a, c), g[c] = Reads<T, DT>::row(b, c);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int c = c0; c < c0 + AHEAD; ++c) s = Elem<T>::mma(f[c], g[c], s);
   }
 }
 
@@ -205,15 +286,24 @@ FM_DEVICE void load_tile(const void* base, unsigned char* tile, int D, int wave,
 #pragma unroll
   for (int u = 0; u < INSTR / WAVES; ++u) {
     const int i = wave * (INSTR / WAVES) + u;
-    const int slot = i * 64 + lane, r = slot / CPR, chunk = (slot % CPR) ^ swz(r);
+    const int slot = i * 64 + lane, r = slot / CPR, chunk = (slot % CPR) ^ swz<T, DT>(r);
     const int off = offset(r);
     const bool ok = off >= 0 && chunk * 16 < D * (int)sizeof(T);
     fm_buf_load_lds16(buf, tile + i * 1024, ok ? off + chunk * 16 : INT_MIN, 0);
   }
 }
 
-// The sum or maximum of the two lane halves, in both.
-FM_DEVICE float other_half(float v) { return __shfl_xor(v, 32, 64); }
+// The sum or maximum of the two lane halves, in both (one register swap).
+FM_DEVICE float half_sum(float v) {
+  const unsigned u = __builtin_bit_cast(unsigned, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (unsigned)r[0]) + __builtin_bit_cast(float, (unsigned)r[1]);
+}
+FM_DEVICE float half_max(float v) {
+  const unsigned u = __builtin_bit_cast(unsigned, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
+}
 
 FM_DEVICE void tile_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -232,7 +322,8 @@ struct Rows {
     b = blockIdx.x / a.KV, kh = blockIdx.x - b * a.KV;
     len = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S;
     R = a.T * a.G;
-    const int r0 = blockIdx.y * 32 * WQ, past = a.S - a.T;
+    // The last rows see the most keys: they start first.
+    const int r0 = (gridDim.y - 1 - blockIdx.y) * 32 * WQ, past = a.S - a.T;
     const int w0 = min(r0 + 32 * wq, R - 1), w1 = min(r0 + 32 * wq + 31, R - 1);
     p_lo = past + (int)fm_div(w0, a.by_g);  // the wave's positions
     p_hi = min(past + (int)fm_div(w1, a.by_g), len - 1);
@@ -252,11 +343,12 @@ struct Rows {
   }
 };
 
-// O^T or dQ^T of four waves that each took a quarter of the keys, summed into
-// wave w's quarter of the registers; weight: the wave's own factor of its part.
+// O^T or dQ^T of the WK waves that shared rows but not keys, summed into their
+// WK-th parts of the registers each; own: which rows (0 .. 4 / WK - 1).
 template <int DT, int WK>
-FM_DEVICE void merge(float* lds, floatx16 (&acc)[DT / 32], int wk, int lane, float (&mine)[DT / 2 / WK]) {
+FM_DEVICE void merge(float* lds, floatx16 (&acc)[DT / 32], int own, int wk, int lane, float (&mine)[DT / 2 / WK]) {
   constexpr int N = DT / 2;
+  lds += own * WK * N * 64;
 #pragma unroll
   for (int i = 0; i < N; ++i) lds[(wk * N + i) * 64 + lane] = acc[i / 16][i % 16];
   __syncthreads();
@@ -269,13 +361,24 @@ FM_DEVICE void merge(float* lds, floatx16 (&acc)[DT / 32], int wk, int lane, flo
   }
 }
 
-template <typename T, int DT, int WQ, int WK>
+// Starts the copies of the keys and values k0 .. k_hi (at most KEYS) of a head.
+template <typename T, int DT, int KEYS, int WAVES = 4>
+FM_DEVICE void load_keys(const Attn& a, const T* kp, const T* vp, int k0, int k_hi, unsigned char* at, int wave, int lane) {
+  constexpr int TILE = KEYS * DT * (int)sizeof(T);
+  const int n = k_hi - k0, ks = (int)(a.k.row * (long)sizeof(T)), vs = (int)(a.v.row * (long)sizeof(T));
+  load_tile<T, DT, KEYS, WAVES>(kp + k0 * a.k.row, at, a.D, wave, lane, [&](int r) { return r <= n ? r * ks : -1; });
+  load_tile<T, DT, KEYS, WAVES>(vp + k0 * a.v.row, at + TILE, a.D, wave, lane, [&](int r) { return r <= n ? r * vs : -1; });
+}
+
+// KEEP: bytes of LDS that a dK / dV block keeps its keys and values in.
+template <typename T, int DT, int WQ, int WK, int KEEP = 0>
 struct Tiling {
   static constexpr int NB = WK > 1 || sizeof(T) == 4 ? 1 : 2;  // 32-key tiles of a wave
   static constexpr int KEYS = 32 * NB * WK;
   static constexpr int TILE = KEYS * DT * (int)sizeof(T);
-  static constexpr int STAGES = 4 * TILE <= 131072 ? 2 : 1;
-  static constexpr int LDS = 2 * STAGES * TILE;
+  static constexpr int STAGES = 4 * TILE <= 131072 && !KEEP ? 2 : 1;
+  static constexpr int MERGE = WK > 1 ? WQ * WK * DT * 128 : 0;  // room for the waves' results
+  static constexpr int LDS = std::max(KEEP + 2 * STAGES * TILE, MERGE);
   // Blocks per CU that the registers are held to.  At two (256 a lane) all of
   // them are vector registers and no result passes through accumulation
   // registers; the kernels that need more (HEAVY) run one block.
@@ -289,9 +392,13 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<false>
   typedef Elem<T> E;
   typedef Tiling<T, DT, WQ, WK> L;
   constexpr int NS = DT / E::STEP, ND = DT / 32;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[L::LDS];
+  // One array for all of the block's LDS: among several the compiler tells the
+  // direct copies' targets apart, and then waits for all copies at every read.
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[L::LDS + (WK > 1 ? 4 * 2 * 128 : 0)];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave % WQ, wk = wave / WQ, half = lane >> 5;
   const Rows<WQ> w(a, wq, lane);
+  typedef Reads<T, DT> R;
+  const unsigned row_lane = R::row_lane(lane), col_lane = R::col_lane(lane);
 
   typename E::Frag qf[NS];
   load_row<T, DT>(w.template of<T>(a.q) + w.t * a.q.row + (w.kh * a.G + (min(w.r, w.R - 1) - w.t * a.G)) * a.q.head, w.live,
@@ -308,14 +415,10 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<false>
   const T* kp = w.template of<T>(a.k) + w.kh * a.k.head;
   const T* vp = w.template of<T>(a.v) + w.kh * a.v.head;
   auto load = [&](int i) {
-    const int k0 = w.k_lo + i * L::KEYS, n = w.k_hi - k0;
-    unsigned char* at = lds + (i - first) % L::STAGES * 2 * L::TILE;
-    const int ks = (int)(a.k.row * (long)sizeof(T)), vs = (int)(a.v.row * (long)sizeof(T));
-    load_tile<T, DT, L::KEYS, 4>(kp + k0 * a.k.row, at, a.D, wave, lane, [&](int r) { return r <= n ? r * ks : -1; });
-    load_tile<T, DT, L::KEYS, 4>(vp + k0 * a.v.row, at + L::TILE, a.D, wave, lane,
-                                 [&](int r) { return r <= n ? r * vs : -1; });
+    load_keys<T, DT, L::KEYS>(a, kp, vp, w.k_lo + i * L::KEYS, w.k_hi, lds + (i - first) % L::STAGES * 2 * L::TILE, wave, lane);
   };
   if (first < tiles) load(first);
+  arrive(qf);
   for (int i = first; i < tiles; ++i) {
     tile_barrier();  // tile i is there, and every wave is past tile i - 1
     if (L::STAGES == 2 && i + 1 < tiles) load(i + 1);
@@ -326,8 +429,7 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<false>
       const int row = (wk * L::NB + nb) * 32, k0 = w.k_lo + i * L::KEYS + row;
       if (k0 > w.p_hi || k0 + 31 <= w.p_lo - a.window) continue;  // nothing that this wave sees
       floatx16 s = {};
-#pragma unroll
-      for (int c = 0; c < NS; ++c) s = E::mma(row_frag<T, DT>(kt, row, c, lane), qf[c], s);
+      products<T, DT>(R::fresh(R::lds(kt) + row * R::PITCH + row_lane), qf, s);
       if (k0 + 31 > w.p_lo || k0 <= w.p_hi - a.window || k0 + 31 > w.k_hi) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -338,8 +440,11 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<false>
       float top = s[0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) top = fmaxf(top, s[e]);
-      top = fmaxf(top, other_half(top)) * a.scale2;
-      if (__any(top > m)) {
+      top = half_max(top) * a.scale2;
+      // m is a reference, not the maximum itself: it follows once a score passes it
+      // by SLACK, so that the accumulators are rescaled a few times a row and not
+      // in most tiles.  Until then exponentials reach 2^SLACK, far from any limit.
+      if (__any(top > m + SLACK)) {
         const float up = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - (up == -INFINITY ? 0.0f : up));
         m = up;
         l *= f;
@@ -354,11 +459,12 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<false>
         s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -sub));
         l += s[e];
       }
+      const unsigned at = R::fresh(R::lds(vt) + row * R::PITCH + col_lane);
 #pragma unroll
       for (int c = 0; c < 32 / E::STEP; ++c) {
         const typename E::Frag p = E::pack(s, c);
         typename E::Frag f[ND];
-        col_frags<T, DT>(vt, row + c * E::STEP, lane, f);
+        R::cols(at, c, f);
 #pragma unroll
         for (int d = 0; d < ND; ++d) acc[d] = E::mma(f[d], p, acc[d]);
       }
@@ -368,13 +474,12 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<false>
       load(i + 1);
     }
   }
-  l += other_half(l);
+  l = half_sum(l);
 
   constexpr int MINE = DT / 2 / WK;
   float mine[MINE];
   if constexpr (WK > 1) {
-    __shared__ float ml[2][WK][32];
-    __syncthreads();
+    float(*ml)[WK][32] = reinterpret_cast<float(*)[WK][32]>(lds + L::LDS) + 2 * wq;
     if (half == 0) ml[0][wk][lane] = m, ml[1][wk][lane] = l;
     __syncthreads();
     const float own = m;
@@ -389,7 +494,7 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<false>
     for (int d = 0; d < ND; ++d)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[d][e] *= f;
-    merge<DT, WK>(reinterpret_cast<float*>(lds), acc, wk, lane, mine);
+    merge<DT, WK>(reinterpret_cast<float*>(lds), acc, wq, wk, lane, mine);
   } else {
 #pragma unroll
     for (int i = 0; i < MINE; ++i) mine[i] = acc[i / 16][i % 16];
@@ -449,25 +554,27 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Attn a) {
 }
 
 // dQ, and rowsum(dO O) for the dK / dV kernel: rows and keys as the forward.
+//
+// 16-bit inputs: dS is two 16-bit pieces here (a fourth product), as its own
+// rounding would put dQ at 1.5 times the error that rounding its result has.  And
+// rowsum(dO O) from the rounded O is only nearly the sum over P dP; the sum of dS,
+// zero but for that, puts it right for the dK / dV kernel.
 template <typename T, int DT, int WQ, int WK>
 __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<sizeof(T) == 4 && DT == 128>())) void attention_dq_kernel(Attn a) {
   typedef Elem<T> E;
   typedef Tiling<T, DT, WQ, WK> L;
   constexpr int NS = DT / E::STEP, ND = DT / 32;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[L::LDS];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[L::LDS + (WK > 1 ? 4 * 128 : 0)];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave % WQ, wk = wave / WQ, half = lane >> 5;
   const Rows<WQ> w(a, wq, lane);
+  typedef Reads<T, DT> R;
+  const unsigned row_lane = R::row_lane(lane), col_lane = R::col_lane(lane);
 
   const T* kp = w.template of<T>(a.k) + w.kh * a.k.head;
   const T* vp = w.template of<T>(a.v) + w.kh * a.v.head;
   const int tiles = w.k_hi >= w.k_lo ? (w.k_hi - w.k_lo) / L::KEYS + 1 : 0;
   auto load = [&](int i) {
-    const int k0 = w.k_lo + i * L::KEYS, n = w.k_hi - k0;
-    unsigned char* at = lds + i % L::STAGES * 2 * L::TILE;
-    const int ks = (int)(a.k.row * (long)sizeof(T)), vs = (int)(a.v.row * (long)sizeof(T));
-    load_tile<T, DT, L::KEYS, 4>(kp + k0 * a.k.row, at, a.D, wave, lane, [&](int r) { return r <= n ? r * ks : -1; });
-    load_tile<T, DT, L::KEYS, 4>(vp + k0 * a.v.row, at + L::TILE, a.D, wave, lane,
-                                 [&](int r) { return r <= n ? r * vs : -1; });
+    load_keys<T, DT, L::KEYS>(a, kp, vp, w.k_lo + i * L::KEYS, w.k_hi, lds + i % L::STAGES * 2 * L::TILE, wave, lane);
   };
   if (tiles) load(0);
 
@@ -478,14 +585,18 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<sizeof
   float delta = 0.0f;
 #pragma unroll
   for (int c = 0; c < NS; ++c) delta = E::dot(gf[c], qf[c], delta);
-  delta += other_half(delta);
+  delta = half_sum(delta);
   load_row<T, DT>(w.template of<T>(a.q) + w.t * a.q.row + head * a.q.head, w.live, a.D, lane, qf);
-  if (w.r < w.R && half == 0 && wk == 0) a.delta[w.row_index] = delta;
   // A row without keys takes every probability as zero.
   float lse = w.live ? a.lse[w.row_index] : INFINITY;
   lse = lse == -INFINITY ? INFINITY : lse;
+  float rest = 0.0f;  // the sum of dS: what the rounding of O took from delta
 
   floatx16 acc[ND] = {};
+  arrive(qf), arrive(gf);
+  float row_stats[2] = {lse, delta};
+  arrive(row_stats);
+  lse = row_stats[0], delta = row_stats[1];
   for (int i = 0; i < tiles; ++i) {
     tile_barrier();
     if (L::STAGES == 2 && i + 1 < tiles) load(i + 1);
@@ -496,10 +607,9 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<sizeof
       const int row = (wk * L::NB + nb) * 32, k0 = w.k_lo + i * L::KEYS + row;
       if (k0 > w.p_hi || k0 + 31 <= w.p_lo - a.window) continue;
       floatx16 s = {}, dp = {};
-#pragma unroll
-      for (int c = 0; c < NS; ++c) s = E::mma(row_frag<T, DT>(kt, row, c, lane), qf[c], s);
-#pragma unroll
-      for (int c = 0; c < NS; ++c) dp = E::mma(row_frag<T, DT>(vt, row, c, lane), gf[c], dp);
+      const unsigned at = R::fresh(R::lds(kt) + row * R::PITCH + row_lane);
+      products<T, DT>(at, qf, s);
+      products<T, DT>(at + L::TILE, gf, dp);
       const bool edge = k0 + 31 > w.p_lo || k0 <= w.p_hi - a.window || k0 + 31 > w.k_hi;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -514,10 +624,18 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<sizeof
         }
       }
 #pragma unroll
+      for (int e = 0; e < 16; ++e) rest += s[e];
+      const unsigned to = R::fresh(R::lds(kt) + row * R::PITCH + col_lane);
+#pragma unroll
       for (int c = 0; c < 32 / E::STEP; ++c) {
         const typename E::Frag ds = E::pack(s, c);
         typename E::Frag f[ND];
-        col_frags<T, DT>(kt, row + c * E::STEP, lane, f);
+        R::cols(to, c, f);
+        if constexpr (sizeof(T) == 2) {
+          const typename E::Frag low = E::pack_rest(s, ds, c);
+#pragma unroll
+          for (int d = 0; d < ND; ++d) acc[d] = E::mma(f[d], low, acc[d]);
+        }
 #pragma unroll
         for (int d = 0; d < ND; ++d) acc[d] = E::mma(f[d], ds, acc[d]);
       }
@@ -527,16 +645,26 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<sizeof
       load(i + 1);
     }
   }
+  rest = half_sum(rest);
   constexpr int MINE = DT / 2 / WK;
   float mine[MINE];
   if constexpr (WK > 1) {
+    float(*rests)[32] = reinterpret_cast<float(*)[32]>(lds + L::LDS) + WK * wq;
+    if (half == 0) rests[wk][lane] = rest;
     __syncthreads();
-    merge<DT, WK>(reinterpret_cast<float*>(lds), acc, wk, lane, mine);
+    rest = 0.0f;
+#pragma unroll
+    for (int u = 0; u < WK; ++u) rest += rests[u][lane & 31];
+    merge<DT, WK>(reinterpret_cast<float*>(lds), acc, wq, wk, lane, mine);
   } else {
 #pragma unroll
     for (int i = 0; i < MINE; ++i) mine[i] = acc[i / 16][i % 16];
   }
   if (w.r >= w.R) return;
+  if (half == 0 && wk == 0) {
+    a.stats[w.row_index] = lse;
+    a.stats[(long)a.B * a.T * a.H + w.row_index] = sizeof(T) == 2 ? delta + rest : delta;
+  }
   T* o = static_cast<T*>(a.out) + w.row_index * a.D;
 #pragma unroll
   for (int i = 0; i < MINE; i += 4) {
@@ -549,19 +677,39 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<sizeof
 }
 
 // dK and dV of 32 keys a wave over every row that sees them.  WK waves take 32
-// keys each and share the row tiles (many keys), or WR waves take the same 32
-// keys and a quarter of each row tile.
+// keys each and share the row tiles (many keys), WR waves take the same 32 keys
+// and a WR-th of each row tile.
+//
+// The keys and values stay in registers as operands, but for 16-bit heads of
+// 128: two accumulators of 64 registers each leave no room for them within the
+// 256 of two waves per SIMD, without which products, exponentials and LDS reads
+// follow one another.  Those blocks read them from LDS: four waves with two
+// blocks to a CU, or eight waves where that many blocks would all run at once and
+// the longest (the first keys of a sequence without a window) set the time.  2 x
+// 4095 positions, 16/4 heads: 740 us from registers, 540 / 404 from LDS with four
+// / eight waves; 16 heads x 2 x 2048: 190, 102 / 126.
+template <typename T, int DT>
+constexpr bool HELD = sizeof(T) == 2 && DT == 128;
+template <typename T, int DT, int WK>
+constexpr int HELD_BYTES = HELD<T, DT> ? 2 * 32 * WK * DT * 2 : 0;
+
 template <typename T, int DT, int WK, int WR>
-__global__ __launch_bounds__(256, (Tiling<T, DT, WK, WR>::template blocks<DT == 128>())) void attention_dkv_kernel(Attn a) {
+__global__ __launch_bounds__(64 * WK * WR,
+                             (HELD<T, DT> ? 2 : Tiling<T, DT, WK, WR>::template blocks<sizeof(T) == 4 && DT == 128>()))
+void attention_dkv_kernel(Attn a) {
   typedef Elem<T> E;
-  typedef Tiling<T, DT, WK, WR> L;  // rows in the place of keys
+  constexpr int KEEP = HELD_BYTES<T, DT, WK>, WAVES = WK * WR;
+  typedef Tiling<T, DT, WK, WR, KEEP> L;  // rows in the place of keys
   constexpr int NS = DT / E::STEP, ND = DT / 32, ROWS = L::KEYS;
-  __shared__ __attribute__((aligned(16))) unsigned char lds[L::LDS];
-  __shared__ __attribute__((aligned(16))) float stat[L::STAGES][3][ROWS];  // lse, delta, position (as an int)
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[L::LDS + L::STAGES * 2 * ROWS * 4];
+  float(*stat)[2][ROWS] = reinterpret_cast<float(*)[2][ROWS]>(lds + L::LDS);  // [stage]: lse, rowsum(dO O)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wk = wave % WK, wr = wave / WK, half = lane >> 5;
+  typedef Reads<T, DT> R;
+  const unsigned row_lane = R::row_lane(lane), col_lane = R::col_lane(lane);
   const int b = blockIdx.x / a.KV, kh = blockIdx.x - b * a.KV;
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S, past = a.S - a.T;
-  const int k0 = blockIdx.y * 32 * WK, w0 = k0 + 32 * wk, key = w0 + (lane & 31);
+  // The first keys are seen by the most rows and start first.
+  const int k0 = (int)blockIdx.y * 32 * WK, w0 = k0 + 32 * wk, key = w0 + (lane & 31);
   const bool live = key < len;
   // Rows of the positions that see any of the block's keys.
   const int p_lo = max(k0, past);
@@ -573,7 +721,7 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WK, WR>::template blocks<DT == 
   const T* gp = static_cast<const T*>(a.dout.p) + b * a.dout.batch + kh * a.G * a.dout.head;
   auto load = [&](int i) {
     const int r0 = r_lo + i * ROWS, t0 = (int)fm_div(r0, a.by_g), stage = i % L::STAGES;
-    unsigned char* at = lds + stage * 2 * L::TILE;
+    unsigned char* at = lds + KEEP + stage * 2 * L::TILE;
     auto offset = [&](const View& v) {
       return [&, rs = (int)(v.row * (long)sizeof(T)), hs = (int)(v.head * (long)sizeof(T))](int u) {
         const int r = r0 + u;
@@ -582,31 +730,42 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WK, WR>::template blocks<DT == 
         return (t - t0) * rs + (r - t * a.G) * hs;
       };
     };
-    load_tile<T, DT, ROWS, 4>(qp + t0 * a.q.row, at, a.D, wave, lane, offset(a.q));
-    load_tile<T, DT, ROWS, 4>(gp + t0 * a.dout.row, at + L::TILE, a.D, wave, lane, offset(a.dout));
-    for (int u = threadIdx.x; u < ROWS; u += 256) {
-      const int r = min(r0 + u, r_hi), t = (int)fm_div(r, a.by_g);
-      const long at = ((long)b * a.T + t) * a.H + kh * a.G + (r - t * a.G);
-      const float lse = a.lse[at];
-      // Rows past the last, and rows without keys, take every probability as zero.
-      stat[stage][0][u] = r0 + u > r_hi || lse == -INFINITY ? INFINITY : lse;
-      stat[stage][1][u] = a.delta[at];
-      stat[stage][2][u] = __builtin_bit_cast(float, past + t);
+    load_tile<T, DT, ROWS, WAVES>(qp + t0 * a.q.row, at, a.D, wave, lane, offset(a.q));
+    load_tile<T, DT, ROWS, WAVES>(gp + t0 * a.dout.row, at + L::TILE, a.D, wave, lane, offset(a.dout));
+    // The rows' statistics, by direct copies as well: a value that passed through
+    // registers would make this tile's copies be waited for.  A row past the last
+    // reads zeros, which its zero operands leave without effect.
+    const long first = ((long)b * a.T + t0) * a.H + kh * a.G;
+    constexpr int CHUNKS = ROWS < 64 ? 1 : ROWS / 64;  // of 64 rows, or one of 32
+    for (int u = wave; u < 2 * CHUNKS; u += WAVES) {
+      const int which = u / CHUNKS, v = u % CHUNKS * 64 + lane, r = r0 + v, t = (int)fm_div(r, a.by_g);
+      if (v < ROWS)
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            fm_buffer(a.stats + which * ((long)a.B * a.T * a.H) + first, INT_MAX),
+            (__attribute__((address_space(3))) void*)&stat[stage][which][u % CHUNKS * 64], 4,
+            r <= r_hi ? ((t - t0) * a.H + r - t * a.G) * 4 : INT_MIN, 0, 0, 0);
     }
   };
-  if (tiles) load(0);
+  // From the last rows back: every block of a head sees those, so blocks that run
+  // at the same time read the same rows.
+  if (tiles) load(tiles - 1);
   typename E::Frag kf[NS], vf[NS];
   const int at_key = min(key, a.S - 1);
-  load_row<T, DT>(static_cast<const T*>(a.k.p) + b * a.k.batch + kh * a.k.head + at_key * a.k.row, live, a.D, lane, kf);
-  load_row<T, DT>(static_cast<const T*>(a.v.p) + b * a.v.batch + kh * a.v.head + at_key * a.v.row, live, a.D, lane, vf);
-
+  const T* kp = static_cast<const T*>(a.k.p) + b * a.k.batch + kh * a.k.head;
+  const T* vp = static_cast<const T*>(a.v.p) + b * a.v.batch + kh * a.v.head;
+  if constexpr (KEEP > 0) {
+    load_keys<T, DT, 32 * WK, WAVES>(a, kp, vp, k0, min(len, k0 + 32 * WK) - 1, lds, wave, lane);
+  } else {
+    load_row<T, DT>(kp + at_key * a.k.row, live, a.D, lane, kf);
+    load_row<T, DT>(vp + at_key * a.v.row, live, a.D, lane, vf);
+    arrive(kf), arrive(vf);
+  }
   floatx16 ak[ND] = {}, av[ND] = {};
-  for (int i = 0; i < tiles; ++i) {
+  for (int i = tiles - 1; i >= 0; --i) {
     tile_barrier();
-    if (L::STAGES == 2 && i + 1 < tiles) load(i + 1);
+    if (L::STAGES == 2 && i > 0) load(i - 1);
     const int stage = i % L::STAGES;
-    const unsigned char* qt = lds + stage * 2 * L::TILE;
-    const unsigned char* gt = qt + L::TILE;
+    const unsigned char* qt = lds + KEEP + stage * 2 * L::TILE;
 #pragma unroll
     for (int nb = 0; nb < L::NB; ++nb) {
       const int row = (wr * L::NB + nb) * 32, r0 = r_lo + i * ROWS + row;
@@ -614,10 +773,15 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WK, WR>::template blocks<DT == 
       const int lo = past + (int)fm_div(r0, a.by_g), hi = past + (int)fm_div(min(r0 + 31, r_hi), a.by_g);
       if (w0 > hi || w0 + 31 <= lo - a.window) continue;  // no row here sees these keys
       floatx16 s = {}, dp = {};
-#pragma unroll
-      for (int c = 0; c < NS; ++c) s = E::mma(row_frag<T, DT>(qt, row, c, lane), kf[c], s);
-#pragma unroll
-      for (int c = 0; c < NS; ++c) dp = E::mma(row_frag<T, DT>(gt, row, c, lane), vf[c], dp);
+      const unsigned at = R::fresh(R::lds(qt) + row * R::PITCH + row_lane);
+      if constexpr (KEEP > 0) {
+        const unsigned held = R::fresh(R::lds(lds) + 32 * wk * R::PITCH + row_lane);
+        products<T, DT, NS>(at, held, s);
+        products<T, DT, NS>(at + L::TILE, held + KEEP / 2, dp);
+      } else {
+        products<T, DT>(at, kf, s);
+        products<T, DT>(at + L::TILE, vf, dp);
+      }
       const bool edge = w0 + 31 > lo || w0 <= hi - a.window;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
@@ -633,27 +797,28 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WK, WR>::template blocks<DT == 
       if (edge) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int p = __builtin_bit_cast(int, stat[stage][2][row + 8 * (e >> 2) + 4 * half + (e & 3)]);
+          const int p = past + (int)fm_div(r0 + 8 * (e >> 2) + 4 * half + (e & 3), a.by_g);
           const bool ok = key <= p && key > p - a.window;
           s[e] = ok ? s[e] : 0.0f;
           dp[e] = ok ? dp[e] : 0.0f;
         }
       }
+      const unsigned to = R::fresh(R::lds(qt) + row * R::PITCH + col_lane);
 #pragma unroll
       for (int c = 0; c < 32 / E::STEP; ++c) {
         const typename E::Frag p = E::pack(s, c), ds = E::pack(dp, c);
         typename E::Frag f[ND];
-        col_frags<T, DT>(gt, row + c * E::STEP, lane, f);
+        R::cols(to + L::TILE, c, f);
 #pragma unroll
         for (int d = 0; d < ND; ++d) av[d] = E::mma(f[d], p, av[d]);
-        col_frags<T, DT>(qt, row + c * E::STEP, lane, f);
+        R::cols(to, c, f);
 #pragma unroll
         for (int d = 0; d < ND; ++d) ak[d] = E::mma(f[d], ds, ak[d]);
       }
     }
-    if (L::STAGES == 1 && i + 1 < tiles) {
+    if (L::STAGES == 1 && i > 0) {
       tile_barrier();
-      load(i + 1);
+      load(i - 1);
     }
   }
   constexpr int MINE = DT / 2 / WR;
@@ -664,7 +829,7 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WK, WR>::template blocks<DT == 
     float mine[MINE];
     if constexpr (WR > 1) {
       __syncthreads();
-      merge<DT, WR>(reinterpret_cast<float*>(lds), acc, wr, lane, mine);
+      merge<DT, WR>(reinterpret_cast<float*>(lds), acc, wk, wr, lane, mine);
     } else {
 #pragma unroll
       for (int i = 0; i < MINE; ++i) mine[i] = acc[i / 16][i % 16];
@@ -711,42 +876,48 @@ int forward_splits(const Attn& a) {
   return (int)std::max<long>(1, std::min<long>({tiles / 4, 512 / std::max<long>(blocks, 1), 64}));
 }
 
-// Whether the waves of a block take rows (or keys) of their own: enough blocks
-// of four times 32 to give every CU one.
-bool wide(const Attn& a, long rows) { return (long)a.B * a.KV * fm_ceil_div(rows, 128) >= 256; }
+// How many of a block's four waves take rows (or keys) of their own, the rest
+// sharing them: four where that leaves about three blocks a CU, two where one
+// is left for each, else one.
+int own_waves(const Attn& a, long rows) {
+  const long seqs = (long)a.B * a.KV;
+  return seqs * fm_ceil_div(rows, 128) >= 768 ? 4 : seqs * fm_ceil_div(rows, 64) >= 256 ? 2 : 1;
+}
 
 size_t workspace_floats(const Attn& a, int splits) {
   return splits > 1 ? (size_t)splits * a.B * a.KV * a.T * a.G * ((a.D > 64 ? 128 : 64) + 2) : 0;
 }
 
+#define FM_ATTENTION_LAUNCH(kernel, own, rows, z)                                                       \
+  do {                                                                                                  \
+    const dim3 grid((unsigned)(a.B * a.KV), fm_ceil_div(rows, 32 * (own)), z);                          \
+    if ((own) == 4) hipLaunchKernelGGL((kernel<T, DT, 4, 1>), grid, dim3(256), 0, stream, a);           \
+    else if ((own) == 2) hipLaunchKernelGGL((kernel<T, DT, 2, 2>), grid, dim3(256), 0, stream, a);      \
+    else hipLaunchKernelGGL((kernel<T, DT, 1, 4>), grid, dim3(256), 0, stream, a);                      \
+  } while (0)
+
 template <typename T, int DT>
 int forward(const Attn& a, hipStream_t stream) {
   const long rows = (long)a.T * a.G;
-  const unsigned seqs = (unsigned)(a.B * a.KV);
-  if (a.splits == 1 && wide(a, rows))
-    hipLaunchKernelGGL((attention_forward_kernel<T, DT, 4, 1>), dim3(seqs, fm_ceil_div(rows, 128)), dim3(256), 0, stream, a);
-  else
-    hipLaunchKernelGGL((attention_forward_kernel<T, DT, 1, 4>), dim3(seqs, fm_ceil_div(rows, 32), a.splits), dim3(256), 0,
-                       stream, a);
+  const int waves = a.splits > 1 ? 1 : own_waves(a, rows);
+  FM_ATTENTION_LAUNCH(attention_forward_kernel, waves, rows, a.splits);
   if (a.splits > 1)
-    hipLaunchKernelGGL((attention_join_kernel<T, DT>), dim3(fm_ceil_div(seqs * rows, 4)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((attention_join_kernel<T, DT>), dim3(fm_ceil_div(a.B * a.KV * rows, 4)), dim3(256), 0, stream, a);
   return (int)hipGetLastError();
 }
 
 template <typename T, int DT>
 int backward(const Attn& a, hipStream_t stream) {
   const long rows = (long)a.T * a.G;
-  const unsigned seqs = (unsigned)(a.B * a.KV);
-  if (rows > 0) {
-    if (wide(a, rows))
-      hipLaunchKernelGGL((attention_dq_kernel<T, DT, 4, 1>), dim3(seqs, fm_ceil_div(rows, 128)), dim3(256), 0, stream, a);
-    else
-      hipLaunchKernelGGL((attention_dq_kernel<T, DT, 1, 4>), dim3(seqs, fm_ceil_div(rows, 32)), dim3(256), 0, stream, a);
+  if (rows > 0) FM_ATTENTION_LAUNCH(attention_dq_kernel, own_waves(a, rows), rows, 1);
+  const int own = own_waves(a, a.S);
+  if constexpr (HELD<T, DT>) {
+    const dim3 grid((unsigned)(a.B * a.KV), fm_ceil_div(a.S, 64));
+    if ((long)grid.x * grid.y > 512) hipLaunchKernelGGL((attention_dkv_kernel<T, DT, 2, 2>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((attention_dkv_kernel<T, DT, 2, 4>), grid, dim3(512), 0, stream, a);
+  } else {
+    FM_ATTENTION_LAUNCH(attention_dkv_kernel, own, a.S, 1);
   }
-  if (wide(a, a.S))
-    hipLaunchKernelGGL((attention_dkv_kernel<T, DT, 4, 1>), dim3(seqs, fm_ceil_div(a.S, 128)), dim3(256), 0, stream, a);
-  else
-    hipLaunchKernelGGL((attention_dkv_kernel<T, DT, 1, 4>), dim3(seqs, fm_ceil_div(a.S, 32)), dim3(256), 0, stream, a);
   return (int)hipGetLastError();
 }
 
@@ -802,15 +973,15 @@ int fm_attention_backward(const void* dout, long dout_batch, long dout_row, long
                           long q_row, long q_head, const void* k, long k_batch, long k_row, long k_head, const void* v,
                           long v_batch, long v_row, long v_head, const void* out, const float* lse, const int* lengths,
                           int batch, int queries, int keys, int heads, int kv_heads, int head_dim, int window, float scale,
-                          int dtype, void* dq, void* dk, void* dv, float* delta, hipStream_t stream) {
+                          int dtype, void* dq, void* dk, void* dv, float* stats, hipStream_t stream) {
   Attn a = sizes(batch, queries, keys, heads, kv_heads, head_dim, window, scale);
   a.q = View{q, q_batch, q_row, q_head}, a.k = View{k, k_batch, k_row, k_head}, a.v = View{v, v_batch, v_row, v_head};
   a.dout = View{dout, dout_batch, dout_row, dout_head};
   a.o = out, a.lengths = lengths, a.lse = const_cast<float*>(lse);
-  a.out = dq, a.dk = dk, a.dv = dv, a.delta = delta, a.splits = 1;
+  a.out = dq, a.dk = dk, a.dv = dv, a.stats = stats, a.splits = 1;
   if (const int status = check(a, dtype)) return status;
   if (batch == 0 || keys == 0) return FM_OK;
-  if (!k || !v || !dk || !dv || (queries > 0 && (!dout || !q || !out || !lse || !dq || !delta))) return FM_BAD_ARGUMENT;
+  if (!k || !v || !dk || !dv || (queries > 0 && (!dout || !q || !out || !lse || !dq || !stats))) return FM_BAD_ARGUMENT;
   for (const void* p : {out, (const void*)dq, (const void*)dk, (const void*)dv})
     if (reinterpret_cast<uintptr_t>(p) & 15) return FM_UNSUPPORTED;
   return FM_ATTENTION_TYPES(backward);

@@ -60,7 +60,7 @@ SPECS = {
     "fm_layer_norm_forward": "in:x i:ld_x in:gamma in:beta i:rows i:channels f:eps i:dtype i:weight_dtype out:y out:mean out:rstd",
     "fm_layer_norm_backward": "in:dy i:ld_dy in:x i:ld_x in:gamma in:mean in:rstd i:rows i:channels i:dtype i:weight_dtype out:dx out:dgamma out:dbeta out:workspace i:workspace_bytes",
     "fm_attention_forward": "in:q i:q_batch i:q_row i:q_head in:k i:k_batch i:k_row i:k_head in:v i:v_batch i:v_row i:v_head in:lengths i:batch i:queries i:keys i:heads i:kv_heads i:head_dim i:window f:scale i:dtype out:out out:lse out:workspace i:workspace_bytes",
-    "fm_attention_backward": "in:dout i:dout_batch i:dout_row i:dout_head in:q i:q_batch i:q_row i:q_head in:k i:k_batch i:k_row i:k_head in:v i:v_batch i:v_row i:v_head in:out in:lse in:lengths i:batch i:queries i:keys i:heads i:kv_heads i:head_dim i:window f:scale i:dtype out:dq out:dk out:dv out:delta",
+    "fm_attention_backward": "in:dout i:dout_batch i:dout_row i:dout_head in:q i:q_batch i:q_row i:q_head in:k i:k_batch i:k_row i:k_head in:v i:v_batch i:v_row i:v_head in:out in:lse in:lengths i:batch i:queries i:keys i:heads i:kv_heads i:head_dim i:window f:scale i:dtype out:dq out:dk out:dv out:stats",
     "fm_code_embedding": "in:codes i:codes_batch i:codes_book i:batch i:books i:frames in:table i:entries i:dim f:scale i:dtype out:out",
     "fm_code_embedding_backward": "in:dout i:ld_dout in:codes i:codes_batch i:codes_book i:batch i:books i:frames i:entries i:dim f:scale i:dtype out:dtable out:workspace i:workspace_bytes",
 }

@@ -337,10 +337,10 @@ def window_attention_backward(grad, q, k, v, out, lse, window: int | None = None
         if t == 0:
             return dq, dk.zero_(), dv.zero_()
         out = _heads(out.contiguous())[0]
-        delta = torch.empty((b, t, h), device=device)
+        stats = torch.empty((2, b, t, h), device=device)
         with _on(device):
             ops.call("fm_attention_backward", *_heads(grad, h // kv), *_heads(q, h // kv), *_heads(k), *_heads(v), out, lse,
-                     lengths, b, t, s, h, kv, d, window, scale, _DTYPES[q.dtype], dq, dk, dv, delta)
+                     lengths, b, t, s, h, kv, d, window, scale, _DTYPES[q.dtype], dq, dk, dv, stats)
     return dq, dk, dv
 
 

@@ -603,7 +603,8 @@ int fm_attention_forward(const void* q, long q_batch, long q_row, long q_head, c
 /*
  * The gradients of fm_attention_forward (its arguments, out and lse), which
  * forms the probabilities again.  dout is strided as q; dq, dk and dv are
- * contiguous; delta [batch][queries][heads] is scratch (the rows' dout . out).
+ * contiguous; stats [2][batch][queries][heads] is scratch (the rows' lse and
+ * dout . out).
  * Padding takes no gradient (zeros), and its dout is not used.
  */
 int fm_attention_backward(const void* dout, long dout_batch, long dout_row, long dout_head,
@@ -612,7 +613,7 @@ int fm_attention_backward(const void* dout, long dout_batch, long dout_row, long
                           long v_row, long v_head, const void* out, const float* lse,
                           const int* lengths, int batch, int queries, int keys, int heads,
                           int kv_heads, int head_dim, int window, float scale, int dtype, void* dq,
-                          void* dk, void* dv, float* delta, hipStream_t stream);
+                          void* dk, void* dv, float* stats, hipStream_t stream);
 
 /*
  * Codebook embedding: out[b][t] = scale * sum over q of table[q][codes[b][q][t]],

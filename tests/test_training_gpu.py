@@ -170,7 +170,8 @@ def test_attention(shape, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("b,t,h,kv,d,window", [(40, 160, 8, 8, 64, 90), (20, 140, 16, 8, 128, None)])
+@pytest.mark.parametrize("b,t,h,kv,d,window", [(40, 160, 8, 8, 64, 90), (20, 140, 16, 8, 128, None), (24, 140, 16, 16, 64, 60),
+                                               (50, 70, 32, 16, 128, None), (70, 260, 8, 4, 64, None)])
 def test_attention_many_blocks(b, t, h, kv, d, window, dtype):
     """Enough heads that each wave has rows (and keys) of its own; a few of the
     clips are compared, the others against the same clips alone."""
