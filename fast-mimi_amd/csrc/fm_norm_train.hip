@@ -291,11 +291,13 @@ Plan plan(int C, int size, bool aligned) {
   return {e, 0, 64};
 }
 
+constexpr int ONE_BLOCK = 8;  // rows of a group that are left to one block
+
 // Backward blocks: enough to fill the chip (four to a CU), each with at least
 // two rows per group, and one alone (no second launch) for a handful of rows.
 int backward_blocks(long rows, const Plan& p) {
   const int groups = p.nv ? 256 / p.lpr : 1;
-  if (p.nv && rows <= 8 * groups) return 1;
+  if (p.nv && rows <= ONE_BLOCK * groups) return 1;
   return (int)std::max<long>(1, std::min<long>(1024, (rows + 2 * groups - 1) / (2 * groups)));
 }
 
@@ -379,9 +381,10 @@ int fm_layer_norm_forward(const void* x, long ld_x, const void* gamma, const voi
   return run_types(a, dtype, weight_dtype, false, stream);
 }
 
-// Room for the most blocks that any alignment of the same call runs.
+// Room for the most blocks that any alignment of the same call runs; none where
+// each of its plans is one block.
 size_t fm_layer_norm_backward_workspace_bytes(long rows, int channels) {
-  if (rows <= 0 || channels <= 0) return 0;
+  if (rows <= 0 || channels <= 0 || (channels <= 64 * 32 && rows <= ONE_BLOCK * 4)) return 0;
   return (size_t)std::min<long>(1024, rows) * 2 * channels * sizeof(float);
 }
 
@@ -396,8 +399,9 @@ int fm_layer_norm_backward(const void* dy, long ld_dy, const void* x, long ld_x,
   if (rows == 0 && !dgamma && !dbeta) return FM_OK;
   if (rows > 0 && (!x || !dy || !dx || !mean || !rstd)) return FM_BAD_ARGUMENT;
   if (rows > 0 && (dgamma || dbeta) &&
-      (!workspace || workspace_bytes < fm_layer_norm_backward_workspace_bytes(rows, channels)))
+      workspace_bytes < fm_layer_norm_backward_workspace_bytes(rows, channels))
     return FM_WORKSPACE_TOO_SMALL;
+  if (workspace_bytes > 0 && !workspace) return FM_BAD_ARGUMENT;
   return run_types(a, dtype, weight_dtype, true, stream);
 }
 

@@ -53,34 +53,39 @@ def _tensor(name: str, t, dtypes=tuple(_DTYPES)) -> torch.Tensor:
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}, got {t.dtype}")
-    t = t.detach() if t.requires_grad else t
+    if t.requires_grad:
+        t = t.detach()
     return t.resolve_neg() if t.is_neg() else t
 
 
 def _on_gpu(**tensors) -> torch.device:
-    """The one GPU that all of the tensors are on."""
-    device = next(iter(tensors.values())).device
+    """The one GPU that all of the tensors (those that are given) are on."""
+    device = None
     for name, t in tensors.items():
-        if t.device.type != "cuda":
-            raise ValueError(f"{name} must be on a ROCm GPU, got {t.device}")
+        if t is None:
+            continue
         if t.device != device:
-            raise ValueError(f"{name} is on {t.device}, the other inputs on {device}")
+            if t.device.type != "cuda":
+                raise ValueError(f"{name} must be on a ROCm GPU, got {t.device}")
+            if device is not None:
+                raise ValueError(f"{name} is on {t.device}, the other inputs on {device}")
+            device = t.device
     return device
 
 
-class _on:
-    """Kernels are launched with their tensors' device as the current one."""
+def _run(device: torch.device, entry: str, *args) -> None:
+    """The entry point, with its tensors' device as the current one."""
+    if device.index == torch.cuda.current_device():
+        ops.call(entry, *args)
+    else:
+        with torch.cuda.device(device):
+            ops.call(entry, *args)
 
-    def __init__(self, device: torch.device) -> None:
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
-    def __enter__(self) -> None:
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc) -> None:
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _scratch(like: torch.Tensor, entry: str, *args) -> tuple[torch.Tensor | None, int]:
+    """Workspace for a call: what its size query asks for."""
+    size = getattr(nat.library(), entry)(*args)
+    return (like.new_empty((size + 3) // 4, dtype=torch.float32) if size else None), size
 
 
 def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
@@ -169,15 +174,16 @@ def layer_norm_forward(x, weight=None, bias=None, eps: float = 1e-5):
     x, weight, bias, wtype = _norm_input(x, weight, bias)
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    device = _on_gpu(**{n: t for n, t in (("x", x), ("weight", weight), ("bias", bias)) if t is not None})
+    device = _on_gpu(x=x, weight=weight, bias=bias)
     x, pitch = _rows(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
-    mean = torch.empty(x.shape[:-1], device=device)
-    rstd = torch.empty(x.shape[:-1], device=device)
-    if x.numel():
-        with _on(device):
-            ops.call("fm_layer_norm_forward", x, pitch, weight, bias, mean.numel(), x.shape[-1], float(eps),
-                     _DTYPES[x.dtype], _DTYPES[wtype], y, mean, rstd)
+    shape = x.shape
+    y = x.new_empty(shape)
+    mean = x.new_empty(shape[:-1], dtype=torch.float32)
+    rstd = torch.empty_like(mean)
+    rows = mean.numel()
+    if rows:
+        _run(device, "fm_layer_norm_forward", x, pitch, weight, bias, rows, shape[-1], float(eps), _DTYPES[x.dtype],
+             _DTYPES[wtype], y, mean, rstd)
     return y, mean, rstd
 
 
@@ -192,19 +198,15 @@ def layer_norm_backward(grad, x, mean, rstd, weight=None, bias=None):
     for name, t in (("mean", mean), ("rstd", rstd)):
         if t.shape != x.shape[:-1] or not t.is_contiguous():
             raise ValueError(f"{name} must be what layer_norm_forward returned for x")
-    given = {n: t for n, t in (("x", x), ("grad", grad), ("mean", mean), ("rstd", rstd), ("weight", weight),
-                               ("bias", bias)) if t is not None}
-    device = _on_gpu(**given)
+    device = _on_gpu(x=x, grad=grad, mean=mean, rstd=rstd, weight=weight, bias=bias)
     (x, ld_x), (grad, ld_dy) = _rows(x), _rows(grad)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=device)
+    dx = x.new_empty(x.shape)
     dw = None if weight is None else torch.empty_like(weight)
     db = None if bias is None else torch.empty_like(bias)
     rows, c = mean.numel(), x.shape[-1]
-    with _on(device):
-        size = nat.library().fm_layer_norm_backward_workspace_bytes(rows, c) if dw is not None or db is not None else 0
-        ws = torch.empty(size // 4, device=device) if size else None
-        ops.call("fm_layer_norm_backward", grad, ld_dy, x, ld_x, weight, mean, rstd, rows, c, _DTYPES[x.dtype],
-                 _DTYPES[wtype], dx, dw, db, ws, size)
+    ws, size = (None, 0) if dw is None and db is None else _scratch(x, "fm_layer_norm_backward_workspace_bytes", rows, c)
+    _run(device, "fm_layer_norm_backward", grad, ld_dy, x, ld_x, weight, mean, rstd, rows, c, _DTYPES[x.dtype],
+         _DTYPES[wtype], dx, dw, db, ws, size)
     return dx, dw, db
 
 
@@ -270,18 +272,16 @@ def _heads(t: torch.Tensor, group: int = 1) -> tuple[torch.Tensor, int, int, int
     kernels take them: 16-byte rows within 32-bit reach, else a copy."""
     size = t.element_size()
     unit = 16 // size
-
-    def strides(t):
-        return [st if n > 1 else 0 for n, st in zip(t.shape[:3], t.stride()[:3])]
-
-    sb, sn, sh = strides(t)
-    reach = (1 << 31) - 1
-    if (t.stride(3) != 1 and t.shape[3] > 1) or sb % unit or sn % unit or sh % unit or t.data_ptr() % 16 \
-            or sn > reach // size // 256 or sh > reach // size // 2 // group:
+    b, n, h, d = t.shape
+    sb, sn, sh, sd = t.stride()
+    # The stride of a single item does not matter, whatever it says.
+    sb, sn, sh = sb if b > 1 else 0, sn if n > 1 else 0, sh if h > 1 else 0
+    reach = 0x7fffffff // size
+    if (sd != 1 and d > 1) or (sb | sn | sh) % unit or t.data_ptr() % 16 or sn > reach // 256 or sh > reach // 2 // group:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
-        sb, sn, sh = strides(t)
+        sb, sn, sh, _ = t.stride()
     return t, sb, sn, sh
 
 
@@ -302,18 +302,15 @@ def window_attention_forward(q, k, v, window: int | None = None, scale: float | 
     what padding holds reaches nothing.
     """
     q, k, v, window, scale, lengths = _attention_input(q, k, v, window, scale, lengths)
-    device = _on_gpu(**{n: t for n, t in (("q", q), ("k", k), ("v", v), ("lengths", lengths)) if t is not None})
+    device = _on_gpu(q=q, k=k, v=v, lengths=lengths)
     b, t, h, d = q.shape
     s, kv = k.shape[1], k.shape[2]
-    out = torch.empty((b, t, h, d), dtype=q.dtype, device=device)
-    lse = torch.empty((b, t, h), device=device)
+    out = q.new_empty((b, t, h, d))
+    lse = q.new_empty((b, t, h), dtype=torch.float32)
     if b and t:
-        q, k, v = _heads(q, h // kv), _heads(k), _heads(v)
-        with _on(device):
-            size = nat.library().fm_attention_forward_workspace_bytes(b, t, s, h, kv, d, window)
-            ws = torch.empty(size // 4, device=device) if size else None
-            ops.call("fm_attention_forward", *q, *k, *v, lengths, b, t, s, h, kv, d, window, scale, _DTYPES[out.dtype], out,
-                     lse, ws, size)
+        ws, size = _scratch(q, "fm_attention_forward_workspace_bytes", b, t, s, h, kv, d, window)
+        _run(device, "fm_attention_forward", *_heads(q, h // kv), *_heads(k), *_heads(v), lengths, b, t, s, h, kv, d, window,
+             scale, _DTYPES[out.dtype], out, lse, ws, size)
     return out, lse
 
 
@@ -328,19 +325,15 @@ def window_attention_backward(grad, q, k, v, out, lse, window: int | None = None
         raise ValueError(f"grad must have q's shape {tuple(q.shape)}, got {tuple(grad.shape)}")
     if out.shape != q.shape or lse.shape != (b, t, h) or not lse.is_contiguous():
         raise ValueError("out and lse must be what window_attention_forward returned for q, k and v")
-    given = {"q": q, "k": k, "v": v, "grad": grad, "out": out, "lse": lse}
-    device = _on_gpu(**given, **({} if lengths is None else {"lengths": lengths}))
-    dq = torch.empty((b, t, h, d), dtype=q.dtype, device=device)
-    dk = torch.empty((b, s, kv, d), dtype=q.dtype, device=device)
-    dv = torch.empty((b, s, kv, d), dtype=q.dtype, device=device)
+    device = _on_gpu(q=q, k=k, v=v, grad=grad, out=out, lse=lse, lengths=lengths)
+    dq, dk, dv = q.new_empty((b, t, h, d)), q.new_empty((b, s, kv, d)), q.new_empty((b, s, kv, d))
     if b and s:
         if t == 0:
             return dq, dk.zero_(), dv.zero_()
         out = _heads(out.contiguous())[0]
-        stats = torch.empty((2, b, t, h), device=device)
-        with _on(device):
-            ops.call("fm_attention_backward", *_heads(grad, h // kv), *_heads(q, h // kv), *_heads(k), *_heads(v), out, lse,
-                     lengths, b, t, s, h, kv, d, window, scale, _DTYPES[q.dtype], dq, dk, dv, stats)
+        stats = lse.new_empty((2, b, t, h))
+        _run(device, "fm_attention_backward", *_heads(grad, h // kv), *_heads(q, h // kv), *_heads(k), *_heads(v), out, lse,
+             lengths, b, t, s, h, kv, d, window, scale, _DTYPES[q.dtype], dq, dk, dv, stats)
     return dq, dk, dv
 
 
@@ -400,11 +393,10 @@ def code_embedding_forward(codes, table, scale: float = 1.0):
     codes, table, scale = _embedding_input(codes, table, scale)
     device = _on_gpu(codes=codes, table=table)
     (b, books, frames), (_, entries, dim) = codes.shape, table.shape
-    out = torch.empty((b, frames, dim), dtype=table.dtype, device=device)
-    if out.numel():
-        with _on(device):
-            ops.call("fm_code_embedding", codes, codes.stride(0), codes.stride(1), b, books, frames, table.contiguous(),
-                     entries, dim, scale, _DTYPES[table.dtype], out)
+    out = table.new_empty((b, frames, dim))
+    if b and frames:
+        _run(device, "fm_code_embedding", codes, codes.stride(0), codes.stride(1), b, books, frames, table.contiguous(),
+             entries, dim, scale, _DTYPES[table.dtype], out)
     return out
 
 
@@ -420,12 +412,10 @@ def code_embedding_backward(grad, codes, table, scale: float = 1.0):
         raise ValueError(f"grad must have shape {(b, frames, dim)}, got {tuple(grad.shape)}")
     device = _on_gpu(codes=codes, table=table, grad=grad)
     grad, pitch = _rows(grad)
-    dtable = torch.empty(table.shape, dtype=table.dtype, device=device)
-    with _on(device):
-        size = nat.library().fm_code_embedding_backward_workspace_bytes(b, books, frames, entries, dim)
-        ws = torch.empty((size + 3) // 4, dtype=torch.int32, device=device)
-        ops.call("fm_code_embedding_backward", grad, pitch, codes, codes.stride(0), codes.stride(1), b, books, frames, entries,
-                 dim, scale, _DTYPES[table.dtype], dtable, ws, size)
+    dtable = table.new_empty(table.shape)
+    ws, size = _scratch(grad, "fm_code_embedding_backward_workspace_bytes", b, books, frames, entries, dim)
+    _run(device, "fm_code_embedding_backward", grad, pitch, codes, codes.stride(0), codes.stride(1), b, books, frames, entries,
+         dim, scale, _DTYPES[table.dtype], dtable, ws, size)
     return dtable
 
 

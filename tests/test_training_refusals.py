@@ -100,7 +100,8 @@ def test_other_abi_refusals():
     assert forward(P, 64, None, None, 4, 64, 1e-5, 0, 1, P, P, P, None) == 1000
     assert forward(P, 64, None, None, 1 << 40, 64, 1e-5, 0, 0, P, P, P, None) == 1002
     assert forward(None, 64, None, None, 0, 64, 1e-5, 0, 0, None, None, None, None) == 0
-    assert backward(P, 64, P, 64, P, P, P, 4, 64, 0, 0, P, P, P, None, 0, None) == 1001
+    assert backward(P, 64, P, 64, P, P, P, 400, 64, 0, 0, P, P, P, None, 0, None) == 1001
+    assert backward(P, 64, P, 64, P, P, P, 400, 64, 0, 0, P, P, P, None, 1 << 20, None) == 1000
     assert backward(P, 64, None, 64, P, P, P, 4, 64, 0, 0, P, P, P, P, 1 << 20, None) == 1000
     embed, gradient = lib.fm_code_embedding, lib.fm_code_embedding_backward
     assert embed(P, 8, 8, 1, 1, 8, None, 16, 8, 1.0, 0, P, None) == 1000
