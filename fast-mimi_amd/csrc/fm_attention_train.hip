@@ -536,14 +536,30 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Attn a) {
   const int t = (int)fm_div(r, a.by_g);
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S;
   const bool live = a.S - a.T + t < len;
-  float m = -INFINITY, l = 0.0f, o[DT / 64] = {};
-  for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[2 * (s * rows + at)]);
-  const float sub = m == -INFINITY ? 0.0f : m;
-  for (int s = 0; s < a.splits; ++s) {
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * (s * rows + at)] - sub);
-    l = fmaf(a.part_ml[2 * (s * rows + at) + 1], f, l);
+  // Lane s holds split s's maximum and sum (at most 64 splits).
+  floatx2_v ml{-INFINITY, 0.0f};
+  if (lane < a.splits) ml = *reinterpret_cast<const floatx2_v*>(a.part_ml + 2 * (lane * rows + at));
+  float m = ml[0];
 #pragma unroll
-    for (int u = 0; u < DT / 64; ++u) o[u] = fmaf(a.part_o[(s * rows + at) * DT + 64 * u + lane], f, o[u]);
+  for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  const float weight = __builtin_amdgcn_exp2f(ml[0] - (m == -INFINITY ? 0.0f : m));
+  float l = ml[1] * weight;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o, 64);
+  float o[DT / 64] = {};
+  constexpr int AHEAD = 8;
+  for (int s = 0; s < a.splits; s += AHEAD) {
+    float v[AHEAD][DT / 64];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+      for (int d = 0; d < DT / 64; ++d) v[u][d] = a.part_o[(min(s + u, a.splits - 1) * rows + at) * DT + 64 * d + lane];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const float f = __shfl(weight, min(s + u, 63), 64);
+#pragma unroll
+      for (int d = 0; d < DT / 64; ++d) o[d] = s + u < a.splits ? fmaf(v[u][d], f, o[d]) : o[d];
+    }
   }
   const long row = ((long)b * a.T + t) * a.H + kh * a.G + (r - t * a.G);
   if (lane == 0) a.lse[row] = live && l != 0.0f ? m + log2f(l) : -INFINITY;
