@@ -219,22 +219,6 @@ struct Reads {
   }
 };
 
-// The B operand of one row straight from memory: chunk s of the lane's half,
-// zeros where the row is not live or the chunk lies past the head's width.
-template <typename T, int DT>
-FM_DEVICE void load_row(const T* row, bool live, int D, int lane, typename Elem<T>::Frag (&f)[DT / Elem<T>::STEP]) {
-  constexpr int N = DT / Elem<T>::STEP, E = 16 / (int)sizeof(T);
-#pragma unroll
-  for (int s = 0; s < N; ++s) {
-    const int d = (2 * s + (lane >> 5)) * E;
-    const bool ok = live && d < D;  // the row itself is always one of the tensor's
-    uintx4_v u = *reinterpret_cast<const uintx4_v*>(row + (d < D ? d : 0));
-#pragma unroll
-    for (int e = 0; e < 4; ++e) u[e] = ok ? u[e] : 0;
-    f[s] = __builtin_bit_cast(typename Elem<T>::Frag, u);
-  }
-}
-
 // Has the compiler wait for these loads here.  Where their first use is inside
 // a loop it would wait there in every turn, for the next tile's copies as well.
 template <typename F, int N>
@@ -243,36 +227,240 @@ FM_DEVICE void arrive(F (&f)[N]) {
   for (int s = 0; s < N; ++s) asm volatile("" : "+v"(f[s]));
 }
 
-// s += 32 rows of a tile (lane address a) times B: a product over the head's
-// width.  The 16-bit forms read four steps' fragments before their products, so
-// that a wave does not wait for LDS at each (32 cycles do not cover a read);
-// FP32 products do.
-template <typename T, int DT, int N>
-FM_DEVICE void products(unsigned a, const typename Elem<T>::Frag (&b)[N], floatx16& s) {
-  typename Elem<T>::Frag f[N];
-  constexpr int AHEAD = 4;
+// The operands of one row and the products with them, for tiles of ROWS rows.
+//
+// 16-bit inputs, and FP32 heads beyond 64: tiles lie in LDS as they are in memory,
+// copied there directly; the FP32 products are FP32 MFMAs.
+template <typename T, int DT>
+constexpr bool SPLIT = std::is_same<T, float>::value && DT == 64;
+
+template <typename T, int DT, int ROWS, bool SPLITS>
+struct Engine {
+  typedef Elem<T> E;
+  typedef Reads<T, DT> R;
+  typedef typename E::Frag Frag;
+  static constexpr int N = DT / E::STEP, ND = DT / 32, TILE = ROWS * R::PITCH;
+
+  // The B operand of one row straight from memory: chunk s of the lane's half,
+  // zeros where the row is not live or the chunk lies past the head's width.
+  struct Held {
+    Frag f[N];
+  };
+  static FM_DEVICE void load(const T* row, bool live, int D, int lane, Held& h) {
+    constexpr int W = 16 / (int)sizeof(T);
 #pragma unroll
-  for (int c0 = 0; c0 < N; c0 += AHEAD) {
+    for (int s = 0; s < N; ++s) {
+      const int d = (2 * s + (lane >> 5)) * W;
+      const bool ok = live && d < D;  // the row itself is always one of the tensor's
+      uintx4_v u = *reinterpret_cast<const uintx4_v*>(row + (d < D ? d : 0));
 #pragma unroll
-    for (int c = c0; c < c0 + AHEAD; ++c) f[c] = Reads<T, DT>::row(a, c);
-    if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int c = c0; c < c0 + AHEAD; ++c) s = Elem<T>::mma(f[c], b[c], s);
+      for (int e = 0; e < 4; ++e) u[e] = ok ? u[e] : 0;
+      h.f[s] = __builtin_bit_cast(Frag, u);
+    }
   }
-}
-// The same with B in LDS as well.
-template <typename T, int DT, int N>
-FM_DEVICE void products(unsigned a, unsigned b, floatx16& s) {
-  typename Elem<T>::Frag f[N], g[N];
-  constexpr int AHEAD = 4;
+  static FM_DEVICE void here(Held& h) { arrive(h.f); }
+
+  // s += 32 rows of a tile (lane address a) times B: a product over the head's
+  // width.  The 16-bit forms read four steps' fragments before their products, so
+  // that a wave does not wait for LDS at each (32 cycles do not cover a read);
+  // FP32 products do.
+  static constexpr int AHEAD = 4;
+  static FM_DEVICE void products(unsigned a, const Held& b, floatx16& s) {
+    Frag f[N];
 #pragma unroll
-  for (int c0 = 0; c0 < N; c0 += AHEAD) {
+    for (int c0 = 0; c0 < N; c0 += AHEAD) {
 #pragma unroll
-    for (int c = c0; c < c0 + AHEAD; ++c) f[c] = Reads<T, DT>::row(a, c), g[c] = Reads<T, DT>::row(b, c);
-    __builtin_amdgcn_sched_barrier(0);
+      for (int c = c0; c < c0 + AHEAD; ++c) f[c] = R::row(a, c);
+      if constexpr (sizeof(T) == 2) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int c = c0; c < c0 + AHEAD; ++c) s = Elem<T>::mma(f[c], g[c], s);
+      for (int c = c0; c < c0 + AHEAD; ++c) s = E::mma(f[c], b.f[c], s);
+    }
   }
+  // The same with B in LDS as well.
+  static FM_DEVICE void products(unsigned a, unsigned b, floatx16& s) {
+    Frag f[N], g[N];
+#pragma unroll
+    for (int c0 = 0; c0 < N; c0 += AHEAD) {
+#pragma unroll
+      for (int c = c0; c < c0 + AHEAD; ++c) f[c] = R::row(a, c), g[c] = R::row(b, c);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int c = c0; c < c0 + AHEAD; ++c) s = E::mma(f[c], g[c], s);
+    }
+  }
+
+  // acc += (32 rows of a tile)^T times s, a product over the rows.  REST: the
+  // second factor in two 16-bit pieces.
+  template <bool REST>
+  static FM_DEVICE void outer(unsigned a, const floatx16& s, floatx16 (&acc)[ND]) {
+#pragma unroll
+    for (int c = 0; c < 32 / E::STEP; ++c) {
+      const Frag p = E::pack(s, c);
+      Frag f[ND];
+      R::cols(a, c, f);
+      if constexpr (REST && sizeof(T) == 2) {
+        const Frag low = E::pack_rest(s, p, c);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[d] = E::mma(f[d], low, acc[d]);
+      }
+#pragma unroll
+      for (int d = 0; d < ND; ++d) acc[d] = E::mma(f[d], p, acc[d]);
+    }
+  }
+};
+
+// FP32 heads up to 64: every factor as three round-to-nearest bf16 pieces (exact
+// to 2^-24) and each product as the six of them of order at most 2, summed in
+// FP32 from the smallest: 768 matrix cycles per 32x32x64 where the FP32 MFMA takes
+// 2048, at its error.  A block's threads bring the next tile into registers, and
+// split it into three planes in LDS once all waves are done with the last one.
+// Infinities have no such pieces (their products with the others' remainders are
+// infinities of either sign): a block that meets a value of 2^127 or more starts
+// again on FP32 MFMAs.
+// 16 x 2500 frames, 8 heads, window 250: forward 250 -> 170 us, dQ 355 -> 270,
+// dK / dV 500 -> 335 (there the matrix cores and the vector work, half of it the
+// splitting, take turns).
+template <int ROWS>
+struct Engine<float, 64, ROWS, true> {
+  typedef Reads<__bf16, 64> R;
+  static constexpr int N = 4, ND = 2, PLANE = ROWS * 128, TILE = 3 * PLANE, UNITS = ROWS / 32;
+
+  struct Held {
+    bf16x8 f[3][N];
+    float most;  // the largest magnitude
+  };
+  static FM_DEVICE float size(floatx4 a, floatx4 b, float u) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) u = fmaxf(u, fmaxf(fabsf(a[e]), fabsf(b[e])));
+    return u;
+  }
+  static FM_DEVICE void split8(floatx4 lo, floatx4 hi, bf16x8 (&h)[3]) {
+    bf16x4 a[3], b[3];
+    split3(lo, a[0], a[1], a[2]);
+    split3(hi, b[0], b[1], b[2]);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) h[k] = __builtin_shufflevector(a[k], b[k], 0, 1, 2, 3, 4, 5, 6, 7);
+  }
+  static FM_DEVICE void load(const float* row, bool live, int D, int lane, Held& h) {
+    h.most = 0.0f;
+#pragma unroll
+    for (int s = 0; s < N; ++s) {
+      floatx4 v[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int d = 16 * s + 8 * (lane >> 5) + 4 * u;
+        const bool ok = live && d < D;
+        v[u] = *reinterpret_cast<const floatx4*>(row + (d < D ? d : 0));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[u][e] = ok ? v[u][e] : 0.0f;
+      }
+      h.most = size(v[0], v[1], h.most);
+      bf16x8 p[3];
+      split8(v[0], v[1], p);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) h.f[k][s] = p[k];
+    }
+  }
+  static FM_DEVICE void here(Held& h) {
+#pragma unroll
+    for (int k = 0; k < 3; ++k) arrive(h.f[k]);
+    // Used behind the loop only: else the values would be kept until there.
+    asm volatile("" : "+v"(h.most));
+  }
+
+  static FM_DEVICE floatx16 six(const bf16x8 (&a)[3], const bf16x8 (&b)[3], floatx16 s) {
+    s = fm_mfma32_bf16(a[2], b[0], s);
+    s = fm_mfma32_bf16(a[0], b[2], s);
+    s = fm_mfma32_bf16(a[1], b[1], s);
+    s = fm_mfma32_bf16(a[1], b[0], s);
+    s = fm_mfma32_bf16(a[0], b[1], s);
+    return fm_mfma32_bf16(a[0], b[0], s);
+  }
+  static FM_DEVICE void products(unsigned a, const Held& b, floatx16& s) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      bf16x8 f[3];
+#pragma unroll
+      for (int k = 0; k < 3; ++k) f[k] = R::row(a + k * PLANE, c);
+      const bf16x8 g[3] = {b.f[0][c], b.f[1][c], b.f[2][c]};
+      s = six(f, g, s);
+    }
+  }
+  // The same with B in LDS as well, in planes of its own size.
+  template <int OTHER>
+  static FM_DEVICE void products(unsigned a, unsigned b, floatx16& s) {
+#pragma unroll
+    for (int c = 0; c < N; ++c) {
+      bf16x8 f[3], g[3];
+#pragma unroll
+      for (int k = 0; k < 3; ++k) f[k] = R::row(a + k * PLANE, c), g[k] = R::row(b + k * OTHER, c);
+      s = six(f, g, s);
+    }
+  }
+  template <bool REST>
+  static FM_DEVICE void outer(unsigned a, const floatx16& s, floatx16 (&acc)[ND]) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      bf16x8 p[3], f[3][ND];
+      split8(floatx4{s[8 * c], s[8 * c + 1], s[8 * c + 2], s[8 * c + 3]},
+             floatx4{s[8 * c + 4], s[8 * c + 5], s[8 * c + 6], s[8 * c + 7]}, p);
+#pragma unroll
+      for (int k = 0; k < 3; ++k) R::cols(a + k * PLANE, c, f[k]);
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const bf16x8 g[3] = {f[0][d], f[1][d], f[2][d]};
+        acc[d] = six(g, p, acc[d]);
+      }
+    }
+  }
+
+  // Rows of a tile on their way: thread i holds eight columns of each of UNITS rows.
+  struct Flight {
+    floatx4 v[UNITS][2];
+  };
+  template <typename Offset>
+  static FM_DEVICE void bring(const void* base, int D, Flight& f, Offset offset) {
+    const __amdgpu_buffer_rsrc_t buf = fm_buffer(base, INT_MAX);
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      const int i = u * 256 + threadIdx.x, off = offset(i >> 3);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int d = 8 * (i & 7) + 4 * k;
+        f.v[u][k] = fm_buf_load4(buf, off >= 0 && d < D ? off + 4 * d : INT_MIN, 0);
+      }
+    }
+  }
+  // Returns the largest magnitude among this lane's values and `most`.
+  static FM_DEVICE float publish(const Flight& f, unsigned char* tile, float most) {
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+      most = size(f.v[u][0], f.v[u][1], most);
+      asm volatile("" : "+v"(most));
+      const int i = u * 256 + threadIdx.x, r = i >> 3;
+      bf16x8 p[3];
+      split8(f.v[u][0], f.v[u][1], p);
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+        *reinterpret_cast<bf16x8*>(tile + k * PLANE + r * 128 + (((i & 7) ^ swz<__bf16, 64>(r)) << 4)) = p[k];
+    }
+    return most;
+  }
+};
+
+// The dot product of two rows, half of it in each lane half.
+template <typename T, int DT>
+FM_DEVICE float row_dot(const T* x, const T* y, bool live, int D, int lane) {
+  constexpr int W = 16 / (int)sizeof(T);
+  float s = 0.0f;
+#pragma unroll
+  for (int d0 = 0; d0 < DT; d0 += 2 * W) {
+    const int d = d0 + (lane >> 5) * W, at = d < D ? d : 0;
+    const typename Elem<T>::Frag a = *reinterpret_cast<const typename Elem<T>::Frag*>(x + at);
+    const typename Elem<T>::Frag b = *reinterpret_cast<const typename Elem<T>::Frag*>(y + at);
+    s = live && d < D ? Elem<T>::dot(a, b, s) : s;
+  }
+  return s;
 }
 
 // Starts the copy of ROWS rows into LDS (global -> LDS, 16 bytes a lane).
@@ -361,6 +549,19 @@ FM_DEVICE void merge(float* lds, floatx16 (&acc)[DT / 32], int own, int wk, int 
   }
 }
 
+// A lane's values first .. of a result row (groups of four columns), times f;
+// zeros for a row that is not live.
+template <typename T, int N>
+FM_DEVICE void store_row(T* o, const float (&v)[N], float f, bool live, int first, int half, int D) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const int e = first + i, d = 32 * (e / 16) + 8 * (e % 16 / 4) + 4 * half;
+    if (d < D)
+      Elem<T>::store4(o + d, live ? v[i] * f : 0.0f, live ? v[i + 1] * f : 0.0f, live ? v[i + 2] * f : 0.0f,
+                      live ? v[i + 3] * f : 0.0f);
+  }
+}
+
 // Starts the copies of the keys and values k0 .. k_hi (at most KEYS) of a head.
 template <typename T, int DT, int KEYS, int WAVES = 4>
 FM_DEVICE void load_keys(const Attn& a, const T* kp, const T* vp, int k0, int k_hi, unsigned char* at, int wave, int lane) {
@@ -370,39 +571,100 @@ FM_DEVICE void load_keys(const Attn& a, const T* kp, const T* vp, int k0, int k_
   load_tile<T, DT, KEYS, WAVES>(vp + k0 * a.v.row, at + TILE, a.D, wave, lane, [&](int r) { return r <= n ? r * vs : -1; });
 }
 
+constexpr float BIG = 1.7014118346046923e38f;  // 2^127
+
 // KEEP: bytes of LDS that a dK / dV block keeps its keys and values in.
-template <typename T, int DT, int WQ, int WK, int KEEP = 0>
+template <typename T, int DT, int WQ, int WK, bool SPLITS, int KEEP = 0>
 struct Tiling {
   static constexpr int NB = WK > 1 || sizeof(T) == 4 ? 1 : 2;  // 32-key tiles of a wave
   static constexpr int KEYS = 32 * NB * WK;
-  static constexpr int TILE = KEYS * DT * (int)sizeof(T);
-  static constexpr int STAGES = 4 * TILE <= 131072 && !KEEP ? 2 : 1;
+  static constexpr int TILE = Engine<T, DT, KEYS, SPLITS>::TILE;
+  static constexpr int STAGES = 4 * TILE <= 131072 && !KEEP && !SPLITS ? 2 : 1;
   static constexpr int MERGE = WK > 1 ? WQ * WK * DT * 128 : 0;  // room for the waves' results
   static constexpr int LDS = std::max(KEEP + 2 * STAGES * TILE, MERGE);
-  // Blocks per CU that the registers are held to.  At two (256 a lane) all of
-  // them are vector registers and no result passes through accumulation
-  // registers; the kernels that need more (HEAVY) run one block.
-  template <bool HEAVY> static constexpr int blocks() { return LDS > 81920 || HEAVY ? 1 : 2; }
 };
 
-// Forward.  WQ waves take 32 rows each and share the key tiles (many rows), or
-// WK waves take the same 32 rows and a quarter of each key tile (few rows).
+// The same call, as something that the compiler does not recognise: what a second
+// form shares with the first would else be held in registers all through it.
+FM_DEVICE Attn again(Attn a) {
+  for (const void** p : {&a.q.p, &a.k.p, &a.v.p, &a.dout.p, &a.o}) asm volatile("" : "+s"(*p));
+  for (int* n : {&a.B, &a.T, &a.S, &a.H, &a.KV, &a.G, &a.D, &a.window}) asm volatile("" : "+s"(*n));
+  asm volatile("" : "+s"(a.lengths));
+  return a;
+}
+
+// A kernel's LDS: what either of its forms takes.
+template <typename T, int DT, template <bool> class Form>
+constexpr int lds_bytes() {
+  if constexpr (SPLIT<T, DT>) return std::max(Form<true>::BYTES, Form<false>::BYTES);
+  else return Form<false>::BYTES;
+}
+
+// Blocks per CU that the registers are held to.  At two (256 a lane) all of them
+// are vector registers and no result passes through accumulation registers; the
+// kernels that need more (heavy) run one block.
+constexpr int blocks(int lds, bool heavy) { return lds > 81920 || heavy ? 1 : 2; }
+
+// The key and value tiles of a row block (forward, dQ) on their way.
+template <typename T, int DT, int KEYS, bool SPLITS>
+struct KeyTiles {
+  FM_DEVICE void start(const Attn& a, const T* kp, const T* vp, int k0, int k_hi, unsigned char* at, int wave, int lane) {
+    load_keys<T, DT, KEYS>(a, kp, vp, k0, k_hi, at, wave, lane);
+  }
+};
+template <typename T, int DT, int KEYS>
+struct KeyTiles<T, DT, KEYS, true> {
+  typedef Engine<T, DT, KEYS, true> G;
+  typename G::Flight k, v;
+  FM_DEVICE void start(const Attn& a, const T* kp, const T* vp, int k0, int k_hi, unsigned char*, int, int) {
+    const int n = k_hi - k0, ks = (int)(a.k.row * (long)sizeof(T)), vs = (int)(a.v.row * (long)sizeof(T));
+    G::bring(kp + k0 * a.k.row, a.D, k, [&](int r) { return r <= n ? r * ks : -1; });
+    G::bring(vp + k0 * a.v.row, a.D, v, [&](int r) { return r <= n ? r * vs : -1; });
+  }
+  FM_DEVICE float publish(unsigned char* at, float most) {
+    most = G::publish(v, at + G::TILE, G::publish(k, at, most));
+    lds_barrier();
+    return most;
+  }
+};
+
+// The forms of a kernel return whether they are done; the split one is not where
+// it met a value that wants FP32 products.
 template <typename T, int DT, int WQ, int WK>
-__global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<false>())) void attention_forward_kernel(Attn a) {
-  typedef Elem<T> E;
-  typedef Tiling<T, DT, WQ, WK> L;
-  constexpr int NS = DT / E::STEP, ND = DT / 32;
+struct Forward {
+  template <bool SPLITS>
+  struct Form {
+    static constexpr int BYTES = Tiling<T, DT, WQ, WK, SPLITS>::LDS + (WK > 1 ? 4 * 2 * 128 : 0);
+  };
+  static constexpr int LDS = lds_bytes<T, DT, Form>();
+  static constexpr int BLOCKS = SPLIT<T, DT> && WK == 1 ? 3 : blocks(LDS, false);
+  template <bool SPLITS> static FM_DEVICE bool run(const Attn& a, unsigned char* lds);
+};
+template <typename T, int DT, int WQ, int WK>
+__global__ __launch_bounds__(256, (Forward<T, DT, WQ, WK>::BLOCKS)) void attention_forward_kernel(Attn a) {
   // One array for all of the block's LDS: among several the compiler tells the
   // direct copies' targets apart, and then waits for all copies at every read.
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[L::LDS + (WK > 1 ? 4 * 2 * 128 : 0)];
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[Forward<T, DT, WQ, WK>::LDS];
+  if constexpr (SPLIT<T, DT>) {
+    if (!Forward<T, DT, WQ, WK>::template run<true>(a, lds)) Forward<T, DT, WQ, WK>::template run<false>(again(a), lds);
+  } else {
+    Forward<T, DT, WQ, WK>::template run<false>(a, lds);
+  }
+}
+
+template <typename T, int DT, int WQ, int WK>
+template <bool SPLITS>
+FM_DEVICE bool Forward<T, DT, WQ, WK>::run(const Attn& a, unsigned char* lds) {
+  typedef Tiling<T, DT, WQ, WK, SPLITS> L;
+  typedef Engine<T, DT, L::KEYS, SPLITS> G;
+  constexpr int ND = DT / 32;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave % WQ, wk = wave / WQ, half = lane >> 5;
   const Rows<WQ> w(a, wq, lane);
-  typedef Reads<T, DT> R;
+  typedef typename G::R R;
   const unsigned row_lane = R::row_lane(lane), col_lane = R::col_lane(lane);
 
-  typename E::Frag qf[NS];
-  load_row<T, DT>(w.template of<T>(a.q) + w.t * a.q.row + (w.kh * a.G + (min(w.r, w.R - 1) - w.t * a.G)) * a.q.head, w.live,
-                  a.D, lane, qf);
+  typename G::Held q;
+  G::load(w.template of<T>(a.q) + w.t * a.q.row + (w.kh * a.G + (min(w.r, w.R - 1) - w.t * a.G)) * a.q.head, w.live, a.D, lane, q);
   floatx16 acc[ND] = {};
   float m = -INFINITY, l = 0.0f;  // l: of this lane's keys only
 
@@ -414,14 +676,17 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<false>
   }
   const T* kp = w.template of<T>(a.k) + w.kh * a.k.head;
   const T* vp = w.template of<T>(a.v) + w.kh * a.v.head;
+  KeyTiles<T, DT, L::KEYS, SPLITS> next;
+  float most = 0.0f;
   auto load = [&](int i) {
-    load_keys<T, DT, L::KEYS>(a, kp, vp, w.k_lo + i * L::KEYS, w.k_hi, lds + (i - first) % L::STAGES * 2 * L::TILE, wave, lane);
+    next.start(a, kp, vp, w.k_lo + i * L::KEYS, w.k_hi, lds + (i - first) % L::STAGES * 2 * L::TILE, wave, lane);
   };
   if (first < tiles) load(first);
-  arrive(qf);
+  G::here(q);
   for (int i = first; i < tiles; ++i) {
     tile_barrier();  // tile i is there, and every wave is past tile i - 1
-    if (L::STAGES == 2 && i + 1 < tiles) load(i + 1);
+    if constexpr (SPLITS) most = next.publish(lds, most);
+    if ((L::STAGES == 2 || SPLITS) && i + 1 < tiles) load(i + 1);
     const unsigned char* kt = lds + (i - first) % L::STAGES * 2 * L::TILE;
     const unsigned char* vt = kt + L::TILE;
 #pragma unroll
@@ -429,7 +694,7 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<false>
       const int row = (wk * L::NB + nb) * 32, k0 = w.k_lo + i * L::KEYS + row;
       if (k0 > w.p_hi || k0 + 31 <= w.p_lo - a.window) continue;  // nothing that this wave sees
       floatx16 s = {};
-      products<T, DT>(R::fresh(R::lds(kt) + row * R::PITCH + row_lane), qf, s);
+      G::products(R::fresh(R::lds(kt) + row * R::PITCH + row_lane), q, s);
       if (k0 + 31 > w.p_lo || k0 <= w.p_hi - a.window || k0 + 31 > w.k_hi) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -459,21 +724,15 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<false>
         s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -sub));
         l += s[e];
       }
-      const unsigned at = R::fresh(R::lds(vt) + row * R::PITCH + col_lane);
-#pragma unroll
-      for (int c = 0; c < 32 / E::STEP; ++c) {
-        const typename E::Frag p = E::pack(s, c);
-        typename E::Frag f[ND];
-        R::cols(at, c, f);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) acc[d] = E::mma(f[d], p, acc[d]);
-      }
+      G::template outer<false>(R::fresh(R::lds(vt) + row * R::PITCH + col_lane), s, acc);
     }
-    if (L::STAGES == 1 && i + 1 < tiles) {
+    if (L::STAGES == 1 && !SPLITS && i + 1 < tiles) {
       tile_barrier();
       load(i + 1);
     }
   }
+  if constexpr (SPLITS)
+    if (__syncthreads_or(fmaxf(most, q.most) >= BIG)) return false;
   l = half_sum(l);
 
   constexpr int MINE = DT / 2 / WK;
@@ -499,31 +758,19 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<false>
 #pragma unroll
     for (int i = 0; i < MINE; ++i) mine[i] = acc[i / 16][i % 16];
   }
-  if (w.r >= w.R) return;
+  if (w.r >= w.R) return true;
   const bool writes = half == 0 && wk == 0;
   if (a.splits > 1) {
     const long at = ((long)blockIdx.z * gridDim.x + blockIdx.x) * w.R + w.r;
     if (writes) *reinterpret_cast<floatx2_v*>(a.part_ml + 2 * at) = floatx2_v{m, l};
-    float* o = a.part_o + at * DT;
-#pragma unroll
-    for (int i = 0; i < MINE; i += 4) {
-      const int e = wk * MINE + i;
-      *reinterpret_cast<floatx4*>(o + 32 * (e / 16) + 8 * (e % 16 / 4) + 4 * half) =
-          floatx4{mine[i], mine[i + 1], mine[i + 2], mine[i + 3]};
-    }
-    return;
+    store_row(a.part_o + at * DT, mine, 1.0f, true, wk * MINE, half, DT);
+    return true;
   }
   // A row that sees nothing (padding) gives zeros.
-  const float inv = w.live && l > 0.0f ? 1.0f / l : (w.live && l != l ? l : 0.0f);
-  if (writes) a.lse[w.row_index] = w.live && l != 0.0f ? m + log2f(l) : -INFINITY;
-  T* o = static_cast<T*>(a.out) + w.row_index * a.D;
-#pragma unroll
-  for (int i = 0; i < MINE; i += 4) {
-    const int e = wk * MINE + i, d = 32 * (e / 16) + 8 * (e % 16 / 4) + 4 * half;
-    if (d < a.D)
-      E::store4(o + d, w.live ? mine[i] * inv : 0.0f, w.live ? mine[i + 1] * inv : 0.0f, w.live ? mine[i + 2] * inv : 0.0f,
-                w.live ? mine[i + 3] * inv : 0.0f);
-  }
+  const bool some = w.live && l != 0.0f;
+  if (writes) a.lse[w.row_index] = some ? m + log2f(l) : -INFINITY;
+  store_row(static_cast<T*>(a.out) + w.row_index * a.D, mine, 1.0f / l, some, wk * MINE, half, a.D);
+  return true;
 }
 
 // Joins the parts of a split forward: one wave per row, lane d of DT columns.
@@ -576,46 +823,67 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Attn a) {
 // rowsum(dO O) from the rounded O is only nearly the sum over P dP; the sum of dS,
 // zero but for that, puts it right for the dK / dV kernel.
 template <typename T, int DT, int WQ, int WK>
-__global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<sizeof(T) == 4 && DT == 128>())) void attention_dq_kernel(Attn a) {
+struct QueryGradient {
+  template <bool SPLITS>
+  struct Form {
+    static constexpr int BYTES = Tiling<T, DT, WQ, WK, SPLITS>::LDS + (WK > 1 ? 4 * 128 : 0);
+  };
+  static constexpr int LDS = lds_bytes<T, DT, Form>();
+  static constexpr int BLOCKS = blocks(LDS, sizeof(T) == 4 && DT == 128);
+  template <bool SPLITS> static FM_DEVICE bool run(const Attn& a, unsigned char* lds);
+};
+template <typename T, int DT, int WQ, int WK>
+__global__ __launch_bounds__(256, (QueryGradient<T, DT, WQ, WK>::BLOCKS)) void attention_dq_kernel(Attn a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[QueryGradient<T, DT, WQ, WK>::LDS];
+  if constexpr (SPLIT<T, DT>) {
+    if (!QueryGradient<T, DT, WQ, WK>::template run<true>(a, lds)) QueryGradient<T, DT, WQ, WK>::template run<false>(again(a), lds);
+  } else {
+    QueryGradient<T, DT, WQ, WK>::template run<false>(a, lds);
+  }
+}
+
+template <typename T, int DT, int WQ, int WK>
+template <bool SPLITS>
+FM_DEVICE bool QueryGradient<T, DT, WQ, WK>::run(const Attn& a, unsigned char* lds) {
   typedef Elem<T> E;
-  typedef Tiling<T, DT, WQ, WK> L;
-  constexpr int NS = DT / E::STEP, ND = DT / 32;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[L::LDS + (WK > 1 ? 4 * 128 : 0)];
+  typedef Tiling<T, DT, WQ, WK, SPLITS> L;
+  typedef Engine<T, DT, L::KEYS, SPLITS> G;
+  constexpr int ND = DT / 32;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave % WQ, wk = wave / WQ, half = lane >> 5;
   const Rows<WQ> w(a, wq, lane);
-  typedef Reads<T, DT> R;
+  typedef typename G::R R;
   const unsigned row_lane = R::row_lane(lane), col_lane = R::col_lane(lane);
 
   const T* kp = w.template of<T>(a.k) + w.kh * a.k.head;
   const T* vp = w.template of<T>(a.v) + w.kh * a.v.head;
   const int tiles = w.k_hi >= w.k_lo ? (w.k_hi - w.k_lo) / L::KEYS + 1 : 0;
+  KeyTiles<T, DT, L::KEYS, SPLITS> next;
+  float most = 0.0f;
   auto load = [&](int i) {
-    load_keys<T, DT, L::KEYS>(a, kp, vp, w.k_lo + i * L::KEYS, w.k_hi, lds + i % L::STAGES * 2 * L::TILE, wave, lane);
+    next.start(a, kp, vp, w.k_lo + i * L::KEYS, w.k_hi, lds + i % L::STAGES * 2 * L::TILE, wave, lane);
   };
   if (tiles) load(0);
 
-  typename E::Frag qf[NS], gf[NS];
+  typename G::Held q, g;
   const int head = w.kh * a.G + (min(w.r, w.R - 1) - w.t * a.G);
-  load_row<T, DT>(w.template of<T>(a.dout) + w.t * a.dout.row + head * a.dout.head, w.live, a.D, lane, gf);
-  load_row<T, DT>(static_cast<const T*>(a.o) + w.row_index * a.D, w.live, a.D, lane, qf);
-  float delta = 0.0f;
-#pragma unroll
-  for (int c = 0; c < NS; ++c) delta = E::dot(gf[c], qf[c], delta);
-  delta = half_sum(delta);
-  load_row<T, DT>(w.template of<T>(a.q) + w.t * a.q.row + head * a.q.head, w.live, a.D, lane, qf);
+  const T* grad = w.template of<T>(a.dout) + w.t * a.dout.row + head * a.dout.head;
+  G::load(w.template of<T>(a.q) + w.t * a.q.row + head * a.q.head, w.live, a.D, lane, q);
+  G::load(grad, w.live, a.D, lane, g);
+  float delta = half_sum(row_dot<T, DT>(grad, static_cast<const T*>(a.o) + w.row_index * a.D, w.live, a.D, lane));
   // A row without keys takes every probability as zero.
   float lse = w.live ? a.lse[w.row_index] : INFINITY;
   lse = lse == -INFINITY ? INFINITY : lse;
   float rest = 0.0f;  // the sum of dS: what the rounding of O took from delta
 
   floatx16 acc[ND] = {};
-  arrive(qf), arrive(gf);
+  G::here(q), G::here(g);
   float row_stats[2] = {lse, delta};
   arrive(row_stats);
   lse = row_stats[0], delta = row_stats[1];
   for (int i = 0; i < tiles; ++i) {
     tile_barrier();
-    if (L::STAGES == 2 && i + 1 < tiles) load(i + 1);
+    if constexpr (SPLITS) most = next.publish(lds, most);
+    if ((L::STAGES == 2 || SPLITS) && i + 1 < tiles) load(i + 1);
     const unsigned char* kt = lds + i % L::STAGES * 2 * L::TILE;
     const unsigned char* vt = kt + L::TILE;
 #pragma unroll
@@ -624,8 +892,8 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<sizeof
       if (k0 > w.p_hi || k0 + 31 <= w.p_lo - a.window) continue;
       floatx16 s = {}, dp = {};
       const unsigned at = R::fresh(R::lds(kt) + row * R::PITCH + row_lane);
-      products<T, DT>(at, qf, s);
-      products<T, DT>(at + L::TILE, gf, dp);
+      G::products(at, q, s);
+      G::products(at + L::TILE, g, dp);
       const bool edge = k0 + 31 > w.p_lo || k0 <= w.p_hi - a.window || k0 + 31 > w.k_hi;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
@@ -641,26 +909,15 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<sizeof
       }
 #pragma unroll
       for (int e = 0; e < 16; ++e) rest += s[e];
-      const unsigned to = R::fresh(R::lds(kt) + row * R::PITCH + col_lane);
-#pragma unroll
-      for (int c = 0; c < 32 / E::STEP; ++c) {
-        const typename E::Frag ds = E::pack(s, c);
-        typename E::Frag f[ND];
-        R::cols(to, c, f);
-        if constexpr (sizeof(T) == 2) {
-          const typename E::Frag low = E::pack_rest(s, ds, c);
-#pragma unroll
-          for (int d = 0; d < ND; ++d) acc[d] = E::mma(f[d], low, acc[d]);
-        }
-#pragma unroll
-        for (int d = 0; d < ND; ++d) acc[d] = E::mma(f[d], ds, acc[d]);
-      }
+      G::template outer<true>(R::fresh(R::lds(kt) + row * R::PITCH + col_lane), s, acc);
     }
-    if (L::STAGES == 1 && i + 1 < tiles) {
+    if (L::STAGES == 1 && !SPLITS && i + 1 < tiles) {
       tile_barrier();
       load(i + 1);
     }
   }
+  if constexpr (SPLITS)
+    if (__syncthreads_or(fmaxf(most, fmaxf(q.most, g.most)) >= BIG)) return false;
   rest = half_sum(rest);
   constexpr int MINE = DT / 2 / WK;
   float mine[MINE];
@@ -676,21 +933,22 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<sizeof
 #pragma unroll
     for (int i = 0; i < MINE; ++i) mine[i] = acc[i / 16][i % 16];
   }
-  if (w.r >= w.R) return;
+  if (w.r >= w.R) return true;
   if (half == 0 && wk == 0) {
     a.stats[w.row_index] = lse;
     a.stats[(long)a.B * a.T * a.H + w.row_index] = sizeof(T) == 2 ? delta + rest : delta;
   }
-  T* o = static_cast<T*>(a.out) + w.row_index * a.D;
-#pragma unroll
-  for (int i = 0; i < MINE; i += 4) {
-    const int e = wk * MINE + i, d = 32 * (e / 16) + 8 * (e % 16 / 4) + 4 * half;
-    const float f = a.scale;
-    if (d < a.D)
-      E::store4(o + d, w.live ? mine[i] * f : 0.0f, w.live ? mine[i + 1] * f : 0.0f, w.live ? mine[i + 2] * f : 0.0f,
-                w.live ? mine[i + 3] * f : 0.0f);
-  }
+  store_row(static_cast<T*>(a.out) + w.row_index * a.D, mine, a.scale, w.live, wk * MINE, half, a.D);
+  return true;
 }
+
+// The query and gradient tiles of a key block on their way in registers.
+template <typename T, int DT, int ROWS, bool SPLITS>
+struct RowTiles {};
+template <typename T, int DT, int ROWS>
+struct RowTiles<T, DT, ROWS, true> {
+  typename Engine<T, DT, ROWS, true>::Flight q, g;
+};
 
 // dK and dV of 32 keys a wave over every row that sees them.  WK waves take 32
 // keys each and share the row tiles (many keys), WR waves take the same 32 keys
@@ -706,21 +964,40 @@ __global__ __launch_bounds__(256, (Tiling<T, DT, WQ, WK>::template blocks<sizeof
 // / eight waves; 16 heads x 2 x 2048: 190, 102 / 126.
 template <typename T, int DT>
 constexpr bool HELD = sizeof(T) == 2 && DT == 128;
-template <typename T, int DT, int WK>
-constexpr int HELD_BYTES = HELD<T, DT> ? 2 * 32 * WK * DT * 2 : 0;
+template <typename T, int DT, int WK, int WR>
+struct KeyGradients {
+  template <bool SPLITS>
+  struct Form {
+    static constexpr int KEEP = SPLITS ? Engine<T, DT, 32 * WK, SPLITS>::TILE : HELD<T, DT> ? 2 * 32 * WK * DT * 2 : 0;
+    typedef Tiling<T, DT, WK, WR, SPLITS, KEEP> L;
+    static constexpr int TURNS = SPLITS ? 2 : L::STAGES;
+    static constexpr int BYTES = L::LDS + TURNS * 2 * L::KEYS * 4;
+  };
+  static constexpr int LDS = lds_bytes<T, DT, Form>();
+  static constexpr int BLOCKS = HELD<T, DT> ? 2 : blocks(LDS, sizeof(T) == 4 && DT == 128);
+  template <bool SPLITS> static FM_DEVICE bool run(const Attn& a, unsigned char* lds);
+};
+template <typename T, int DT, int WK, int WR>
+__global__ __launch_bounds__(64 * WK * WR, (KeyGradients<T, DT, WK, WR>::BLOCKS)) void attention_dkv_kernel(Attn a) {
+  __shared__ __attribute__((aligned(1024))) unsigned char lds[KeyGradients<T, DT, WK, WR>::LDS];
+  if constexpr (SPLIT<T, DT>) {
+    if (!KeyGradients<T, DT, WK, WR>::template run<true>(a, lds)) KeyGradients<T, DT, WK, WR>::template run<false>(again(a), lds);
+  } else {
+    KeyGradients<T, DT, WK, WR>::template run<false>(a, lds);
+  }
+}
 
 template <typename T, int DT, int WK, int WR>
-__global__ __launch_bounds__(64 * WK * WR,
-                             (HELD<T, DT> ? 2 : Tiling<T, DT, WK, WR>::template blocks<sizeof(T) == 4 && DT == 128>()))
-void attention_dkv_kernel(Attn a) {
-  typedef Elem<T> E;
-  constexpr int KEEP = HELD_BYTES<T, DT, WK>, WAVES = WK * WR;
-  typedef Tiling<T, DT, WK, WR, KEEP> L;  // rows in the place of keys
-  constexpr int NS = DT / E::STEP, ND = DT / 32, ROWS = L::KEYS;
-  __shared__ __attribute__((aligned(1024))) unsigned char lds[L::LDS + L::STAGES * 2 * ROWS * 4];
+template <bool SPLITS>
+FM_DEVICE bool KeyGradients<T, DT, WK, WR>::run(const Attn& a, unsigned char* lds) {
+  typedef Form<SPLITS> F;
+  typedef typename F::L L;  // rows in the place of keys
+  constexpr int KEEP = F::KEEP, TURNS = F::TURNS, WAVES = WK * WR;
+  constexpr int ND = DT / 32, ROWS = L::KEYS;
+  typedef Engine<T, DT, ROWS, SPLITS> G;
   float(*stat)[2][ROWS] = reinterpret_cast<float(*)[2][ROWS]>(lds + L::LDS);  // [stage]: lse, rowsum(dO O)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wk = wave % WK, wr = wave / WK, half = lane >> 5;
-  typedef Reads<T, DT> R;
+  typedef typename G::R R;
   const unsigned row_lane = R::row_lane(lane), col_lane = R::col_lane(lane);
   const int b = blockIdx.x / a.KV, kh = blockIdx.x - b * a.KV;
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S, past = a.S - a.T;
@@ -735,9 +1012,10 @@ void attention_dkv_kernel(Attn a) {
 
   const T* qp = static_cast<const T*>(a.q.p) + b * a.q.batch + kh * a.G * a.q.head;
   const T* gp = static_cast<const T*>(a.dout.p) + b * a.dout.batch + kh * a.G * a.dout.head;
+  RowTiles<T, DT, ROWS, SPLITS> next;
+  float most = 0.0f;
   auto load = [&](int i) {
-    const int r0 = r_lo + i * ROWS, t0 = (int)fm_div(r0, a.by_g), stage = i % L::STAGES;
-    unsigned char* at = lds + KEEP + stage * 2 * L::TILE;
+    const int r0 = r_lo + i * ROWS, t0 = (int)fm_div(r0, a.by_g), stage = i % TURNS;
     auto offset = [&](const View& v) {
       return [&, rs = (int)(v.row * (long)sizeof(T)), hs = (int)(v.head * (long)sizeof(T))](int u) {
         const int r = r0 + u;
@@ -746,8 +1024,14 @@ void attention_dkv_kernel(Attn a) {
         return (t - t0) * rs + (r - t * a.G) * hs;
       };
     };
-    load_tile<T, DT, ROWS, WAVES>(qp + t0 * a.q.row, at, a.D, wave, lane, offset(a.q));
-    load_tile<T, DT, ROWS, WAVES>(gp + t0 * a.dout.row, at + L::TILE, a.D, wave, lane, offset(a.dout));
+    if constexpr (SPLITS) {
+      G::bring(qp + t0 * a.q.row, a.D, next.q, offset(a.q));
+      G::bring(gp + t0 * a.dout.row, a.D, next.g, offset(a.dout));
+    } else {
+      unsigned char* at = lds + KEEP + stage * 2 * L::TILE;
+      load_tile<T, DT, ROWS, WAVES>(qp + t0 * a.q.row, at, a.D, wave, lane, offset(a.q));
+      load_tile<T, DT, ROWS, WAVES>(gp + t0 * a.dout.row, at + L::TILE, a.D, wave, lane, offset(a.dout));
+    }
     // The rows' statistics, by direct copies as well: a value that passed through
     // registers would make this tile's copies be waited for.  A row past the last
     // reads zeros, which its zero operands leave without effect.
@@ -765,23 +1049,35 @@ void attention_dkv_kernel(Attn a) {
   // From the last rows back: every block of a head sees those, so blocks that run
   // at the same time read the same rows.
   if (tiles) load(tiles - 1);
-  typename E::Frag kf[NS], vf[NS];
+  typename G::Held kf, vf;
   const int at_key = min(key, a.S - 1);
   const T* kp = static_cast<const T*>(a.k.p) + b * a.k.batch + kh * a.k.head;
   const T* vp = static_cast<const T*>(a.v.p) + b * a.v.batch + kh * a.v.head;
-  if constexpr (KEEP > 0) {
+  if constexpr (SPLITS) {
+    G::load(kp + at_key * a.k.row, live, a.D, lane, kf);
+    G::here(kf);
+    typedef Engine<T, DT, 32 * WK, true> V;
+    typename V::Flight values;
+    const int n = min(len, k0 + 32 * WK) - 1 - k0, vs = (int)(a.v.row * (long)sizeof(T));
+    V::bring(vp + k0 * a.v.row, a.D, values, [&](int r) { return r <= n ? r * vs : -1; });
+    most = V::publish(values, lds, kf.most);
+  } else if constexpr (KEEP > 0) {
     load_keys<T, DT, 32 * WK, WAVES>(a, kp, vp, k0, min(len, k0 + 32 * WK) - 1, lds, wave, lane);
   } else {
-    load_row<T, DT>(kp + at_key * a.k.row, live, a.D, lane, kf);
-    load_row<T, DT>(vp + at_key * a.v.row, live, a.D, lane, vf);
-    arrive(kf), arrive(vf);
+    G::load(kp + at_key * a.k.row, live, a.D, lane, kf);
+    G::load(vp + at_key * a.v.row, live, a.D, lane, vf);
+    G::here(kf), G::here(vf);
   }
   floatx16 ak[ND] = {}, av[ND] = {};
   for (int i = tiles - 1; i >= 0; --i) {
     tile_barrier();
-    if (L::STAGES == 2 && i > 0) load(i - 1);
-    const int stage = i % L::STAGES;
-    const unsigned char* qt = lds + KEEP + stage * 2 * L::TILE;
+    if constexpr (SPLITS) {
+      most = G::publish(next.g, lds + KEEP + L::TILE, G::publish(next.q, lds + KEEP, most));
+      lds_barrier();
+    }
+    if ((L::STAGES == 2 || SPLITS) && i > 0) load(i - 1);
+    const int stage = i % TURNS;
+    const unsigned char* qt = lds + KEEP + (SPLITS ? 0 : stage * 2 * L::TILE);
 #pragma unroll
     for (int nb = 0; nb < L::NB; ++nb) {
       const int row = (wr * L::NB + nb) * 32, r0 = r_lo + i * ROWS + row;
@@ -790,13 +1086,16 @@ void attention_dkv_kernel(Attn a) {
       if (w0 > hi || w0 + 31 <= lo - a.window) continue;  // no row here sees these keys
       floatx16 s = {}, dp = {};
       const unsigned at = R::fresh(R::lds(qt) + row * R::PITCH + row_lane);
-      if constexpr (KEEP > 0) {
+      if constexpr (SPLITS) {
+        G::products(at, kf, s);
+        G::template products<KEEP / 3>(at + L::TILE, R::fresh(R::lds(lds) + 32 * wk * R::PITCH + row_lane), dp);
+      } else if constexpr (KEEP > 0) {
         const unsigned held = R::fresh(R::lds(lds) + 32 * wk * R::PITCH + row_lane);
-        products<T, DT, NS>(at, held, s);
-        products<T, DT, NS>(at + L::TILE, held + KEEP / 2, dp);
+        G::products(at, held, s);
+        G::products(at + L::TILE, held + KEEP / 2, dp);
       } else {
-        products<T, DT>(at, kf, s);
-        products<T, DT>(at + L::TILE, vf, dp);
+        G::products(at, kf, s);
+        G::products(at + L::TILE, vf, dp);
       }
       const bool edge = w0 + 31 > lo || w0 <= hi - a.window;
 #pragma unroll
@@ -820,23 +1119,16 @@ void attention_dkv_kernel(Attn a) {
         }
       }
       const unsigned to = R::fresh(R::lds(qt) + row * R::PITCH + col_lane);
-#pragma unroll
-      for (int c = 0; c < 32 / E::STEP; ++c) {
-        const typename E::Frag p = E::pack(s, c), ds = E::pack(dp, c);
-        typename E::Frag f[ND];
-        R::cols(to + L::TILE, c, f);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) av[d] = E::mma(f[d], p, av[d]);
-        R::cols(to, c, f);
-#pragma unroll
-        for (int d = 0; d < ND; ++d) ak[d] = E::mma(f[d], ds, ak[d]);
-      }
+      G::template outer<false>(to + L::TILE, s, av);
+      G::template outer<false>(to, dp, ak);
     }
-    if (L::STAGES == 1 && i > 0) {
+    if (L::STAGES == 1 && !SPLITS && i > 0) {
       tile_barrier();
       load(i - 1);
     }
   }
+  if constexpr (SPLITS)
+    if (__syncthreads_or(most >= BIG)) return false;
   constexpr int MINE = DT / 2 / WR;
   const long row_index = ((long)b * a.S + key) * a.KV + kh;
 #pragma unroll
@@ -850,17 +1142,10 @@ void attention_dkv_kernel(Attn a) {
 #pragma unroll
       for (int i = 0; i < MINE; ++i) mine[i] = acc[i / 16][i % 16];
     }
-    if (key >= a.S) continue;
-    T* o = static_cast<T*>(which ? a.dv : a.dk) + row_index * a.D;
-    const float f = which ? 1.0f : a.scale;
-#pragma unroll
-    for (int i = 0; i < MINE; i += 4) {
-      const int e = wr * MINE + i, d = 32 * (e / 16) + 8 * (e % 16 / 4) + 4 * half;
-      if (d < a.D)  // padding takes no gradient
-        E::store4(o + d, live ? mine[i] * f : 0.0f, live ? mine[i + 1] * f : 0.0f, live ? mine[i + 2] * f : 0.0f,
-                  live ? mine[i + 3] * f : 0.0f);
-    }
+    if (key < a.S)  // padding takes no gradient
+      store_row(static_cast<T*>(which ? a.dv : a.dk) + row_index * a.D, mine, which ? 1.0f : a.scale, live, wr * MINE, half, a.D);
   }
+  return true;
 }
 
 enum { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };

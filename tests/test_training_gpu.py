@@ -258,6 +258,49 @@ def test_attention_minus_infinity_keys():
     ref.assert_within("out", out[:, 3:], want["out"], bound["out"])
 
 
+@pytest.mark.parametrize("b,t,h,kv,pick", [(1, 70, 2, 1, [0]), (40, 160, 8, 8, [0, 39]), (24, 140, 16, 16, [3])])
+def test_attention_values_near_the_types_largest(b, t, h, kv, pick):
+    """FP32 factors that have no bf16 pieces (2^127 and more) among ordinary ones,
+    as a value, a key, a query and a gradient, in blocks of every kind."""
+    q, k, v, grad = attention_case(b, t, t, h, kv, 64, torch.float32, 8)
+    grad = grad * 1e-3
+    for i in pick:
+        v[i, 5, 0, 3] = 3.399e38
+        v[i, 20, 0, 1] = -2.0 ** 127
+    q[pick[0], 9, 0, 2], k[pick[0], :, 0, 2] = 2.0e38, k[pick[0], :, 0, 2] * 1e-38
+    got = attention_run(q, k, v, grad, None)
+    part = [x[pick] for x in (q, k, v, grad)]
+    want, bound = ref.attention(*part, None, 0.125, None)
+    most, got = torch.finfo(torch.float32).max, {n: x[pick].double().cpu() for n, x in got.items()}
+    for n, x in want.items():
+        # dS, near 1e34 through the largest value, times the query 2e38 leaves FP32:
+        # what exceeds the type's largest value by more than its bound rounds to infinity.
+        over = (x.abs() - ref.SECOND_ORDER * bound[n].expand_as(x) > most) & (n in ("dq", "dk"))
+        assert torch.equal(got[n][over], x[over].sign() * math.inf), n
+        got[n], want[n] = got[n].masked_fill(over, 0.0), x.masked_fill(over, 0.0)
+    check(got, (want, bound))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_infinities_reach_what_sees_them(dtype):
+    """An infinite key scores minus infinity against positive queries (no
+    probability) and an infinite value makes the rows that see it infinite; an
+    infinite gradient reaches the keys its row sees. The rows before them, in
+    other tiles, are as they were."""
+    q, k, v, grad = attention_case(1, 130, 130, 1, 1, 64, dtype, 9)
+    q = q.abs()
+    clean = attention_run(q, k, v, grad, None)
+    v[0, 100, 0, 7] = math.inf
+    got = attention_run(q, k, v, grad, None)
+    assert torch.equal(got["out"][0, :96], clean["out"][0, :96])
+    assert (got["out"][0, 100:, 0, 7] == math.inf).all()
+    assert torch.isfinite(got["out"][0, 100:, 0, :7]).all()
+    v[0, 100, 0, 7] = 0.0
+    grad[0, 3, 0, 2] = math.inf
+    got = attention_run(q, k, v, grad, None)
+    assert (got["dv"][0, :4, 0, 2] == math.inf).all() and torch.isfinite(got["dv"][0, 64:]).all()
+
+
 def test_attention_scale_and_window_beyond_the_keys():
     q, k, v, grad = attention_case(1, 60, 60, 2, 2, 64, torch.float32, 7)
     check(attention_run(q, k, v, grad, 10 ** 9, 0.5), ref.attention(q, k, v, grad, None, 0.5, None))
