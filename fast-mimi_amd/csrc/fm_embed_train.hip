@@ -368,13 +368,14 @@ Embed embed_sizes(int batch, int books, int frames, int entries, int dim, float 
   a.by_frames = fm_divisor((unsigned)std::max(frames, 1));
   // Runs of at least sqrt(rows) / 2 rows: a code that owns every row is then at
   // most four times as many parts as a run has rows.
+  const long rows = std::min(a.rows, 1l << 30);  // more are refused
   a.run_rows = 64;
-  while (4l * a.run_rows * a.run_rows < a.rows) a.run_rows *= 2;
+  while (4l * a.run_rows * a.run_rows < rows) a.run_rows *= 2;
   a.runs = a.rows >= a.run_rows ? (int)((a.rows + a.run_rows - 1) / a.run_rows) : 0;
   // The sort's chunks: 4096 rows are a block's time; more than 16 would make
   // their counts the larger part.
   a.chunk_rows = 4096;
-  while (16l * a.chunk_rows < a.rows) a.chunk_rows *= 2;
+  while (16l * a.chunk_rows < rows) a.chunk_rows *= 2;
   a.chunks = (int)std::max<long>(1, (a.rows + a.chunk_rows - 1) / a.chunk_rows);
   return a;
 }

@@ -361,6 +361,18 @@ int run(Norm a, bool back, hipStream_t stream) {
     hipLaunchKernelGGL((norm_zero_kernel<W>), dim3(fm_ceil_div(a.C, 256)), dim3(256), 0, stream, a);
     return (int)hipGetLastError();
   }
+  constexpr long MOST = 1 << 23;  // rows of a forward launch: a grid has at most 2^32 threads
+  if (!back && a.rows > MOST) {
+    Norm part = a;
+    for (long first = 0; first < a.rows; first += MOST) {
+      part.rows = std::min(MOST, a.rows - first);
+      part.x = static_cast<const T*>(a.x) + first * a.ld_x;
+      part.y = static_cast<T*>(a.y) + first * a.C;
+      part.mean = a.mean + first, part.rstd = a.rstd + first;
+      if (const int status = run<T, W>(part, false, stream)) return status;
+    }
+    return FM_OK;
+  }
   a.blocks = back ? backward_blocks(a.rows, p, sizeof(T)) : 0;
   if (p.nv == 0) {
     if (back)

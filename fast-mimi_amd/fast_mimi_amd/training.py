@@ -299,7 +299,8 @@ def window_attention_forward(q, k, v, window: int | None = None, scale: float | 
     for :func:`window_attention_backward`.
 
     An infinity or NaN in a visible key or value may reach other rows near it;
-    what padding holds reaches nothing.
+    what padding holds reaches nothing.  At most 2097120 keys, and queries times
+    heads per key head.
     """
     q, k, v, window, scale, lengths = _attention_input(q, k, v, window, scale, lengths)
     device = _on_gpu(q=q, k=k, v=v, lengths=lengths)
@@ -385,7 +386,8 @@ def code_embedding_forward(codes, table, scale: float = 1.0):
     """``scale * sum_q table[q, codes[:, q]]``: ``[batch, frames, dim]`` of ``table``'s type.
 
     ``codes`` is int64 ``[batch, codebooks, frames]``, ``table``
-    ``[codebooks, entries, dim]`` (at most 32768 entries).  Code -1 is absent
+    ``[codebooks, entries, dim]`` (at most 32768 entries; 2097120 frames in
+    all).  Code -1 is absent
     and adds nothing (padding, delayed codebooks); any other code outside the
     table makes its frame NaN, as ``rvq_decode`` does.  The split quantizer's
     two sums are two calls, on ``codes[:, :n]`` / ``table[:n]`` and the rest.
@@ -422,15 +424,15 @@ def code_embedding_backward(grad, codes, table, scale: float = 1.0):
 class _CodeEmbedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, codes, scale):
-        ctx.save_for_backward(table, codes)
-        ctx.scale = scale
+        ctx.save_for_backward(codes)
+        # Of the table only the shape matters: it may change before the backward pass.
+        ctx.how = table.detach(), scale
         return code_embedding_forward(codes, table, scale)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        table, codes = ctx.saved_tensors
-        return code_embedding_backward(grad, codes, table, ctx.scale), None, None
+        return code_embedding_backward(grad, *ctx.saved_tensors, *ctx.how), None, None
 
 
 def code_embedding(codes, table, scale: float = 1.0):

@@ -549,7 +549,7 @@ enum { FM_DTYPE_F32 = 0, FM_DTYPE_BF16 = 1, FM_DTYPE_F16 = 2 };
  * y = (x - mean) rstd gamma + beta, rstd = 1 / sqrt(biased variance + eps).
  * x has rows of `channels` elements at a pitch of ld_x elements; y is
  * contiguous; mean and rstd are [rows].  gamma / beta may be NULL (one /
- * zero); weight_dtype is theirs: dtype, or FP32.
+ * zero); weight_dtype is theirs: dtype, or FP32.  Fewer than 2^31 - 1 rows.
  * Replaces nn.LayerNorm in MimiTransformerLayer (model.py:2028-2061) where
  * the layer is trained.
  */
@@ -581,7 +581,8 @@ int fm_layer_norm_backward(const void* dy, long ld_dy, const void* x, long ld_x,
  * h / (heads / kv_heads).  q / k / v are strided (strides in elements of the
  * batch, position and head dimensions; a packed projection is such a view);
  * rows must be 16-byte aligned, head_dim <= 128 a multiple of 8 (FP32: 4),
- * scale positive.  out [batch][queries][heads][head_dim] and lse
+ * scale positive; at most 2097120 keys, and rows per key head (queries x heads /
+ * kv_heads), 2^23 sequences x key heads, 2^20 heads.  out [batch][queries][heads][head_dim] and lse
  * [batch][queries][heads] (log2 of the row's sum of exponentials, -inf for a
  * row without keys) are contiguous.  A visible key or value row that holds an
  * infinity or NaN may reach other rows of its 32-row tiles.
@@ -621,7 +622,8 @@ int fm_attention_backward(const void* dout, long dout_batch, long dout_row, long
  * codes_book (elements; frames adjacent), table [books][entries][dim] and out
  * [batch][frames][dim] contiguous, of dtype.  Code -1 is absent (adds
  * nothing); any other code outside [0, entries) gives NaN, as in
- * fm_rvq_decode.  At most 32768 entries.
+ * fm_rvq_decode.  At most 32768 entries, 65535 codebooks, 2097120 frames in all
+ * (batch x frames).
  * Replaces the codebook sum of MimiResidualVectorQuantizer.decode
  * (model.py:2430-2444) where the codebooks are trained.
  */

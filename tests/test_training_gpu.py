@@ -122,6 +122,18 @@ def test_layer_norm_many_elements():
     check(got, ref.norm(tail, grad, w, b, 1e-5))
 
 
+def test_layer_norm_more_rows_than_a_grid_holds():
+    rows, c = (1 << 24) + 9, 8
+    tail, _, w, b = norm_case(7, c, torch.bfloat16, torch.float32, 7)
+    x = torch.zeros(rows, c, dtype=torch.bfloat16, device=DEV)
+    first = 1 << 23
+    for at in (0, first - 7, first, rows - 7):
+        x[at:at + 7] = tail
+    got, want = tr.layer_norm_forward(x, w, b), tr.layer_norm_forward(tail, w, b)
+    for at in (0, first - 7, first, rows - 7):
+        assert all(torch.equal(t[at:at + 7], s) for t, s in zip(got, want)), at
+
+
 # ---------------------------------------------------------------- attention
 def attention_case(b, t, s, h, kv, d, dtype, seed=0, packed=False):
     g = gen(seed)
@@ -256,6 +268,32 @@ def test_attention_minus_infinity_keys():
     # The type's lowest values are far below every other score and above none.
     out = tr.window_attention_forward(q, lowest, v)[0]
     ref.assert_within("out", out[:, 3:], want["out"], bound["out"])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_minus_infinity_keys_have_no_gradient(dtype):
+    """Probability zero in every row, also beside the rows that fill up a tile."""
+    q, k, v, grad = attention_case(1, 40, 40, 2, 1, 64, dtype, 6)
+    q = q.abs()
+    k[:, :3] = -math.inf
+    got = attention_run(q, k, v, grad, None)
+    assert not got["dk"][:, :3].any() and not got["dv"][:, :3].any()
+    want, bound = ref.attention(q[:, 3:], k[:, 3:], v[:, 3:], grad[:, 3:], None, 0.125, None)
+    for n in ("out", "dk", "dv"):
+        ref.assert_within(n, got[n][:, 3:], want[n], bound[n])
+
+
+def test_attention_scores_that_overflow():
+    """Scores of -1e42 are minus infinity in FP32: no probability, no gradient, as
+    for a key whose score is far below the others but finite."""
+    q, k, v, grad = attention_case(1, 80, 80, 2, 2, 64, torch.float32, 10)
+    q[..., 0] = 1e21 * (1 + q[..., 0].abs())
+    k[..., 0] = 0.0
+    low = k.clone()
+    k[:, 5, :, 0], low[:, 5, :, 0] = -1e21, -1e-17
+    got = attention_run(q, k, v, grad, None)
+    assert not got["dk"][:, 5].any() and not got["dv"][:, 5].any()
+    check(got, ref.attention(q, low, v, grad, None, 0.125, None))
 
 
 @pytest.mark.parametrize("b,t,h,kv,pick", [(1, 70, 2, 1, [0]), (40, 160, 8, 8, [0, 39]), (24, 140, 16, 16, [3])])
@@ -406,6 +444,16 @@ def test_embedding_matches_the_decoders_sum():
     out = out.view(2, 33, 512)
     assert torch.equal(tr.code_embedding_forward(codes[:, :1], table[:1]), out[..., :256])
     assert torch.equal(tr.code_embedding_forward(codes[:, 1:], table[1:]), out[..., 256:])
+
+
+def test_embedding_table_may_change_before_the_backward_pass():
+    codes, table, grad = embedding_case(2, 3, 40, 32, 64, torch.float32, 8)
+    table.requires_grad_()
+    out = tr.code_embedding(codes, table)
+    with torch.no_grad():
+        table.mul_(2.0)
+    out.backward(grad)
+    assert torch.equal(table.grad, tr.code_embedding_backward(grad, codes, table))
 
 
 def test_embedding_far_entries():

@@ -84,6 +84,7 @@ def attention(**change):
     (1000, dict(scale=0.0)), (1000, dict(scale=float("nan"))), (1000, dict(dtype=3)), (1000, dict(q=None)), (1000, dict(out=None)),
     (1002, dict(head_dim=136)), (1002, dict(head_dim=60)), (1002, dict(q=P + 2)), (1002, dict(row=129)), (1002, dict(row=1 << 40)),
     (1002, dict(head=-64)), (1002, dict(out=P + 4)), (1002, dict(queries=1 << 30, keys=1 << 30)),
+    (1000, dict(scale=3e38)), (1002, dict(keys=2_097_121)), (1002, dict(batch=1 << 23)), (1002, dict(heads=1 << 21, kv_heads=1)),
     (1001, dict(queries=1, keys=100_000, window=100_000)),
     (0, dict(batch=0)), (0, dict(queries=0)),
 ])
