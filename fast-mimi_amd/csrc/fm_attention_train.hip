@@ -314,9 +314,12 @@ struct Engine {
 // FP32 from the smallest: 768 matrix cycles per 32x32x64 where the FP32 MFMA takes
 // 2048, at its error.  A block's threads bring the next tile into registers, and
 // split it into three planes in LDS once all waves are done with the last one.
-// Infinities have no such pieces (their products with the others' remainders are
-// infinities of either sign): a block that meets a value of 2^127 or more starts
-// again on FP32 MFMAs.
+// An infinity has no such pieces, and where a product overflows, so may those of
+// its factors' remainders, with either sign.  A block that meets a value of 2^36
+// or more starts again on FP32 MFMAs: below, scores stay under 2^78, dS under 2^81
+// and no product or sum of them comes near the largest value.  (At the other end
+// a piece may be lost below 2^-126: of values under 2^-102 more than an FP32
+// rounding, and never more than 2^-126 of any.)
 // 16 x 2500 frames, 8 heads, window 250: forward 250 -> 170 us, dQ 355 -> 270,
 // dK / dV 500 -> 335 (there the matrix cores and the vector work, half of it the
 // splitting, take turns).
@@ -571,7 +574,7 @@ FM_DEVICE void load_keys(const Attn& a, const T* kp, const T* vp, int k0, int k_
   load_tile<T, DT, KEYS, WAVES>(vp + k0 * a.v.row, at + TILE, a.D, wave, lane, [&](int r) { return r <= n ? r * vs : -1; });
 }
 
-constexpr float BIG = 1.7014118346046923e38f;  // 2^127
+constexpr float BIG = 68719476736.0f;  // 2^36
 
 // KEEP: bytes of LDS that a dK / dV block keeps its keys and values in.
 template <typename T, int DT, int WQ, int WK, bool SPLITS, int KEEP = 0>
@@ -1097,7 +1100,8 @@ FM_DEVICE bool KeyGradients<T, DT, WK, WR>::run(const Attn& a, unsigned char* ld
         G::products(at, kf, s);
         G::products(at + L::TILE, vf, dp);
       }
-      const bool edge = w0 + 31 > lo || w0 <= hi - a.window;
+      // Rows past the last are zeros, whose products with infinities are not.
+      const bool edge = w0 + 31 > lo || w0 <= hi - a.window || r0 + 31 > r_hi;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const floatx4 lse = *reinterpret_cast<const floatx4*>(&stat[stage][0][row + 8 * g + 4 * half]);
@@ -1112,8 +1116,8 @@ FM_DEVICE bool KeyGradients<T, DT, WK, WR>::run(const Attn& a, unsigned char* ld
       if (edge) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int p = past + (int)fm_div(r0 + 8 * (e >> 2) + 4 * half + (e & 3), a.by_g);
-          const bool ok = key <= p && key > p - a.window;
+          const int r = r0 + 8 * (e >> 2) + 4 * half + (e & 3), p = past + (int)fm_div(r, a.by_g);
+          const bool ok = key <= p && key > p - a.window && r <= r_hi;
           s[e] = ok ? s[e] : 0.0f;
           dp[e] = ok ? dp[e] : 0.0f;
         }
@@ -1152,12 +1156,13 @@ enum { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };
 
 int check(const Attn& a, int dtype) {
   if (a.B < 0 || a.T < 0 || a.S < 0 || a.H <= 0 || a.KV <= 0 || a.D <= 0 || a.window <= 0 || !(a.scale > 0.0f) ||
-      a.scale == INFINITY || a.H % a.KV || a.T > a.S || dtype < DT_F32 || dtype > DT_F16)
+      a.scale2 == INFINITY || a.H % a.KV || a.T > a.S || dtype < DT_F32 || dtype > DT_F16)
     return FM_BAD_ARGUMENT;
   const int unit = dtype == DT_F32 ? 4 : 8, size = dtype == DT_F32 ? 4 : 2;
   if (a.D > 128 || a.D % unit) return FM_UNSUPPORTED;
-  if ((long)a.T * a.G >= INT_MAX - 256 || a.S >= INT_MAX - 256 || (long)a.B * a.KV >= INT_MAX) return FM_UNSUPPORTED;
-  if (((long)a.T * a.G + 31) / 32 > 65535 || (a.S + 31) / 32 > 65535) return FM_UNSUPPORTED;
+  // A grid holds 65535 blocks of 32 rows or keys and 2^23 sequences (heads: offsets
+  // of a tile's statistics).
+  if ((long)a.T * a.G > 32l * 65535 || a.S > 32 * 65535 || (long)a.B * a.KV > 1 << 23 || a.H > 1 << 20) return FM_UNSUPPORTED;
   for (const View* v : {&a.q, &a.k, &a.v, &a.dout}) {
     if (!v->p) continue;
     // 16-byte rows, and a tile's rows within reach of 32-bit offsets.
