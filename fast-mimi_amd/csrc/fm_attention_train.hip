@@ -506,7 +506,7 @@ FM_DEVICE void tile_barrier() {
 // the keys they see.
 template <int WQ>
 struct Rows {
-  int b, kh, len, R, r, t, p, p_lo, p_hi, k_lo, k_hi;
+  int b, kh, len, R, r, t, p, p_lo, p_hi, b_lo, k_lo, k_hi;
   bool live;
   long row_index;  // into [B][T][H]
   FM_DEVICE Rows(const Attn& a, int wq, int lane) {
@@ -524,7 +524,7 @@ struct Rows {
     live = r < R && p < len;
     row_index = ((long)b * a.T + t) * a.H + kh * a.G + (min(r, R - 1) - t * a.G);
     // The block's keys.
-    const int b_lo = past + (int)fm_div(r0, a.by_g);
+    b_lo = past + (int)fm_div(r0, a.by_g);
     const int b_hi = past + (int)fm_div(min(r0 + 32 * WQ, R) - 1, a.by_g);
     k_lo = max(0, b_lo - a.window + 1);
     k_hi = min(b_hi, len - 1);
@@ -824,7 +824,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Attn a) {
 // 16-bit inputs: dS is two 16-bit pieces here (a fourth product), as its own
 // rounding would put dQ at 1.5 times the error that rounding its result has.  And
 // rowsum(dO O) from the rounded O is only nearly the sum over P dP; the sum of dS,
-// zero but for that, puts it right for the dK / dV kernel.
+// zero but for that, puts it right for the dK / dV kernel.  Where a row sees few
+// keys it would also be most of dQ's error (1.5 times the rounding's with 4 keys,
+// less than 1.1 from 32 on): blocks with such rows go over their keys twice.
 template <typename T, int DT, int WQ, int WK>
 struct QueryGradient {
   template <bool SPLITS>
@@ -848,7 +850,6 @@ __global__ __launch_bounds__(256, (QueryGradient<T, DT, WQ, WK>::BLOCKS)) void a
 template <typename T, int DT, int WQ, int WK>
 template <bool SPLITS>
 FM_DEVICE bool QueryGradient<T, DT, WQ, WK>::run(const Attn& a, unsigned char* lds) {
-  typedef Elem<T> E;
   typedef Tiling<T, DT, WQ, WK, SPLITS> L;
   typedef Engine<T, DT, L::KEYS, SPLITS> G;
   constexpr int ND = DT / 32;
@@ -878,59 +879,76 @@ FM_DEVICE bool QueryGradient<T, DT, WQ, WK>::run(const Attn& a, unsigned char* l
   lse = lse == -INFINITY ? INFINITY : lse;
   float rest = 0.0f;  // the sum of dS: what the rounding of O took from delta
 
+  // The row's sum over both lane halves and all the waves that share it.
+  auto total = [&]() {
+    float sum = half_sum(rest);
+    if constexpr (WK > 1) {
+      float(*rests)[32] = reinterpret_cast<float(*)[32]>(lds + L::LDS) + WK * wq;
+      if (half == 0) rests[wk][lane] = sum;
+      __syncthreads();
+      sum = 0.0f;
+#pragma unroll
+      for (int u = 0; u < WK; ++u) sum += rests[u][lane & 31];
+    }
+    return sum;
+  };
+
   floatx16 acc[ND] = {};
   G::here(q), G::here(g);
   float row_stats[2] = {lse, delta};
   arrive(row_stats);
   lse = row_stats[0], delta = row_stats[1];
-  for (int i = 0; i < tiles; ++i) {
-    tile_barrier();
-    if constexpr (SPLITS) most = next.publish(lds, most);
-    if ((L::STAGES == 2 || SPLITS) && i + 1 < tiles) load(i + 1);
-    const unsigned char* kt = lds + i % L::STAGES * 2 * L::TILE;
-    const unsigned char* vt = kt + L::TILE;
-#pragma unroll
-    for (int nb = 0; nb < L::NB; ++nb) {
-      const int row = (wk * L::NB + nb) * 32, k0 = w.k_lo + i * L::KEYS + row;
-      if (k0 > w.p_hi || k0 + 31 <= w.p_lo - a.window) continue;
-      floatx16 s = {}, dp = {};
-      const unsigned at = R::fresh(R::lds(kt) + row * R::PITCH + row_lane);
-      G::products(at, q, s);
-      G::products(at + L::TILE, g, dp);
-      const bool edge = k0 + 31 > w.p_lo || k0 <= w.p_hi - a.window || k0 + 31 > w.k_hi;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -lse));
-        s[e] = p * (dp[e] - delta);
-      }
-      if (edge) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int key = k0 + 8 * (e >> 2) + 4 * half + (e & 3);
-          s[e] = key <= w.p && key > w.p - a.window && key <= w.k_hi && w.live ? s[e] : 0.0f;
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) rest += s[e];
-      G::template outer<true>(R::fresh(R::lds(kt) + row * R::PITCH + col_lane), s, acc);
-    }
-    if (L::STAGES == 1 && !SPLITS && i + 1 < tiles) {
+  // With few keys (some row sees fewer than FEW) a first pass makes delta exact.
+  constexpr int FEW = 32;
+  bool first = sizeof(T) == 2 && tiles > 0 && min(w.b_lo + 1, a.window) < FEW;
+  for (;; first = false) {
+    for (int i = 0; i < tiles; ++i) {
       tile_barrier();
-      load(i + 1);
+      if constexpr (SPLITS) most = next.publish(lds, most);
+      if ((L::STAGES == 2 || SPLITS) && i + 1 < tiles) load(i + 1);
+      const unsigned char* kt = lds + i % L::STAGES * 2 * L::TILE;
+  #pragma unroll
+      for (int nb = 0; nb < L::NB; ++nb) {
+        const int row = (wk * L::NB + nb) * 32, k0 = w.k_lo + i * L::KEYS + row;
+        if (k0 > w.p_hi || k0 + 31 <= w.p_lo - a.window) continue;
+        floatx16 s = {}, dp = {};
+        const unsigned at = R::fresh(R::lds(kt) + row * R::PITCH + row_lane);
+        G::products(at, q, s);
+        G::products(at + L::TILE, g, dp);
+        const bool edge = k0 + 31 > w.p_lo || k0 <= w.p_hi - a.window || k0 + 31 > w.k_hi;
+  #pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -lse));
+          s[e] = p * (dp[e] - delta);
+        }
+        if (edge) {
+  #pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int key = k0 + 8 * (e >> 2) + 4 * half + (e & 3);
+            s[e] = key <= w.p && key > w.p - a.window && key <= w.k_hi && w.live ? s[e] : 0.0f;
+          }
+        }
+  #pragma unroll
+        for (int e = 0; e < 16; ++e) rest += s[e];
+        if (!first) G::template outer<true>(R::fresh(R::lds(kt) + row * R::PITCH + col_lane), s, acc);
+      }
+      if (L::STAGES == 1 && !SPLITS && i + 1 < tiles) {
+        tile_barrier();
+        load(i + 1);
+      }
     }
+    if (!first) break;
+    tile_barrier();  // every wave is past the last tile
+    load(0);
+    rest = total();
+    delta += rest, rest = 0.0f;
   }
   if constexpr (SPLITS)
     if (__syncthreads_or(fmaxf(most, fmaxf(q.most, g.most)) >= BIG)) return false;
-  rest = half_sum(rest);
+  rest = total();
   constexpr int MINE = DT / 2 / WK;
   float mine[MINE];
   if constexpr (WK > 1) {
-    float(*rests)[32] = reinterpret_cast<float(*)[32]>(lds + L::LDS) + WK * wq;
-    if (half == 0) rests[wk][lane] = rest;
-    __syncthreads();
-    rest = 0.0f;
-#pragma unroll
-    for (int u = 0; u < WK; ++u) rest += rests[u][lane & 31];
     merge<DT, WK>(reinterpret_cast<float*>(lds), acc, wq, wk, lane, mine);
   } else {
 #pragma unroll
@@ -967,6 +985,11 @@ struct RowTiles<T, DT, ROWS, true> {
 // / eight waves; 16 heads x 2 x 2048: 190, 102 / 126.
 template <typename T, int DT>
 constexpr bool HELD = sizeof(T) == 2 && DT == 128;
+//
+// The rounding of P and dS to 16 bits puts dV and dK at 1.4 times the error of
+// rounding the results.  Sums over few rows, where chance adds to that, have them
+// in two pieces; a block of that many rows is one or two tiles long.
+constexpr int FEW_ROWS = 128;
 template <typename T, int DT, int WK, int WR>
 struct KeyGradients {
   template <bool SPLITS>
@@ -1012,6 +1035,7 @@ FM_DEVICE bool KeyGradients<T, DT, WK, WR>::run(const Attn& a, unsigned char* ld
   const int p_hi = min((long)min(k0 + 32 * WK, len) - 1 + a.window - 1, (long)len - 1);
   const int r_lo = (p_lo - past) * a.G, r_hi = (p_hi - past + 1) * a.G - 1;
   const int tiles = k0 < len && p_hi >= p_lo ? (r_hi - r_lo) / ROWS + 1 : 0;
+  const bool few = sizeof(T) == 2 && r_hi - r_lo < FEW_ROWS;
 
   const T* qp = static_cast<const T*>(a.q.p) + b * a.q.batch + kh * a.G * a.q.head;
   const T* gp = static_cast<const T*>(a.dout.p) + b * a.dout.batch + kh * a.G * a.dout.head;
@@ -1123,8 +1147,14 @@ FM_DEVICE bool KeyGradients<T, DT, WK, WR>::run(const Attn& a, unsigned char* ld
         }
       }
       const unsigned to = R::fresh(R::lds(qt) + row * R::PITCH + col_lane);
-      G::template outer<false>(to + L::TILE, s, av);
-      G::template outer<false>(to, dp, ak);
+#pragma unroll 1
+      for (int pieces = few ? 2 : 1;;) {
+        G::template outer<false>(to + L::TILE, s, av);
+        G::template outer<false>(to, dp, ak);
+        if (sizeof(T) == 4 || --pieces == 0) break;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] -= (float)(T)s[e], dp[e] -= (float)(T)dp[e];
+      }
     }
     if (L::STAGES == 1 && !SPLITS && i > 0) {
       tile_barrier();

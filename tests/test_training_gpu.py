@@ -320,6 +320,38 @@ def test_attention_values_near_the_types_largest(b, t, h, kv, pick):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b,t,h,kv,d,window", [(1, 5, 1, 1, 64, 1), (3, 70, 8, 2, 64, 1), (2, 40, 2, 2, 128, 1),
+                                               (50, 200, 8, 8, 64, 1), (2, 1, 4, 4, 64, None)])
+def test_attention_one_key_has_no_query_gradient(b, t, h, kv, d, window, dtype):
+    """One visible key: dP is exactly the row's delta. What is left of dQ is FP32
+    rounding: a 16-bit output's own (u |G| |O|) must not reach it, other than times
+    the error es of a probability of one."""
+    q, k, v, grad = attention_case(b, t, t, h, kv, d, dtype, 12)
+    got = attention_run(q, k, v, grad, window)["dq"].double().cpu()
+    q, grad = q.double().cpu(), grad.double().cpu()
+    k, v = (x.double().cpu().repeat_interleave(h // kv, 2) for x in (k, v))
+    size = (grad.abs() * v.abs()).sum(-1, keepdim=True)  # no less than |dP|, |delta|
+    es = (d + 8) * ref.H * (q.abs() * k.abs()).sum(-1, keepdim=True) * d ** -0.5
+    if dtype == torch.float32:
+        ds = 2 * (d + 4) * ref.H * size
+    else:  # (1 - p) (dP - delta), and four FP32 roundings of values of that size
+        ds = es * 2 * ref.half(dtype) * size + 6 * ref.H * size
+    bound = ds * k.abs() * d ** -0.5 * 1.01 + ref.step0(dtype)
+    assert (got.abs() <= bound).all(), (got.abs() / bound).max()
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("b,t,h,kv,d,window", [(7, 4, 2, 1, 128, None), (1, 13, 8, 8, 64, None), (16, 2, 4, 4, 64, None),
+                                               (3, 30, 4, 2, 32, None), (2, 100, 4, 4, 64, 30)])
+def test_attention_gradients_of_few_rows(b, t, h, kv, d, window, dtype):
+    """Few keys and few rows: the only 16-bit rounding that counts is the gradients' own."""
+    q, k, v, grad = attention_case(b, t, t, h, kv, d, dtype, 13)
+    got = attention_run(q, k, v, grad, window)
+    del got["out"]
+    check(got, ref.attention(q, k, v, grad, window, d ** -0.5, None, pieces=2))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_attention_infinities_reach_what_sees_them(dtype):
     """An infinite key scores minus infinity against positive queries (no
     probability) and an infinite value makes the rows that see it infinite; an

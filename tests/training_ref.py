@@ -82,8 +82,12 @@ def visible(queries, keys, window, length):
     return ok if window is None else ok & (j > p - window)
 
 
-def attention(q, k, v, grad, window, scale, lengths):
-    """(values, bounds): out, dq, dk, dv in float64; padding is not read."""
+def attention(q, k, v, grad, window, scale, lengths, pieces=1):
+    """(values, bounds): out, dq, dk, dv in float64; padding is not read.
+
+    pieces=2: the gradients' bounds where 16-bit inputs keep P and dS in two
+    pieces (of relative error u^2 together) and delta is the sum over P dP.
+    """
     t = q.dtype
     b, tq, h, d = q.shape
     s, kv = k.shape[1], k.shape[2]
@@ -92,6 +96,9 @@ def attention(q, k, v, grad, window, scale, lengths):
     # FP32 inputs keep their probabilities in FP32; the hardware's exponential
     # gives zero for results below FP32's smallest normal number, 2^-126.
     up, eta = (0.0, 2.0 ** -126) if t == torch.float32 else (u, max(step0(t), 2.0 ** -126))
+    du = u
+    if pieces == 2:
+        up, du = up * up, 0.0
     val = {m: torch.zeros(x.shape, dtype=torch.float64) for m, x in (("out", q), ("dq", q), ("dk", k), ("dv", v))}
     err = {m: torch.zeros_like(x) for m, x in val.items()}
     q, k, v, grad = (x.double().cpu() for x in (q, k, v, grad))
@@ -119,7 +126,7 @@ def attention(q, k, v, grad, window, scale, lengths):
             D = (G * O).sum(1, keepdim=True)
             DS = P * (DP - D)
             edp = (d + 2) * H * (G.abs() @ V.abs().T)
-            eD = (G.abs() * (u * O.abs() + eo + step0(t) + (d + 2) * H * O.abs())).sum(1, keepdim=True)
+            eD = (G.abs() * (du * O.abs() + eo + step0(t) + (d + 2) * H * O.abs())).sum(1, keepdim=True)
             eds = ep * (DP - D).abs() + P * (edp + eD + 2 * H * (DP.abs() + D.abs())) + (up + 2 * H) * DS.abs() + eta * see
             val["out"][i, :, a] = O
             err["out"][i, :, a] = eo + u * O.abs() + step0(t)
