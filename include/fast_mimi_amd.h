@@ -584,8 +584,8 @@ int fm_layer_norm_backward(const void* dy, long ld_dy, const void* x, long ld_x,
  * scale positive; at most 2097120 keys, and rows per key head (queries x heads /
  * kv_heads), 2^23 sequences x key heads, 2^20 heads.  out [batch][queries][heads][head_dim] and lse
  * [batch][queries][heads] (log2 of the row's sum of exponentials, -inf for a
- * row without keys) are contiguous.  A visible key or value row that holds an
- * infinity or NaN may reach other rows of its 32-row tiles.
+ * row without keys) are contiguous.  An infinity or NaN outside padding may
+ * reach other rows of its 32-row tiles.
  * The workspace holds the parts of calls whose keys are split over blocks (few
  * queries over many keys); NULL where its size is 0.
  * Replaces F.scaled_dot_product_attention in MimiAttention.forward
@@ -606,7 +606,9 @@ int fm_attention_forward(const void* q, long q_batch, long q_row, long q_head, c
  * forms the probabilities again.  dout is strided as q; dq, dk and dv are
  * contiguous; stats [2][batch][queries][heads] is scratch (the rows' lse and
  * dout . out).
- * Padding takes no gradient (zeros), and its dout is not used.
+ * Padding takes no gradient (zeros), and its dout is not used.  float16: the
+ * probability times dout . v - dout . out is an operand of that type; past 65504
+ * the gradients are not finite.
  */
 int fm_attention_backward(const void* dout, long dout_batch, long dout_row, long dout_head,
                           const void* q, long q_batch, long q_row, long q_head, const void* k,
