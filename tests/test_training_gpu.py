@@ -50,6 +50,15 @@ def test_layer_norm(rows, c, dtype):
     check(norm_run(x, grad, w, b), ref.norm(x, grad, w, b, 1e-5))
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [1, 8, 9, 32, 33, 1100])
+@pytest.mark.parametrize("c", [511, 516, 1023, 1028, 2049, 2052, 4099, 4104, 8191, 8192, 8193, 8200])
+def test_layer_norm_plans(rows, c, dtype):
+    """Every number of lanes and vectors per row, at its edges, alone and in many blocks."""
+    x, grad, w, b = norm_case(rows, c, dtype, torch.float32, rows)
+    check(norm_run(x, grad, w, b), ref.norm(x, grad, w, b, 1e-5))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("weight,bias", [(True, True), (True, False), (False, True), (False, False)])
 def test_layer_norm_fp32_weights(dtype, weight, bias):
