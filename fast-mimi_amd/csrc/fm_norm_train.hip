@@ -85,6 +85,23 @@ __global__ __launch_bounds__(256) void norm_forward_kernel(Norm a) {
 #pragma unroll
     for (int e = 0; e < E; ++e) v[u][e] = widen(t[e]), s += v[u][e];
   }
+  // The weights are on their way during the sums, where the registers allow (20000
+  // rows: 8192 bfloat16 channels 144 -> 124 us, 2047 64 -> 51; 4095, with 32 single
+  // elements a lane, 263 -> 293).
+  constexpr bool EARLY = NV * E <= (E == 1 ? 8 : 32);
+  const VW* w = static_cast<const VW*>(a.w);
+  const VW* b = static_cast<const VW*>(a.b);
+  VW wv[NV], bv[NV];
+  auto weights = [&](int u) {
+    const int i = p + u * LPR;
+    wv[u] = bv[u] = VW{};
+    if (w && i < n) wv[u] = w[i];
+    if (b && i < n) bv[u] = b[i];
+  };
+  if constexpr (EARLY) {
+#pragma unroll
+    for (int u = 0; u < NV; ++u) weights(u);
+  }
   const float mean = row_sum<LPR>(s, waves[0]) / (float)a.C;
   float q = 0.0f;
 #pragma unroll
@@ -97,18 +114,14 @@ __global__ __launch_bounds__(256) void norm_forward_kernel(Norm a) {
   const float rstd = 1.0f / sqrtf(row_sum<LPR>(q, waves[1]) / (float)a.C + a.eps);
   if (p == 0) a.mean[row] = mean, a.rstd[row] = rstd;
   VT* y = reinterpret_cast<VT*>(static_cast<T*>(a.y) + row * a.C);
-  const VW* w = static_cast<const VW*>(a.w);
-  const VW* b = static_cast<const VW*>(a.b);
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
     const int i = p + u * LPR;
     if (i >= n) break;
-    VW wv{}, bv{};
-    if (w) wv = w[i];
-    if (b) bv = b[i];
+    if constexpr (!EARLY) weights(u);
     VT t;
 #pragma unroll
-    for (int e = 0; e < E; ++e) t[e] = (T)fmaf(v[u][e] * rstd, w ? widen(wv[e]) : 1.0f, b ? widen(bv[e]) : 0.0f);
+    for (int e = 0; e < E; ++e) t[e] = (T)fmaf(v[u][e] * rstd, w ? widen(wv[u][e]) : 1.0f, b ? widen(bv[u][e]) : 0.0f);
     y[i] = t;
   }
 }
