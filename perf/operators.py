@@ -12,7 +12,6 @@ With ``own`` false, ``run`` computes the same from elementary torch operations i
 
 from __future__ import annotations
 
-import functools
 import math
 
 import torch
@@ -170,7 +169,6 @@ def run(state):
     return {"norm": _norm, "attend": _attend, "embed": _embed}[kind](state)
 
 
-@functools.lru_cache(maxsize=None)
 def _own():
     import sys
     from pathlib import Path
