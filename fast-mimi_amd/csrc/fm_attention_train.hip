@@ -37,7 +37,16 @@ typedef unsigned uintx2_v __attribute__((ext_vector_type(2)));
 typedef unsigned uintx4_v __attribute__((ext_vector_type(4)));
 
 constexpr float LOG2E = 1.44269504088896341f;
-constexpr float SLACK = 8.0f;
+
+// float16 ends at 2^16 and 2^-24, so what is rounded to it carries a power of two.
+// The forward's probabilities, relative to a reference that the maximum may pass by
+// 2^SLACK, stand 2^UP higher, and the gradients' (at most 1, and a rounding) 2^P_UP:
+// a step is 2^-35 of a row's largest probability and 2^-38 of 1 then, where 2^-24
+// would lose what thousands of small ones add up to.
+template <typename T> constexpr bool SCALED = std::is_same<T, _Float16>::value;
+template <typename T> constexpr float SLACK = SCALED<T> ? 4.0f : 8.0f;
+template <typename T> constexpr float UP = SCALED<T> ? 11.0f : 0.0f;
+template <typename T> constexpr float P_UP = SCALED<T> ? 14.0f : 0.0f;
 
 template <typename T> struct Elem;
 template <> struct Elem<float> {
@@ -502,6 +511,38 @@ FM_DEVICE float half_max(float v) {
   return fmaxf(__builtin_bit_cast(float, (unsigned)r[0]), __builtin_bit_cast(float, (unsigned)r[1]));
 }
 
+// The power of two that dS carries as a float16 operand, one for each column of its
+// products (a row of dQ, a key of dK: a lane of either half), and with it the sums
+// over the column, until their end.  At the start a step is 2^-72: times the largest
+// float16 and over 2^21 rows under the smallest.  When a value passes 2^15 the level
+// falls until that one lies between 2^8 and 2^9 (for infinities it stays), so that
+// a step is at most 2^-32 of the column's largest dS.  (2 x 4095 positions, 16/4
+// heads of 128, float16, backward: 683 -> 712 us.)
+struct Level {
+  int up = 48;
+  // Whether any lane's largest magnitude passes 2^15 (called by whole waves).
+  FM_DEVICE bool passed(float most) const { return __any(most > 32768.0f); }
+  // Returns what the sums and the values are to be multiplied by.
+  FM_DEVICE float lower(float most) {
+    const int by = most > 32768.0f ? max(__builtin_amdgcn_frexp_expf(most) - 9, 0) : 0;
+    up -= by;
+    return __builtin_ldexpf(1.0f, -by);
+  }
+};
+FM_DEVICE float column_most(const floatx16& s) {
+  float most = fabsf(s[0]);
+#pragma unroll
+  for (int e = 1; e < 16; ++e) most = fmaxf(most, fabsf(s[e]));
+  return half_max(most);
+}
+template <int ND>
+FM_DEVICE void times(floatx16 (&acc)[ND], float f) {
+#pragma unroll
+  for (int d = 0; d < ND; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[d][e] *= f;
+}
+
 FM_DEVICE void tile_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
@@ -720,7 +761,7 @@ FM_DEVICE bool Forward<T, DT, WQ, WK>::run(const Attn& a, unsigned char* lds) {
       // m is a reference, not the maximum itself: it follows once a score passes it
       // by SLACK, so that the accumulators are rescaled a few times a row and not
       // in most tiles.  Until then exponentials reach 2^SLACK, far from any limit.
-      if (__any(top > m + SLACK)) {
+      if (__any(top > m + SLACK<T>)) {
         const float up = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - (up == -INFINITY ? 0.0f : up));
         m = up;
         l *= f;
@@ -729,7 +770,7 @@ FM_DEVICE bool Forward<T, DT, WQ, WK>::run(const Attn& a, unsigned char* lds) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[d][e] *= f;
       }
-      const float sub = m == -INFINITY ? 0.0f : m;
+      const float sub = m == -INFINITY ? 0.0f : m - UP<T>;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -sub));
@@ -779,7 +820,7 @@ FM_DEVICE bool Forward<T, DT, WQ, WK>::run(const Attn& a, unsigned char* lds) {
   }
   // A row that sees nothing (padding) gives zeros.
   const bool some = w.live && l != 0.0f;
-  if (writes) a.lse[w.row_index] = some ? m + log2f(l) : -INFINITY;
+  if (writes) a.lse[w.row_index] = some ? m + (log2f(l) - UP<T>) : -INFINITY;
   store_row(static_cast<T*>(a.out) + w.row_index * a.D, mine, 1.0f / l, some, wk * MINE, half, a.D);
   return true;
 }
@@ -822,7 +863,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Attn a) {
     }
   }
   const long row = ((long)b * a.T + t) * a.H + kh * a.G + (r - t * a.G);
-  if (lane == 0) a.lse[row] = live && l != 0.0f ? m + log2f(l) : -INFINITY;
+  if (lane == 0) a.lse[row] = live && l != 0.0f ? m + (log2f(l) - UP<T>) : -INFINITY;
   T* out = static_cast<T*>(a.out) + row * a.D;
 #pragma unroll
   for (int u = 0; u < DT / 64; ++u)
@@ -890,9 +931,11 @@ FM_DEVICE bool QueryGradient<T, DT, WQ, WK>::run(const Attn& a, unsigned char* l
   lse = lse == -INFINITY ? INFINITY : lse;
   float rest = 0.0f;  // the sum of dS: what the rounding of O took from delta
 
+  Level level;
+
   // The row's sum over both lane halves and all the waves that share it.
   auto total = [&]() {
-    float sum = half_sum(rest);
+    float sum = half_sum(SCALED<T> ? __builtin_ldexpf(rest, -level.up) : rest);
     if constexpr (WK > 1) {
       float(*rests)[32] = reinterpret_cast<float(*)[32]>(lds + L::LDS) + WK * wq;
       if (half == 0) rests[wk][lane] = sum;
@@ -927,9 +970,10 @@ FM_DEVICE bool QueryGradient<T, DT, WQ, WK>::run(const Attn& a, unsigned char* l
         G::products(at, q, s);
         G::products(at + L::TILE, g, dp);
         const bool edge = k0 + 31 > w.p_lo || k0 <= w.p_hi - a.window || k0 + 31 > w.k_hi;
+        const float sub = SCALED<T> ? lse - (float)level.up : lse;
   #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -lse));
+          const float p = __builtin_amdgcn_exp2f(fmaf(s[e], a.scale2, -sub));
           s[e] = p * (dp[e] - delta);
         }
         if (edge) {
@@ -937,6 +981,16 @@ FM_DEVICE bool QueryGradient<T, DT, WQ, WK>::run(const Attn& a, unsigned char* l
           for (int e = 0; e < 16; ++e) {
             const int key = k0 + 8 * (e >> 2) + 4 * half + (e & 3);
             s[e] = key <= w.p && key > w.p - a.window && key <= w.k_hi && w.live ? s[e] : 0.0f;
+          }
+        }
+        if constexpr (SCALED<T>) {
+          const float top = column_most(s);
+          if (level.passed(top)) {
+            const float f = level.lower(top);
+            rest *= f;
+            times(acc, f);
+  #pragma unroll
+            for (int e = 0; e < 16; ++e) s[e] *= f;
           }
         }
   #pragma unroll
@@ -957,6 +1011,7 @@ FM_DEVICE bool QueryGradient<T, DT, WQ, WK>::run(const Attn& a, unsigned char* l
   if constexpr (SPLITS)
     if (__syncthreads_or(fmaxf(most, fmaxf(q.most, g.most)) >= BIG)) return false;
   rest = total();
+  if constexpr (SCALED<T>) times(acc, __builtin_ldexpf(1.0f, -level.up));
   constexpr int MINE = DT / 2 / WK;
   float mine[MINE];
   if constexpr (WK > 1) {
@@ -967,7 +1022,7 @@ FM_DEVICE bool QueryGradient<T, DT, WQ, WK>::run(const Attn& a, unsigned char* l
   }
   if (w.r >= w.R) return true;
   if (half == 0 && wk == 0) {
-    a.stats[w.row_index] = lse;
+    a.stats[w.row_index] = lse - P_UP<T>;
     a.stats[(long)a.B * a.T * a.H + w.row_index] = sizeof(T) == 2 ? delta + rest : delta;
   }
   store_row(static_cast<T*>(a.out) + w.row_index * a.D, mine, a.scale, w.live, wk * MINE, half, a.D);
@@ -1107,6 +1162,7 @@ FM_DEVICE bool KeyGradients<T, DT, WK, WR>::run(const Attn& a, unsigned char* ld
     G::here(kf), G::here(vf);
   }
   floatx16 ak[ND] = {}, av[ND] = {};
+  Level level;  // of dS; the probabilities' own part of it is P_UP
   for (int i = tiles - 1; i >= 0; --i) {
     tile_barrier();
     if constexpr (SPLITS) {
@@ -1137,6 +1193,7 @@ FM_DEVICE bool KeyGradients<T, DT, WK, WR>::run(const Attn& a, unsigned char* ld
       }
       // Rows past the last are zeros, whose products with infinities are not.
       const bool edge = w0 + 31 > lo || w0 <= hi - a.window || r0 + 31 > r_hi;
+      const float f = SCALED<T> ? __builtin_ldexpf(1.0f, level.up - (int)P_UP<T>) : 1.0f;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const floatx4 lse = *reinterpret_cast<const floatx4*>(&stat[stage][0][row + 8 * g + 4 * half]);
@@ -1145,7 +1202,7 @@ FM_DEVICE bool KeyGradients<T, DT, WK, WR>::run(const Attn& a, unsigned char* ld
         for (int e = 0; e < 4; ++e) {
           const float p = __builtin_amdgcn_exp2f(fmaf(s[4 * g + e], a.scale2, -lse[e]));
           s[4 * g + e] = p;
-          dp[4 * g + e] = p * (dp[4 * g + e] - delta[e]);
+          dp[4 * g + e] = p * (SCALED<T> ? (dp[4 * g + e] - delta[e]) * f : dp[4 * g + e] - delta[e]);
         }
       }
       if (edge) {
@@ -1155,6 +1212,15 @@ FM_DEVICE bool KeyGradients<T, DT, WK, WR>::run(const Attn& a, unsigned char* ld
           const bool ok = key <= p && key > p - a.window && r <= r_hi;
           s[e] = ok ? s[e] : 0.0f;
           dp[e] = ok ? dp[e] : 0.0f;
+        }
+      }
+      if constexpr (SCALED<T>) {
+        const float top = column_most(dp);
+        if (level.passed(top)) {
+          const float by = level.lower(top);
+          times(ak, by);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) dp[e] *= by;
         }
       }
       const unsigned to = R::fresh(R::lds(qt) + row * R::PITCH + col_lane);
@@ -1174,6 +1240,7 @@ FM_DEVICE bool KeyGradients<T, DT, WK, WR>::run(const Attn& a, unsigned char* ld
   }
   if constexpr (SPLITS)
     if (__syncthreads_or(most >= BIG)) return false;
+  if constexpr (SCALED<T>) times(ak, __builtin_ldexpf(1.0f, -level.up));
   constexpr int MINE = DT / 2 / WR;
   const long row_index = ((long)b * a.S + key) * a.KV + kh;
 #pragma unroll
@@ -1188,7 +1255,8 @@ FM_DEVICE bool KeyGradients<T, DT, WK, WR>::run(const Attn& a, unsigned char* ld
       for (int i = 0; i < MINE; ++i) mine[i] = acc[i / 16][i % 16];
     }
     if (key < a.S)  // padding takes no gradient
-      store_row(static_cast<T*>(which ? a.dv : a.dk) + row_index * a.D, mine, which ? 1.0f : a.scale, live, wr * MINE, half, a.D);
+      store_row(static_cast<T*>(which ? a.dv : a.dk) + row_index * a.D, mine, which ? __builtin_exp2f(-P_UP<T>) : a.scale, live, wr * MINE,
+                half, a.D);
   }
   return true;
 }

@@ -318,9 +318,6 @@ def window_attention_forward(q, k, v, window: int | None = None, scale: float | 
 def window_attention_backward(grad, q, k, v, out, lse, window: int | None = None, scale: float | None = None, lengths=None):
     """``(dq, dk, dv)`` for the gradient ``grad`` of the output of
     :func:`window_attention_forward` (``out``, ``lse``: what it returned).
-
-    float16: ``grad . v - grad . out`` of a visible pair is a float16 operand; past
-    65504 the gradients are not finite.
     """
     q, k, v, window, scale, lengths = _attention_input(q, k, v, window, scale, lengths)
     grad, out, lse = _tensor("grad", grad, (q.dtype,)), _tensor("out", out, (q.dtype,)), _tensor("lse", lse, (torch.float32,))

@@ -606,9 +606,7 @@ int fm_attention_forward(const void* q, long q_batch, long q_row, long q_head, c
  * forms the probabilities again.  dout is strided as q; dq, dk and dv are
  * contiguous; stats [2][batch][queries][heads] is scratch (the rows' lse and
  * dout . out).
- * Padding takes no gradient (zeros), and its dout is not used.  float16: the
- * probability times dout . v - dout . out is an operand of that type; past 65504
- * the gradients are not finite.
+ * Padding takes no gradient (zeros), and its dout is not used.
  */
 int fm_attention_backward(const void* dout, long dout_batch, long dout_row, long dout_head,
                           const void* q, long q_batch, long q_row, long q_head, const void* k,
