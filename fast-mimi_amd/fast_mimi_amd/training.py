@@ -4,7 +4,8 @@ What a transformer over codec frames and the codebooks below it need to be
 trained, on the HIP kernels of ``libfast_mimi_amd.so``:
 
 * :func:`layer_norm`, :func:`window_attention` and :func:`code_embedding` are
-  differentiable (``torch.autograd``, first order);
+  differentiable (``torch.autograd``, reverse mode, first order: dual tensors
+  raise ``NotImplementedError``);
 * ``*_forward`` / ``*_backward`` are the same without autograd, for a training
   loop that keeps its own tape, or that records its step in a hipGraph.
 
@@ -25,6 +26,7 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as nat
@@ -47,12 +49,21 @@ _DTYPES = {torch.float32: nat.DTYPE_F32, torch.bfloat16: nat.DTYPE_BF16, torch.f
 
 
 # ------------------------------------------------------------------- checks
+def _reverse_mode(*tensors) -> None:
+    """Refuses tensors with a forward-mode tangent, which would be lost without a word."""
+    if forward_ad._current_level < 0:
+        return
+    if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("the training operators have no forward-mode derivative: an input has a tangent")
+
+
 def _tensor(name: str, t, dtypes=tuple(_DTYPES)) -> torch.Tensor:
     """``t`` as the kernels read it (no graph, no lazy negation), or TypeError."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}, got {t.dtype}")
+    _reverse_mode(t)
     if t.requires_grad:
         t = t.detach()
     return t.resolve_neg() if t.is_neg() else t
@@ -125,6 +136,7 @@ def _apply(function, inputs, *args):
     """``function.apply(*args)``, refused under stream capture for a leaf of
     ``inputs`` that an eager graph of these functions still holds (see the
     module's text)."""
+    _reverse_mode(*inputs)  # a Function's forward does not see tangents
     capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
     if capturing and any(_EAGER in node.metadata for node in _accumulators(inputs)):
         raise RuntimeError("a captured graph cannot use a leaf of an eager autograd graph that is still alive: drop the "
