@@ -286,14 +286,14 @@ def _heads(t: torch.Tensor, group: int = 1) -> tuple[torch.Tensor, int, int, int
     unit = 16 // size
     b, n, h, d = t.shape
     sb, sn, sh, sd = t.stride()
-    # The stride of a single item does not matter, whatever it says.
+    # The stride of a single item does not matter, whatever it says (also of a copy).
     sb, sn, sh = sb if b > 1 else 0, sn if n > 1 else 0, sh if h > 1 else 0
     reach = 0x7fffffff // size
     if (sd != 1 and d > 1) or (sb | sn | sh) % unit or t.data_ptr() % 16 or sn > reach // 256 or sh > reach // 2 // group:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
-        sb, sn, sh, _ = t.stride()
+        sb, sn, sh = n * h * d if b > 1 else 0, h * d if n > 1 else 0, d if h > 1 else 0
     return t, sb, sn, sh
 
 
