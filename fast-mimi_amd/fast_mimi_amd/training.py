@@ -15,10 +15,12 @@ Outputs and scratch memory are allocated by the call, on the current stream;
 nothing synchronises.  Inputs must be on a ROCm GPU: there is no other backend.
 
 In a hipGraph: torch gives a leaf's gradient on the stream on which the leaf
-was first used, so a backward pass that is captured while an eager graph of the
-same leaves is alive ends the process.  The differentiable functions raise
-``RuntimeError`` for leaves that went through them eagerly and still do; capture
-the ``*_backward`` functions, or drop the eager graph first.
+was first used, for as long as an autograd graph of it (or whoever else holds its
+gradient accumulator) lives.  Where that is the default stream, which cannot be
+captured, a captured backward pass of the same leaf ends the process: the
+differentiable functions raise ``RuntimeError`` for a leaf that went through them
+there first.  Warm up on a side stream, as ``torch.cuda.make_graphed_callables``
+does, drop the eager graph, or capture the ``*_backward`` functions.
 """
 
 from __future__ import annotations
@@ -44,7 +46,7 @@ __all__ = [
     "window_attention_forward",
 ]
 
-_EAGER = "fast_mimi_amd.eager"
+_DEFAULT_STREAM = "fast_mimi_amd.default_stream"
 _DTYPES = {torch.float32: nat.DTYPE_F32, torch.bfloat16: nat.DTYPE_BF16, torch.float16: nat.DTYPE_F16}
 
 
@@ -134,17 +136,18 @@ def _accumulators(inputs):
 
 def _apply(function, inputs, *args):
     """``function.apply(*args)``, refused under stream capture for a leaf of
-    ``inputs`` that an eager graph of these functions still holds (see the
-    module's text)."""
+    ``inputs`` whose gradient would come on the default stream (see the module's
+    text).  An accumulator keeps its stream, so the first use decides."""
     _reverse_mode(*inputs)  # a Function's forward does not see tangents
     capturing = torch.cuda.is_available() and torch.cuda.is_current_stream_capturing()
-    if capturing and any(_EAGER in node.metadata for node in _accumulators(inputs)):
-        raise RuntimeError("a captured graph cannot use a leaf of an eager autograd graph that is still alive: drop the "
-                           "eager graph, or capture the *_forward and *_backward functions")
+    if capturing and any(node.metadata.get(_DEFAULT_STREAM) for node in _accumulators(inputs)):
+        raise RuntimeError("a captured graph cannot use a leaf of an eager autograd graph that was made on the default stream "
+                           "and is still alive: drop the eager graph (and what else holds the leaf's gradient accumulator), "
+                           "make it on another stream, or capture the *_forward and *_backward functions")
     out = function.apply(*args)
-    if not capturing:
-        for node in _accumulators(inputs):
-            node.metadata[_EAGER] = True
+    default = torch._C._cuda_getCurrentRawStream(out.device.index) == 0
+    for node in _accumulators(inputs):
+        node.metadata.setdefault(_DEFAULT_STREAM, default)
     return out
 
 
