@@ -385,6 +385,7 @@ void launch(const Norm& a, bool back, hipStream_t stream) {
                        a);
 }
 
+// False where the plan has no kernel (none of plan()'s).
 template <typename T, typename W, int E>
 bool launch_width(const Norm& a, const Plan& p, bool back, hipStream_t stream) {
   if (p.lpr == 16) return launch<T, W, E, 1, 16>(a, back, stream), true;
@@ -432,9 +433,9 @@ int run(Norm a, bool back, hipStream_t stream) {
     else
       hipLaunchKernelGGL((norm_forward_any_kernel<T, W>), dim3((unsigned)a.rows), dim3(256), 0, stream, a);
   } else if (p.e == 1) {
-    launch_width<T, W, 1>(a, p, back, stream);
+    if (!launch_width<T, W, 1>(a, p, back, stream)) return FM_UNSUPPORTED;
   } else {
-    launch_width<T, W, 16 / sizeof(T)>(a, p, back, stream);
+    if (!launch_width<T, W, 16 / sizeof(T)>(a, p, back, stream)) return FM_UNSUPPORTED;
   }
   if (back && (a.dw || a.db) && (a.blocks > 1 || p.nv == 0))
     hipLaunchKernelGGL((norm_join_kernel<W>), dim3(fm_ceil_div(2l * a.C, 32)), dim3(1024), 0, stream, a);
