@@ -331,8 +331,10 @@ struct Engine {
 // split it into three planes in LDS once all waves are done with the last one.
 // An infinity has no such pieces, and where a product overflows, so may those of
 // its factors' remainders, with either sign.  A block that meets a value of 2^36
-// or more starts again on FP32 MFMAs: below, scores stay under 2^78, dS under 2^81
-// and no product or sum of them comes near the largest value.  (At the other end
+// or more starts again on FP32 MFMAs: below, scores stay under 2^78 and dS under
+// 2^81, so that no value that is split and no single product (2^117) comes near the
+// largest one.  (dK sums such products over its rows and overflows where 2^11 of the
+// largest meet, as an FP32 sum does: to infinity, as its terms are finite.  At the other end
 // a piece may be lost below 2^-126: of values under 2^-102 more than an FP32
 // rounding, and never more than 2^-126 of any.)
 // 16 x 2500 frames, 8 heads, window 250: forward 250 -> 170 us, dQ 355 -> 270,
