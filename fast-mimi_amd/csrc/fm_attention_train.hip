@@ -1157,7 +1157,9 @@ FM_DEVICE bool KeyGradients<T, DT, WK, WR>::run(const Attn& a, unsigned char* ld
     V::bring(vp + k0 * a.v.row, a.D, values, [&](int r) { return r <= n ? r * vs : -1; });
     most = V::publish(values, lds, kf.most);
   } else if constexpr (KEEP > 0) {
-    load_keys<T, DT, 32 * WK, WAVES>(a, kp, vp, k0, min(len, k0 + 32 * WK) - 1, lds, wave, lane);
+    // The first tile's barrier waits for these copies; where there is none they would
+    // still be on their way when the results take their place.
+    if (tiles) load_keys<T, DT, 32 * WK, WAVES>(a, kp, vp, k0, min(len, k0 + 32 * WK) - 1, lds, wave, lane);
   } else {
     G::load(kp + at_key * a.k.row, live, a.D, lane, kf);
     G::load(vp + at_key * a.v.row, live, a.D, lane, vf);
