@@ -23,7 +23,7 @@
 //
 // Long calls are bound by the matrix cores and the exponentials and conversions
 // beside them, which add on this part: 2 x 4095 positions, 16/4 heads of 128,
-// bfloat16, no window: forward 190 us (720 TFLOP/s), dQ 294, dK / dV 420.  Short
+// bfloat16, no window: forward 180 us (760 TFLOP/s), dQ 285, dK / dV 410.  Short
 // ones by latency: 2500 positions, 8 heads of 64, window 250: 11.5, 15.5, 15.5 us.
 
 #include "fm_common.h"
@@ -878,9 +878,12 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Attn a) {
 // rounding would put dQ at 1.5 times the error that rounding its result has.  And
 // rowsum(dO O) from the rounded O is only nearly the sum over P dP; the sum of dS,
 // zero but for that, puts it right for the dK / dV kernel.  Where a row sees few
-// keys it would also be most of dQ's error (1.5 times the rounding's with 4 keys,
-// less than 1.1 from 32 on): blocks with such rows go over their keys twice (16 x
-// 2500 frames, all of them under a window of 31: backward 155 -> 169 us).
+// keys it would also be most of dQ's error (1.5 times the rounding's with 4 keys of
+// ordinary scores, less than 1.1 from 32 on): blocks with such rows go over their
+// keys twice (16 x 2500 frames, all of them under a window of 31: backward 155 -> 169
+// us).  Rows of more keys with one large probability keep it (1.4 times at 0.3, 2.2
+// at 0.65): which they are is known after the pass only, and a second one for all
+// would be 12-24% of the backward (16 x 2500, window 250: 201 -> 230 us).
 template <typename T, int DT, int WQ, int WK>
 struct QueryGradient {
   template <bool SPLITS>
@@ -1050,7 +1053,11 @@ struct RowTiles<T, DT, ROWS, true> {
 // blocks to a CU, or eight waves where that many blocks would all run at once and
 // the longest (the first keys of a sequence without a window) set the time.  2 x
 // 4095 positions, 16/4 heads: 740 us from registers, 540 / 404 from LDS with four
-// / eight waves; 16 heads x 2 x 2048: 190, 102 / 126.
+// / eight waves; 16 heads x 2 x 2048: 190, 102 / 126.  Backward with four / eight
+// waves (the rule takes eight up to 512 blocks): 8 heads x 2048 (256 blocks) 121 / 99
+// us, 16 x 2048 (512) 129 / 116, 32 x 2048 (1024) 195 / 211, 64 x 2048 363 / 396; with a
+// window of 250, where blocks are alike, 8 x 2500 (320) 44 / 52, 32 x 250 (128) 26 / 24,
+// 128 x 250 (512) 39 / 44, 32 x 2500 (1280) 114 / 133.
 template <typename T, int DT>
 constexpr bool HELD = sizeof(T) == 2 && DT == 128;
 //
@@ -1297,7 +1304,11 @@ int forward_splits(const Attn& a) {
 
 // How many of a block's four waves take rows (or keys) of their own, the rest
 // sharing them: four where that leaves about three blocks a CU, two where one
-// is left for each, else one.
+// is left for each, else one.  Backward with one / two / four, 64 channels, window
+// 250, bfloat16: 8 heads x 1000 (125 blocks of 64 rows) 20 / 23 / 35 us, 8 x 2500 (320) 39
+// / 30 / 36, 8 x 10000 (1264; 632 of 128) 100 / 68 / 71, 128 x 1000 (1024 of 128) 146 / 94 /
+// 81; FP32 the same order.  (128 heads of 128 channels x 500, 512 of 128: forward two
+// / four 26 / 22, the largest loss seen.)
 int own_waves(const Attn& a, long rows) {
   const long seqs = (long)a.B * a.KV;
   return seqs * fm_ceil_div(rows, 128) >= 768 ? 4 : seqs * fm_ceil_div(rows, 64) >= 256 ? 2 : 1;
