@@ -880,8 +880,9 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Attn a) {
 // zero but for that, puts it right for the dK / dV kernel.  Where a row sees few
 // keys it would also be most of dQ's error (1.5 times the rounding's with 4 keys of
 // ordinary scores, less than 1.1 from 32 on): blocks with such rows go over their
-// keys twice (16 x 2500 frames, all of them under a window of 31: backward 155 -> 169
-// us).  Rows of more keys with one large probability keep it (1.4 times at 0.3, 2.2
+// keys twice (backward of 16 x 2500 frames without it / up to 31 keys / up to 63, under
+// windows of 31, 48 and 63: 151 / 162 / 162, 158 / 161 / 172, 159 / 163 / 175 us; of 13
+// frames 12 / 13 / 13).  Rows of more keys with one large probability keep it (1.4 times at 0.3, 2.2
 // at 0.65): which they are is known after the pass only, and a second one for all
 // would be 12-24% of the backward (16 x 2500, window 250: 201 -> 230 us).
 template <typename T, int DT, int WQ, int WK>
@@ -1063,7 +1064,9 @@ constexpr bool HELD = sizeof(T) == 2 && DT == 128;
 //
 // The rounding of P and dS to 16 bits puts dV and dK at 1.4 times the error of
 // rounding the results.  Sums over few rows, where chance adds to that, have them
-// in two pieces; a block of that many rows is one or two tiles long.
+// in two pieces; a block of that many rows is one or two tiles long (backward of 16 x
+// 13, 100 and 250 positions, never / up to 128 rows / up to 512: 13.0 / 13.4 / 13.4, 16.9 /
+// 17.7 / 17.8, 25.2 / 25.6 / 26.8 us; 16 x 2500 under a window of 100: 172 / 170 / 184).
 constexpr int FEW_ROWS = 128;
 template <typename T, int DT, int WK, int WR>
 struct KeyGradients {

@@ -423,7 +423,11 @@ int embed_backward(const Embed& a, hipStream_t stream) {
   const unsigned slices = fm_ceil_div(a.D / E, SLICE), per = 256 / SLICE;
   if (a.runs)
     hipLaunchKernelGGL((embed_run_kernel<T, E>), dim3(slices, fm_ceil_div(a.runs, per), a.books), dim3(256), 0, stream, a);
-  // One entry at a time where that alone does not fill the chip.
+  // One entry at a time where that alone does not fill the chip.  Gradients with one /
+  // four, codes even and a third of them one, in us: 16384 units (4 x 512 entries of 256)
+  // 20 / 33 and 33 / 40; 65536 (4 x 1024 of 512, 24000 rows) 45 / 49 and 58 / 69; 131072 (8
+  // x 2048 of 256, 2000 rows) 23 / 22 and 33 / 33, 125 rows 18 / 16 and 21 / 22; 524288 (32
+  // x 2048 of 256, 8000 rows) 59 / 53 and 81 / 78.
   if ((long)a.books * a.entries * slices >= 32768)
     hipLaunchKernelGGL((embed_entry_kernel<T, E, 4>), dim3(slices, fm_ceil_div(a.entries, 4 * per), a.books), dim3(256), 0,
                        stream, a);
