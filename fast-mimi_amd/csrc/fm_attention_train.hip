@@ -1275,8 +1275,6 @@ FM_DEVICE bool KeyGradients<T, DT, WK, WR>::run(const Attn& a, unsigned char* ld
   return true;
 }
 
-enum { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };
-
 int check(const Attn& a, int dtype) {
   if (a.B < 0 || a.T < 0 || a.S < 0 || a.H <= 0 || a.KV <= 0 || a.D <= 0 || a.window <= 0 || !(a.scale > 0.0f) ||
       a.scale2 == INFINITY || a.H % a.KV || a.T > a.S || dtype < DT_F32 || dtype > DT_F16)

@@ -294,3 +294,20 @@ FM_DEVICE bool fm_arrive_and_wait(unsigned* counter, unsigned target, long spin)
     if (__hip_atomic_load(counter, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) >= target) return true;
   return false;
 }
+
+// ---------------------------------------------------------------------------
+// The training kernels' element types (FM_DTYPE_*), and E consecutive elements
+// of one, loaded and stored as one access.
+enum { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };
+template <typename T, int E>
+struct Vec {
+  typedef T type __attribute__((ext_vector_type(E)));
+};
+template <typename T>
+struct Vec<T, 1> {
+  struct type {
+    T v;
+    FM_DEVICE T& operator[](int) { return v; }
+    FM_DEVICE const T& operator[](int) const { return v; }
+  };
+};

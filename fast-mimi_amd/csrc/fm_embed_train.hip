@@ -13,8 +13,6 @@
 
 namespace {
 
-enum { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };
-
 constexpr int HISTOGRAMS = 32768;  // of LDS, in counters: waves x entries at most
 
 struct Embed {
@@ -30,19 +28,6 @@ struct Embed {
   int frames, books, entries, D, run_rows, runs, chunk_rows, chunks;
   FmDivisor by_frames;
   float scale;
-};
-
-template <typename T, int E>
-struct Vec {
-  typedef T type __attribute__((ext_vector_type(E)));
-};
-template <typename T>
-struct Vec<T, 1> {
-  struct type {
-    T v;
-    FM_DEVICE T& operator[](int) { return v; }
-    FM_DEVICE const T& operator[](int) const { return v; }
-  };
 };
 
 // Work is cut into slices of 128 bytes of columns (8 lanes of 16 bytes), the

@@ -13,23 +13,7 @@
 
 namespace {
 
-enum { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };
-
 template <typename T> FM_DEVICE float widen(T v) { return (float)v; }
-
-// E consecutive elements of T, loaded and stored as one access.
-template <typename T, int E>
-struct Vec {
-  typedef T type __attribute__((ext_vector_type(E)));
-};
-template <typename T>
-struct Vec<T, 1> {
-  struct type {
-    T v;
-    FM_DEVICE T& operator[](int) { return v; }
-    FM_DEVICE const T& operator[](int) const { return v; }
-  };
-};
 
 // Sums over the LPR lanes of a row; with 256, a block's waves, through `waves`
 // (of its own for each sum between two barriers).
