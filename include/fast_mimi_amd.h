@@ -580,7 +580,8 @@ int fm_layer_norm_backward(const void* dy, long ld_dy, const void* x, long ld_x,
  * zeros.  heads is a multiple of kv_heads; query head h reads key head
  * h / (heads / kv_heads).  q / k / v are strided (strides in elements of the
  * batch, position and head dimensions; a packed projection is such a view);
- * rows must be 16-byte aligned, head_dim <= 128 a multiple of 8 (FP32: 4),
+ * rows must be 16-byte aligned, at most 2^23 - 1 bytes from one position to the
+ * next and 2^30 - 1 over a key head's query heads, head_dim <= 128 a multiple of 8 (FP32: 4),
  * scale positive; at most 2097120 keys, and rows per key head (queries x heads /
  * kv_heads), 2^23 sequences x key heads, 2^20 heads.  out [batch][queries][heads][head_dim] and lse
  * [batch][queries][heads] (log2 of the row's sum of exponentials, -inf for a

@@ -52,3 +52,24 @@ def test_attention_of_odd_views(i, dtype):
     got = tr.window_attention_backward(x, x, x, x, out, lse, 20)
     for a, b in zip(got, tr.window_attention_backward(plain, plain, plain, plain, want, lse, 20)):
         assert torch.equal(a, b)
+
+
+def test_pitches_at_the_abi():
+    """A row or head pitch beyond what a tile's 32-bit offsets reach is refused; the
+    largest ones are not (an empty batch, so that nothing runs)."""
+    from fast_mimi_amd import _native as nat
+
+    if not nat.LIBRARY_PATH.is_file():
+        pytest.skip("library not built")
+    p = 0x10000  # never dereferenced
+
+    def status(row, head, heads=4, dtype=1):
+        view, keys = (p, 0, row, head), (p, 0, 64, 64)
+        return nat.library().fm_attention_forward(*view, *keys, *keys, None, 0, 4, 4, heads, 1, 64, 4, 0.125, dtype, p, p, None, 0,
+                                                  None)
+
+    row, head = (2 ** 31 - 1) // 2 // 256, (2 ** 31 - 1) // 2 // 2 // 4
+    assert status(row // 8 * 8, head // 8 * 8) == 0
+    assert status(row // 8 * 8 + 8, 64) == 1002 and status(64, head // 8 * 8 + 8) == 1002
+    assert status(row // 2 // 4 * 4, head // 2 // 4 * 4, dtype=0) == 0
+    assert status(row // 2 // 4 * 4 + 4, 64, dtype=0) == 1002
