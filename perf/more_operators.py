@@ -227,7 +227,9 @@ def _own(name):
 def _own_norm(state):
     f = _own("training")
     y, h, rstd = f.rms_norm_forward(state["x"], state["weight"], state["residual"], EPS)
-    dx, dh, dw = f.rms_norm_backward(state["grad"], h, rstd, state["weight"], state["grad_h"])
+    # What a program keeps for the backward pass: an FP32 stream's sum, or the two 16-bit parts of it.
+    x, residual = (h, None) if h.dtype == torch.float32 else (state["x"], state["residual"])
+    dx, dh, dw = f.rms_norm_backward(state["grad"], x, rstd, state["weight"], residual, state["grad_h"])
     return {"y": y, "h": h, "dx": dx, "dresidual": dh, "dw": dw}
 
 
