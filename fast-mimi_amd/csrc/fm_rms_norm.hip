@@ -1,0 +1,586 @@
+// RMS norm of a branch added to its residual stream: forward, backward, and the
+// forward with its output in 8 bits.  Branch FP32, bfloat16 or float16; stream and
+// weight of that type or FP32; every sum in FP32.
+//
+//   forward   h = x + res, r = 1 / sqrt(mean h^2 + eps), y = h r w
+//   backward  hh = (x + res) r, g = dy w, dh = dstream + r (g - hh mean(g hh)),
+//             dw = sum over rows of dy hh
+//   8 bits    of each 128 channels of y: e the least with max |y| <= 448 2^e,
+//             y 2^-e rounded to e4m3, e + 127 kept in a byte (e8m0)
+//
+// y comes from the sum before it is rounded to the stream's type.  All are bound by
+// memory: a row is read once, held in registers, and reduced by the lanes that hold
+// it.  Rows start anywhere: 16-byte accesses need no alignment on this part, so
+// channels that are not whole vectors cost their last vector only.
+
+#include "fm_rows.h"
+
+namespace {
+
+// E consecutive elements at any address.
+template <typename T, int E>
+using AnyVec = typename Vec<T, E>::type __attribute__((aligned(sizeof(T))));
+
+struct Rms {
+  const void *x, *res, *w, *dy, *dh;  // x, res: backward, either may be NULL; dh: the stream's gradient, or NULL
+  void *y, *sum, *scales, *dx, *dres, *dw;
+  float *rstd, *part;  // part: [blocks][C]
+  long rows, ld_x, ld_res, ld_dy, ld_dh;
+  int C, blocks;
+  float eps;
+};
+
+// Vector i of a row of C elements, zeros past its end.
+template <typename T, int E>
+FM_DEVICE typename Vec<T, E>::type row_load(const T* row, int i, int C) {
+  typename Vec<T, E>::type t{};
+  const T* at = row + i * E;
+  if ((i + 1) * E <= C) {
+    t = *reinterpret_cast<const AnyVec<T, E>*>(at);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E - 1; ++e)
+      if (i * E + e < C) t[e] = at[e];
+  }
+  return t;
+}
+template <typename T, int E>
+FM_DEVICE void row_store(T* row, int i, int C, typename Vec<T, E>::type t) {
+  T* at = row + i * E;
+  if ((i + 1) * E <= C) {
+    *reinterpret_cast<AnyVec<T, E>*>(at) = t;
+  } else {
+#pragma unroll
+    for (int e = 0; e < E - 1; ++e)
+      if (i * E + e < C) at[e] = t[e];
+  }
+}
+
+// The scale byte of 128 values whose largest magnitude is `most`: 255 (NaN) for an
+// infinity or NaN among them.
+FM_DEVICE int scale_byte(float most) {
+  const unsigned u = __builtin_bit_cast(unsigned, most);
+  return u >= 0x7f800000u ? 255 : max((int)(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u), 0);
+}
+// Four values times 2^-(byte - 127), to e4m3.
+FM_DEVICE unsigned four_in_8_bits(float a, float b, float c, float d, int byte) {
+  const int by = 127 - byte;
+  int u = __builtin_amdgcn_cvt_pk_fp8_f32(__builtin_ldexpf(a, by), __builtin_ldexpf(b, by), 0, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(__builtin_ldexpf(c, by), __builtin_ldexpf(d, by), u, true);
+}
+
+// Writes vector i of a row in 8 bits.  The lanes of a block's 128 channels call it
+// together; GROUP of them (neighbours) hold one.
+template <int E, int GROUP>
+FM_DEVICE void store_8_bits(const float (&v)[E], unsigned char* row, unsigned char* scales, int i, int C) {
+  float most = 0.0f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float m = fabsf(v[e]);
+    // As integers: a NaN is above every other magnitude.
+    most = __builtin_bit_cast(float, max(__builtin_bit_cast(int, most), __builtin_bit_cast(int, m)));
+  }
+  const int byte = scale_byte(lanes_max<GROUP>(most));
+  if (i * E >= C) return;
+  if (i * E % 128 == 0) scales[i * E / 128] = (unsigned char)byte;
+  typename Vec<unsigned char, E>::type t;
+#pragma unroll
+  for (int e = 0; e < E; e += 4) {
+    const unsigned u = four_in_8_bits(v[e], v[e + 1], v[e + 2], v[e + 3], byte);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) t[e + k] = (unsigned char)(u >> (8 * k));
+  }
+  row_store<unsigned char, E>(row, i, C, t);
+}
+
+// Lane p of a row holds vectors p, p + LPR, ... (NV of them, E elements each).
+template <typename T, typename S, typename W, int NV, int LPR, bool BITS8>
+__global__ __launch_bounds__(256) void rms_forward_kernel(Rms a) {
+  constexpr int E = 16 / (int)sizeof(T);
+  __shared__ float waves[4];
+  const int p = threadIdx.x % LPR;
+  const long row = (long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  if (row >= a.rows) return;
+  const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
+  const S* res = a.res ? static_cast<const S*>(a.res) + row * a.ld_res : nullptr;
+  float v[NV][E];
+  typename Vec<W, E>::type wv[NV];
+  float s = 0.0f;
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    const int i = p + u * LPR;
+    const typename Vec<T, E>::type t = row_load<T, E>(x, i, a.C);
+    typename Vec<S, E>::type r{};
+    if (res) r = row_load<S, E>(res, i, a.C);
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[u][e] = widen(t[e]) + widen(r[e]);
+  }
+  // The weights are on their way during the sum.
+  const W* w = static_cast<const W*>(a.w);
+#pragma unroll
+  for (int u = 0; u < NV; ++u) wv[u] = w ? row_load<W, E>(w, p + u * LPR, a.C) : typename Vec<W, E>::type{};
+#pragma unroll
+  for (int u = 0; u < NV; ++u)
+#pragma unroll
+    for (int e = 0; e < E; ++e) s = fmaf(v[u][e], v[u][e], s);
+  if (a.sum) {
+    S* h = static_cast<S*>(a.sum) + row * a.C;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      typename Vec<S, E>::type t;
+#pragma unroll
+      for (int e = 0; e < E; ++e) t[e] = (S)v[u][e];
+      row_store<S, E>(h, p + u * LPR, a.C, t);
+    }
+  }
+  const float rstd = 1.0f / sqrtf(row_sum<LPR>(s, waves) / (float)a.C + a.eps);
+  if (p == 0 && a.rstd) a.rstd[row] = rstd;
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    const int i = p + u * LPR;
+    float y[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] = v[u][e] * rstd * (w ? widen(wv[u][e]) : 1.0f);
+    if constexpr (BITS8) {
+      const int blocks = (a.C + 127) / 128;
+      store_8_bits<E, (128 / E < LPR ? 128 / E : LPR)>(y, static_cast<unsigned char*>(a.y) + row * a.C,
+                                                       static_cast<unsigned char*>(a.scales) + row * blocks, i, a.C);
+    } else {
+      typename Vec<T, E>::type t;
+#pragma unroll
+      for (int e = 0; e < E; ++e) t[e] = (T)y[e];
+      row_store<T, E>(static_cast<T*>(a.y) + row * a.C, i, a.C, t);
+    }
+  }
+}
+
+// dh, and this block's share of dw: a row group walks rows blockIdx * groups + g,
+// + gridDim * groups, ... with the columns' sums in registers; the block joins its
+// groups through LDS in order and writes one partial row (or, when it is the only
+// block, the gradient itself).
+template <typename T, typename S, typename W, int NV, int LPR>
+__global__ __launch_bounds__(256) void rms_backward_kernel(Rms a) {
+  constexpr int E = 16 / (int)sizeof(T), GROUPS = 256 / LPR;
+  typedef typename Vec<T, E>::type VT;
+  typedef typename Vec<S, E>::type VS;
+  __shared__ float joined[256 * E], waves[2][4];
+  const int p = threadIdx.x % LPR, g = threadIdx.x / LPR;
+  float wv[NV][E], dw[NV][E];
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    typename Vec<W, E>::type t{};
+    if (a.w) t = row_load<W, E>(static_cast<const W*>(a.w), p + u * LPR, a.C);
+#pragma unroll
+    for (int e = 0; e < E; ++e) wv[u][e] = a.w ? widen(t[e]) : 1.0f, dw[u][e] = 0.0f;
+  }
+  const float inv = 1.0f / (float)a.C;
+  VT xv[NV], xn[NV], gv[NV], gn[NV];
+  VS rv[NV], rn[NV], sv[NV], sn[NV];
+  float rstd, rstd_n = 0.0f;
+  const long step = (long)gridDim.x * GROUPS;
+  // The next row is on its way while this one is worked on.
+  auto load = [&](long row) {
+    const T* dy = static_cast<const T*>(a.dy) + row * a.ld_dy;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      const int i = p + u * LPR;
+      xn[u] = VT{}, rn[u] = VS{}, sn[u] = VS{};
+      if (a.x) xn[u] = row_load<T, E>(static_cast<const T*>(a.x) + row * a.ld_x, i, a.C);
+      if (a.res) rn[u] = row_load<S, E>(static_cast<const S*>(a.res) + row * a.ld_res, i, a.C);
+      if (a.dh) sn[u] = row_load<S, E>(static_cast<const S*>(a.dh) + row * a.ld_dh, i, a.C);
+      gn[u] = row_load<T, E>(dy, i, a.C);
+    }
+    rstd_n = a.rstd[row];
+  };
+  int turn = 0;
+  long row = (long)blockIdx.x * GROUPS + g;
+  if (row < a.rows) load(row);
+  for (; row < a.rows; row += step) {
+#pragma unroll
+    for (int u = 0; u < NV; ++u) xv[u] = xn[u], rv[u] = rn[u], gv[u] = gn[u], sv[u] = sn[u];
+    rstd = rstd_n;
+    if (row + step < a.rows) load(row + step);
+    float s = 0.0f;
+#pragma unroll
+    for (int u = 0; u < NV; ++u)
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float hh = (widen(xv[u][e]) + widen(rv[u][e])) * rstd, d = widen(gv[u][e]);
+        s = fmaf(d * wv[u][e], hh, s);
+        dw[u][e] = fmaf(d, hh, dw[u][e]);
+      }
+    s = row_sum<LPR>(s, waves[turn]) * inv, turn ^= 1;
+#pragma unroll
+    for (int u = 0; u < NV; ++u) {
+      VS t;
+      VT b;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float hh = (widen(xv[u][e]) + widen(rv[u][e])) * rstd;
+        const float dh = fmaf(rstd, fmaf(widen(gv[u][e]), wv[u][e], -hh * s), widen(sv[u][e]));
+        t[e] = (S)dh, b[e] = (T)dh;
+      }
+      row_store<S, E>(static_cast<S*>(a.dres) + row * a.C, p + u * LPR, a.C, t);
+      if constexpr (!std::is_same<T, S>::value)
+        if (a.dx) row_store<T, E>(static_cast<T*>(a.dx) + row * a.C, p + u * LPR, a.C, b);
+    }
+  }
+  if (!a.dw) return;
+#pragma unroll
+  for (int u = 0; u < NV; ++u) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < E; ++e) joined[e * 256 + threadIdx.x] = dw[u][e];
+    __syncthreads();
+    if (g != 0) continue;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int c = (p + u * LPR) * E + e;
+      if (c >= a.C) continue;
+      float s = 0.0f;
+      for (int j = 0; j < GROUPS; ++j) s += joined[e * 256 + j * LPR + p];
+      if (a.blocks > 1) a.part[(long)blockIdx.x * a.C + c] = s;
+      else static_cast<W*>(a.dw)[c] = (W)s;
+    }
+  }
+}
+
+// Any number of channels: one block per row (forward) or per run of rows
+// (backward), the row read again for each step.
+template <typename T, typename S, typename W, bool BITS8>
+__global__ __launch_bounds__(256) void rms_forward_any_kernel(Rms a) {
+  __shared__ float waves[4];
+  const long row = blockIdx.x;
+  const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
+  const S* res = a.res ? static_cast<const S*>(a.res) + row * a.ld_res : nullptr;
+  const W* w = static_cast<const W*>(a.w);
+  auto h = [&](int c) { return widen(x[c]) + (res ? widen(res[c]) : 0.0f); };
+  float s = 0.0f;
+  for (int c = threadIdx.x; c < a.C; c += 256) {
+    const float v = h(c);
+    s = fmaf(v, v, s);
+    if (a.sum) static_cast<S*>(a.sum)[row * a.C + c] = (S)v;
+  }
+  const float rstd = 1.0f / sqrtf(row_sum<256>(s, waves) / (float)a.C + a.eps);
+  if (threadIdx.x == 0 && a.rstd) a.rstd[row] = rstd;
+  if constexpr (BITS8) {
+    const int blocks = (a.C + 127) / 128;
+    // Vectors of four channels, 32 lanes to a block; whole waves go round together.
+    for (int c0 = 0; c0 < a.C; c0 += 1024) {
+      const int i = c0 / 4 + threadIdx.x;
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int c = 4 * i + e;
+        y[e] = c < a.C ? h(c) * rstd * (w ? widen(w[c]) : 1.0f) : 0.0f;
+      }
+      store_8_bits<4, 32>(y, static_cast<unsigned char*>(a.y) + row * a.C, static_cast<unsigned char*>(a.scales) + row * blocks,
+                          i, a.C);
+    }
+  } else {
+    for (int c = threadIdx.x; c < a.C; c += 256)
+      static_cast<T*>(a.y)[row * a.C + c] = (T)(h(c) * rstd * (w ? widen(w[c]) : 1.0f));
+  }
+}
+
+template <typename T, typename S, typename W>
+__global__ __launch_bounds__(256) void rms_backward_any_kernel(Rms a) {
+  __shared__ float waves[2][4];
+  const W* w = static_cast<const W*>(a.w);
+  float* part = a.part + (long)blockIdx.x * a.C;
+  bool first = true;
+  int turn = 0;
+  for (long row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1, first = false) {
+    const T* x = a.x ? static_cast<const T*>(a.x) + row * a.ld_x : nullptr;
+    const S* res = a.res ? static_cast<const S*>(a.res) + row * a.ld_res : nullptr;
+    auto h = [&](int c) { return (x ? widen(x[c]) : 0.0f) + (res ? widen(res[c]) : 0.0f); };
+    const T* dy = static_cast<const T*>(a.dy) + row * a.ld_dy;
+    const S* dh = a.dh ? static_cast<const S*>(a.dh) + row * a.ld_dh : nullptr;
+    const float rstd = a.rstd[row];
+    float s = 0.0f;
+    for (int c = threadIdx.x; c < a.C; c += 256) {
+      const float hh = h(c) * rstd, d = widen(dy[c]);
+      s = fmaf(d * (w ? widen(w[c]) : 1.0f), hh, s);
+      if (a.dw) part[c] = first ? d * hh : fmaf(d, hh, part[c]);
+    }
+    s = row_sum<256>(s, waves[turn]) / (float)a.C;
+    for (int c = threadIdx.x; c < a.C; c += 256) {
+      const float hh = h(c) * rstd;
+      const float v = fmaf(rstd, fmaf(widen(dy[c]), w ? widen(w[c]) : 1.0f, -hh * s), dh ? widen(dh[c]) : 0.0f);
+      static_cast<S*>(a.dres)[row * a.C + c] = (S)v;
+      if constexpr (!std::is_same<T, S>::value)
+        if (a.dx) static_cast<T*>(a.dx)[row * a.C + c] = (T)v;
+    }
+  }
+}
+
+// dw from the blocks' partial rows: 32 columns a block, 32 threads to a column, each
+// summing every 32nd row in order, then joined in order.
+template <typename W>
+__global__ __launch_bounds__(1024) void rms_join_kernel(Rms a) {
+  __shared__ float sums[32][33];
+  const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
+  const long col = (long)blockIdx.x * 32 + c;
+  float s = 0.0f;
+  if (col < a.C) {
+    const float* from = a.part + col;
+#pragma unroll 4
+    for (int r = g; r < a.blocks; r += 32) s += from[(long)r * a.C];
+  }
+  sums[g][c] = s;
+  __syncthreads();
+  if (g != 0 || col >= a.C) return;
+  float total = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) total += sums[j][c];
+  static_cast<W*>(a.dw)[col] = (W)total;
+}
+
+// No rows: a zero gradient.
+template <typename W>
+__global__ __launch_bounds__(256) void rms_zero_kernel(Rms a) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c < a.C) static_cast<W*>(a.dw)[c] = (W)0.0f;
+}
+
+// Rows as they are, in 8 bits: a lane a vector.  A row has whole 128-channel blocks of
+// vectors, so that a block's lanes are neighbours.
+template <typename T>
+__global__ __launch_bounds__(256) void quantize_kernel(Rms a, unsigned vectors, unsigned per_row, FmDivisor by) {
+  constexpr int E = 16 / (int)sizeof(T);
+  const unsigned at = blockIdx.x * 256 + threadIdx.x;
+  if ((at & ~63u) >= vectors) return;  // whole waves
+  const unsigned row = at < vectors ? fm_div(at, by) : 0;
+  const int i = at < vectors ? (int)(at - row * per_row) : a.C;  // C: past every row's end
+  const typename Vec<T, E>::type t = row_load<T, E>(static_cast<const T*>(a.x) + row * a.ld_x, i, a.C);
+  float v[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = widen(t[e]);
+  store_8_bits<E, 128 / E>(v, static_cast<unsigned char*>(a.y) + (long)row * a.C,
+                           static_cast<unsigned char*>(a.scales) + (long)row * ((a.C + 127) / 128), i, a.C);
+}
+
+// Weights [N][K] in 8 bits, one scale to 128 x 128 of them: a block each.
+template <typename T>
+__global__ __launch_bounds__(256) void quantize_weight_kernel(const T* w, int N, int K, unsigned char* out, unsigned char* scales) {
+  __shared__ int waves[4];
+  const int k0 = blockIdx.x * 128, n0 = blockIdx.y * 128, k = k0 + (threadIdx.x & 31) * 4;
+  const int rows = min(128, N - n0);
+  auto values = [&](int r, float (&v)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = k + e < K ? widen(w[(long)(n0 + r) * K + k + e]) : 0.0f;
+  };
+  int most = 0;
+  for (int r = threadIdx.x >> 5; r < rows; r += 8) {
+    float v[4];
+    values(r, v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) most = max(most, __builtin_bit_cast(int, fabsf(v[e])));
+  }
+  most = __builtin_bit_cast(int, lanes_max<64>(__builtin_bit_cast(float, most)));
+  if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = most;
+  __syncthreads();
+  most = max(max(waves[0], waves[1]), max(waves[2], waves[3]));
+  const int byte = scale_byte(__builtin_bit_cast(float, most));
+  if (threadIdx.x == 0) scales[(long)blockIdx.y * gridDim.x + blockIdx.x] = (unsigned char)byte;
+  for (int r = threadIdx.x >> 5; r < rows; r += 8) {
+    float v[4];
+    values(r, v);
+    const unsigned u = four_in_8_bits(v[0], v[1], v[2], v[3], byte);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (k + e < K) out[(long)(n0 + r) * K + k + e] = (unsigned char)(u >> (8 * e));
+  }
+}
+
+constexpr int MOST_CHANNELS = 1 << 26;
+constexpr long MOST_ROWS = 1 << 23;  // of a launch: a grid has at most 2^32 threads
+
+int rms_check(const Rms& a, int dtype, int stype, int wtype) {
+  if (a.rows < 0 || a.C <= 0 || dtype < DT_F32 || dtype > DT_F16 || (stype != dtype && stype != DT_F32) ||
+      (wtype != dtype && wtype != DT_F32) || !(a.eps >= 0.0f))
+    return FM_BAD_ARGUMENT;
+  if (a.rows > 1 && (a.ld_x < 0 || a.ld_res < 0 || a.ld_dy < 0 || a.ld_dh < 0)) return FM_BAD_ARGUMENT;
+  if (a.rows >= INT_MAX || a.C > MOST_CHANNELS) return FM_UNSUPPORTED;
+  return FM_OK;
+}
+
+// The lanes and vectors of a row: the rule of plan(), rows being whole vectors here.
+Plan rms_plan(int C, int size) {
+  const int e = 16 / size;
+  return plan((C + e - 1) / e * e, size, true);
+}
+
+enum Pass { FORWARD, BITS8, BACKWARD };
+
+template <typename T, typename S, typename W, int NV, int LPR, Pass PASS>
+void launch(const Rms& a, hipStream_t stream) {
+  if constexpr (PASS == BACKWARD)
+    hipLaunchKernelGGL((rms_backward_kernel<T, S, W, NV, LPR>), dim3(a.blocks), dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((rms_forward_kernel<T, S, W, NV, LPR, PASS == BITS8>), dim3(fm_ceil_div(a.rows, 256 / LPR)), dim3(256),
+                       0, stream, a);
+}
+
+// False where the plan has no kernel (none of plan()'s).
+template <typename T, typename S, typename W, Pass PASS>
+bool launch_plan(const Rms& a, const Plan& p, hipStream_t stream) {
+  if (p.lpr == 16) return launch<T, S, W, 1, 16, PASS>(a, stream), true;
+  if (p.lpr == 64) {
+    if (p.nv == 1) return launch<T, S, W, 1, 64, PASS>(a, stream), true;
+    if (p.nv == 2) return launch<T, S, W, 2, 64, PASS>(a, stream), true;
+    if (p.nv == 4) return launch<T, S, W, 4, 64, PASS>(a, stream), true;
+  } else {
+    if (p.nv == 2) return launch<T, S, W, 2, 256, PASS>(a, stream), true;
+    if (p.nv == 4) return launch<T, S, W, 4, 256, PASS>(a, stream), true;
+    if constexpr (sizeof(T) == 4)
+      if (p.nv == 8) return launch<T, S, W, 8, 256, PASS>(a, stream), true;
+  }
+  return false;
+}
+
+template <typename T, typename S, typename W, Pass PASS>
+int run(Rms a, hipStream_t stream) {
+  const Plan p = rms_plan(a.C, sizeof(T));
+  if (PASS == BACKWARD && a.rows == 0) {
+    hipLaunchKernelGGL((rms_zero_kernel<W>), dim3(fm_ceil_div(a.C, 256)), dim3(256), 0, stream, a);
+    return (int)hipGetLastError();
+  }
+  if (PASS != BACKWARD && a.rows > MOST_ROWS) {
+    Rms part = a;
+    for (long first = 0; first < a.rows; first += MOST_ROWS) {
+      part.rows = std::min(MOST_ROWS, a.rows - first);
+      part.x = static_cast<const T*>(a.x) + first * a.ld_x;
+      if (a.res) part.res = static_cast<const S*>(a.res) + first * a.ld_res;
+      if (a.sum) part.sum = static_cast<S*>(a.sum) + first * a.C;
+      part.y = static_cast<char*>(a.y) + first * a.C * (PASS == BITS8 ? 1 : sizeof(T));
+      if (a.scales) part.scales = static_cast<char*>(a.scales) + first * ((a.C + 127) / 128);
+      if (a.rstd) part.rstd = a.rstd + first;
+      if (const int status = run<T, S, W, PASS>(part, stream)) return status;
+    }
+    return FM_OK;
+  }
+  a.blocks = PASS == BACKWARD ? backward_blocks(a.rows, p, sizeof(T)) : 0;
+  if (p.nv == 0) {
+    if constexpr (PASS == BACKWARD)
+      hipLaunchKernelGGL((rms_backward_any_kernel<T, S, W>), dim3(a.blocks), dim3(256), 0, stream, a);
+    else
+      hipLaunchKernelGGL((rms_forward_any_kernel<T, S, W, PASS == BITS8>), dim3((unsigned)a.rows), dim3(256), 0, stream, a);
+  } else if (!launch_plan<T, S, W, PASS>(a, p, stream)) {
+    return FM_UNSUPPORTED;
+  }
+  if (PASS == BACKWARD && a.dw && (a.blocks > 1 || p.nv == 0))
+    hipLaunchKernelGGL((rms_join_kernel<W>), dim3(fm_ceil_div(a.C, 32)), dim3(1024), 0, stream, a);
+  return (int)hipGetLastError();
+}
+
+template <typename T, Pass PASS>
+int run_types(const Rms& a, bool wide_stream, bool wide_weight, hipStream_t stream) {
+  if constexpr (std::is_same<T, float>::value) return run<float, float, float, PASS>(a, stream);
+  else if (wide_stream) return wide_weight ? run<T, float, float, PASS>(a, stream) : run<T, float, T, PASS>(a, stream);
+  else return wide_weight ? run<T, T, float, PASS>(a, stream) : run<T, T, T, PASS>(a, stream);
+}
+
+template <Pass PASS>
+int dispatch(const Rms& a, int dtype, int stype, int wtype, hipStream_t stream) {
+  const bool s = stype == DT_F32, w = wtype == DT_F32;
+  if (dtype == DT_F32) return run_types<float, PASS>(a, s, w, stream);
+  return dtype == DT_BF16 ? run_types<__bf16, PASS>(a, s, w, stream) : run_types<_Float16, PASS>(a, s, w, stream);
+}
+
+template <typename T>
+int quantize(Rms a, hipStream_t stream) {
+  constexpr int E = 16 / (int)sizeof(T);
+  const long per_row = (a.C + 127) / 128 * (128 / E), most = std::max<long>(1, (1u << 30) / per_row);
+  const FmDivisor by = fm_divisor((unsigned)per_row);
+  const Rms whole = a;
+  for (long first = 0; first < whole.rows; first += most) {
+    a.rows = std::min(most, whole.rows - first);
+    a.x = static_cast<const T*>(whole.x) + first * whole.ld_x;
+    a.y = static_cast<char*>(whole.y) + first * whole.C;
+    a.scales = static_cast<char*>(whole.scales) + first * ((whole.C + 127) / 128);
+    const long vectors = a.rows * per_row;
+    hipLaunchKernelGGL((quantize_kernel<T>), dim3(fm_ceil_div(vectors, 256)), dim3(256), 0, stream, a, (unsigned)vectors,
+                       (unsigned)per_row, by);
+  }
+  return (int)hipGetLastError();
+}
+
+template <typename T>
+int quantize_weight(const void* w, int N, int K, void* out, void* scales, hipStream_t stream) {
+  hipLaunchKernelGGL((quantize_weight_kernel<T>), dim3(fm_ceil_div(K, 128), fm_ceil_div(N, 128)), dim3(256), 0, stream,
+                     static_cast<const T*>(w), N, K, static_cast<unsigned char*>(out), static_cast<unsigned char*>(scales));
+  return (int)hipGetLastError();
+}
+
+}  // namespace
+
+extern "C" {
+
+int fm_rms_norm_forward(const void* x, long ld_x, const void* residual, long ld_residual, const void* gamma, long rows,
+                        int channels, float eps, int dtype, int stream_dtype, int weight_dtype, void* y, void* h, float* rstd,
+                        hipStream_t stream) {
+  Rms a{};
+  a.x = x, a.res = residual, a.w = gamma, a.y = y, a.sum = h, a.rstd = rstd;
+  a.rows = rows, a.ld_x = ld_x, a.ld_res = ld_residual, a.C = channels, a.eps = eps;
+  if (const int status = rms_check(a, dtype, stream_dtype, weight_dtype)) return status;
+  if (rows == 0) return FM_OK;
+  if (!x || !y || !rstd || (residual && !h)) return FM_BAD_ARGUMENT;
+  return dispatch<FORWARD>(a, dtype, stream_dtype, weight_dtype, stream);
+}
+
+int fm_rms_norm_quantized(const void* x, long ld_x, const void* residual, long ld_residual, const void* gamma, long rows,
+                          int channels, float eps, int dtype, int stream_dtype, int weight_dtype, void* y, void* scales, void* h,
+                          hipStream_t stream) {
+  Rms a{};
+  a.x = x, a.res = residual, a.w = gamma, a.y = y, a.scales = scales, a.sum = h;
+  a.rows = rows, a.ld_x = ld_x, a.ld_res = ld_residual, a.C = channels, a.eps = eps;
+  if (const int status = rms_check(a, dtype, stream_dtype, weight_dtype)) return status;
+  if (rows == 0) return FM_OK;
+  if (!x || !y || !scales || (residual && !h)) return FM_BAD_ARGUMENT;
+  return dispatch<BITS8>(a, dtype, stream_dtype, weight_dtype, stream);
+}
+
+// Room for the most blocks that the call runs; none where its plan is one block.
+size_t fm_rms_norm_backward_workspace_bytes(long rows, int channels) {
+  if (rows <= 0 || channels <= 0) return 0;
+  if (rows <= (channels <= 512 ? 4 * ONE_BLOCK : channels <= 8192 ? ONE_BLOCK : 0)) return 0;
+  return (size_t)std::min<long>(1024, rows) * channels * sizeof(float);
+}
+
+int fm_rms_norm_backward(const void* dy, long ld_dy, const void* x, long ld_x, const void* residual, long ld_residual,
+                         const void* gamma, const float* rstd, const void* dh, long ld_dh, long rows, int channels, int dtype,
+                         int stream_dtype, int weight_dtype, void* dx, void* dresidual, void* dgamma, float* workspace,
+                         size_t workspace_bytes, hipStream_t stream) {
+  Rms a{};
+  a.x = x, a.res = residual, a.dy = dy, a.w = gamma, a.dh = dh, a.dx = dx, a.dres = dresidual, a.dw = dgamma;
+  a.rstd = const_cast<float*>(rstd), a.part = workspace;
+  a.rows = rows, a.ld_x = ld_x, a.ld_res = ld_residual, a.ld_dy = ld_dy, a.ld_dh = ld_dh, a.C = channels;
+  if (const int status = rms_check(a, dtype, stream_dtype, weight_dtype)) return status;
+  if (rows == 0 && !dgamma) return FM_OK;
+  if (rows > 0 && ((!x && !residual) || !dy || !dresidual || !rstd)) return FM_BAD_ARGUMENT;
+  if (rows > 0 && dgamma && workspace_bytes < fm_rms_norm_backward_workspace_bytes(rows, channels)) return FM_WORKSPACE_TOO_SMALL;
+  if (workspace_bytes > 0 && !workspace) return FM_BAD_ARGUMENT;
+  return dispatch<BACKWARD>(a, dtype, stream_dtype, weight_dtype, stream);
+}
+
+int fm_quantize_rows(const void* x, long ld_x, long rows, int channels, int dtype, void* y, void* scales, hipStream_t stream) {
+  Rms a{};
+  a.x = x, a.ld_x = ld_x, a.rows = rows, a.C = channels, a.y = y, a.scales = scales;
+  if (const int status = rms_check(a, dtype, dtype, dtype)) return status;
+  if (rows == 0) return FM_OK;
+  if (!x || !y || !scales) return FM_BAD_ARGUMENT;
+  return dtype == DT_F32 ? quantize<float>(a, stream) : dtype == DT_BF16 ? quantize<__bf16>(a, stream) : quantize<_Float16>(a, stream);
+}
+
+int fm_quantize_weight(const void* weight, int out_features, int in_features, int dtype, void* values, void* scales,
+                       hipStream_t stream) {
+  if (out_features <= 0 || in_features <= 0 || dtype < DT_F32 || dtype > DT_F16 || !weight || !values || !scales)
+    return FM_BAD_ARGUMENT;
+  if (out_features > 128 * 65535 || in_features > MOST_CHANNELS) return FM_UNSUPPORTED;
+  return dtype == DT_F32    ? quantize_weight<float>(weight, out_features, in_features, values, scales, stream)
+         : dtype == DT_BF16 ? quantize_weight<__bf16>(weight, out_features, in_features, values, scales, stream)
+                            : quantize_weight<_Float16>(weight, out_features, in_features, values, scales, stream);
+}
+
+}  // extern "C"

@@ -102,6 +102,15 @@ _SIGNATURES = {
     "fm_attention_backward": ([_P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P, _P, _P], _I),
     "fm_code_embedding": ([_P, _L, _L, _I, _I, _I, _P, _I, _I, _F, _I, _P, _P], _I),
     "fm_code_embedding_backward_workspace_bytes": ([_I, _I, _I, _I, _I], _S),
+    "fm_rms_norm_forward": ([_P, _L, _P, _L, _P, _L, _I, _F, _I, _I, _I, _P, _P, _P, _P], _I),
+    "fm_rms_norm_backward_workspace_bytes": ([_L, _I], _S),
+    "fm_rms_norm_backward": ([_P, _L, _P, _L, _P, _L, _P, _P, _P, _L, _L, _I, _I, _I, _I, _P, _P, _P, _P, _S, _P], _I),
+    "fm_rms_norm_quantized": ([_P, _L, _P, _L, _P, _L, _I, _F, _I, _I, _I, _P, _P, _P, _P], _I),
+    "fm_quantize_rows": ([_P, _L, _L, _I, _I, _P, _P, _P], _I),
+    "fm_quantize_weight": ([_P, _I, _I, _I, _P, _P, _P], _I),
+    "fm_linear_fp8_workspace_bytes": ([_L, _I, _I], _S),
+    "fm_linear_fp8": ([_P, _P, _P, _P, _L, _I, _I, _I, _P, _P, _S, _P], _I),
+    "fm_rotary": ([_P, _L, _L, _L, _I, _P, _L, _L, _L, _I, _P, _P, _L, _I, _L, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P, _P], _I),
     "fm_code_embedding_backward": ([_P, _L, _P, _L, _L, _I, _I, _I, _I, _I, _F, _I, _P, _P, _S, _P], _I),
 }
 

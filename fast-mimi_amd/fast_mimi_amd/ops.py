@@ -63,6 +63,13 @@ SPECS = {
     "fm_attention_backward": "in:dout i:dout_batch i:dout_row i:dout_head in:q i:q_batch i:q_row i:q_head in:k i:k_batch i:k_row i:k_head in:v i:v_batch i:v_row i:v_head in:out in:lse in:lengths i:batch i:queries i:keys i:heads i:kv_heads i:head_dim i:window f:scale i:dtype out:dq out:dk out:dv out:stats",
     "fm_code_embedding": "in:codes i:codes_batch i:codes_book i:batch i:books i:frames in:table i:entries i:dim f:scale i:dtype out:out",
     "fm_code_embedding_backward": "in:dout i:ld_dout in:codes i:codes_batch i:codes_book i:batch i:books i:frames i:entries i:dim f:scale i:dtype out:dtable out:workspace i:workspace_bytes",
+    "fm_rms_norm_forward": "in:x i:ld_x in:residual i:ld_residual in:gamma i:rows i:channels f:eps i:dtype i:stream_dtype i:weight_dtype out:y out:h out:rstd",
+    "fm_rms_norm_backward": "in:dy i:ld_dy in:x i:ld_x in:residual i:ld_residual in:gamma in:rstd in:dh i:ld_dh i:rows i:channels i:dtype i:stream_dtype i:weight_dtype out:dx out:dresidual out:dgamma out:workspace i:workspace_bytes",
+    "fm_rms_norm_quantized": "in:x i:ld_x in:residual i:ld_residual in:gamma i:rows i:channels f:eps i:dtype i:stream_dtype i:weight_dtype out:y out:scales out:h",
+    "fm_quantize_rows": "in:x i:ld_x i:rows i:channels i:dtype out:y out:scales",
+    "fm_quantize_weight": "in:weight i:out_features i:in_features i:dtype out:values out:scales",
+    "fm_linear_fp8": "in:x in:x_scales in:weight in:weight_scales i:rows i:in_features i:out_features i:dtype out:y out:workspace i:workspace_bytes",
+    "fm_rotary": "in:q i:q_batch i:q_row i:q_head i:heads in:k i:k_batch i:k_row i:k_head i:kv_heads in:frequencies in:positions i:positions_batch i:positions_bytes i:first i:batch i:length i:head_dim i:rotated i:interleaved f:scale i:inverse i:dtype out:q_out out:k_out",
 }
 
 _TYPE = {"i": "int", "f": "float"}

@@ -1,0 +1,133 @@
+"""Projections in 8 bits, for serving a model over the codes.
+
+Values are ``torch.float8_e4m3fn``; every 128 of them along a row of activations,
+and every 128 x 128 weights, share a scale that is a power of two
+(``torch.float8_e8m0fnu``), which the matrix instructions of this part apply
+themselves.  :func:`quantize_weight` lays a projection's weights out once;
+:func:`rms_norm` (a norm with its residual, straight to 8 bits) and :func:`quantize`
+make the activations; :func:`linear` is the product::
+
+    w, w_scale = quantize_weight(weight)                     # [out, in], once
+    x, x_scale, stream = rms_norm(branch, norm_weight, stream)
+    y = linear(x, x_scale, w, w_scale)                       # bfloat16 [..., out]
+
+Products are summed in FP32 and rounded once.  The same call gives the same bits.
+Outputs and scratch memory are allocated by the call, on the current stream;
+nothing synchronises, so every call may be captured into a hipGraph.  There are no
+gradients: inputs that require one are refused while gradients are recorded.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from .training import _DTYPES, _branch, _differentiable, _norm_weights, _on_gpu, _rows, _run, _scratch, _tensor
+
+__all__ = ["BLOCK", "linear", "quantize", "quantize_weight", "rms_norm"]
+
+BLOCK = 128  # values that share a scale
+_VALUES, _SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def _no_gradient(*inputs) -> None:
+    if _differentiable(*inputs):
+        raise RuntimeError("the 8-bit operators have no gradient: an input requires one (call them under torch.no_grad())")
+
+
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def quantize(x):
+    """``(values, scales)`` of ``x`` ``[..., channels]`` (FP32, bfloat16 or float16): ``values`` of its shape,
+    ``scales`` ``[..., ceil(channels / 128)]``.
+
+    A scale is the least power of two that keeps its block's largest value at or below
+    448 (2^-127 at least); values are rounded to the nearest, ties to even.  A block with
+    an infinity or NaN has the scale NaN.
+    """
+    _no_gradient(x)
+    x = _tensor("x", x)
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"x must have a last dimension, got shape {tuple(x.shape)}")
+    device = _on_gpu(x=x)
+    c = x.shape[-1]
+    values = x.new_empty(x.shape, dtype=_VALUES)
+    scales = x.new_empty((*x.shape[:-1], _blocks(c)), dtype=_SCALES)
+    if x.numel():
+        rows, pitch = _rows(x)
+        _run(device, "fm_quantize_rows", rows, pitch, x.numel() // c, c, _DTYPES[x.dtype], values, scales)
+    return values, scales
+
+
+def quantize_weight(weight):
+    """``(values, scales)`` of weights ``[out, in]``, as :func:`linear` takes them: ``scales`` is
+    ``[ceil(out / 128), ceil(in / 128)]``, made as :func:`quantize` makes them."""
+    _no_gradient(weight)
+    weight = _tensor("weight", weight)
+    if weight.dim() != 2 or 0 in weight.shape:
+        raise ValueError(f"weight must be [out, in], got shape {tuple(weight.shape)}")
+    device = _on_gpu(weight=weight)
+    n, k = weight.shape
+    values = weight.new_empty((n, k), dtype=_VALUES)
+    scales = weight.new_empty((_blocks(n), _blocks(k)), dtype=_SCALES)
+    _run(device, "fm_quantize_weight", weight.contiguous(), n, k, _DTYPES[weight.dtype], values, scales)
+    return values, scales
+
+
+def rms_norm(x, weight=None, residual=None, eps: float = 1e-5):
+    """``(values, scales, h)``: the ``y`` of :func:`fast_mimi_amd.training.rms_norm_forward` as
+    :func:`quantize` gives it, rounded once, from FP32, and its ``h``."""
+    _no_gradient(x, weight, residual)
+    x, residual = _branch(x, residual, eps)
+    weight, _, wtype = _norm_weights(x, weight, None)
+    device = _on_gpu(x=x, residual=residual, weight=weight)
+    c = x.shape[-1]
+    values = x.new_empty(x.shape, dtype=_VALUES)
+    scales = x.new_empty((*x.shape[:-1], _blocks(c)), dtype=_SCALES)
+    h = x if residual is None else residual.new_empty(x.shape)
+    if x.numel():
+        rows_x, pitch = _rows(x)
+        rows_r, pitch_r = (None, 0) if residual is None else _rows(residual)
+        _run(device, "fm_rms_norm_quantized", rows_x, pitch, rows_r, pitch_r, weight, x.numel() // c, c, float(eps),
+             _DTYPES[x.dtype], _DTYPES[h.dtype], _DTYPES[wtype], values, scales, None if residual is None else h)
+    return values, scales, h
+
+
+def linear(x, x_scale, weight, weight_scale, dtype: torch.dtype = torch.bfloat16):
+    """``x @ weight.T`` ``[..., out]`` of 8-bit ``x`` ``[..., in]`` and ``weight`` ``[out, in]`` with their scales, in
+    ``dtype`` (FP32, bfloat16 or float16).
+
+    ``x`` and ``x_scale`` are what :func:`quantize` or :func:`rms_norm` gave, ``weight`` and
+    ``weight_scale`` what :func:`quantize_weight` did.  ``in`` must be a multiple of 16.
+    """
+    x, weight = _tensor("x", x, (_VALUES,)), _tensor("weight", weight, (_VALUES,))
+    x_scale, weight_scale = _tensor("x_scale", x_scale, (_SCALES,)), _tensor("weight_scale", weight_scale, (_SCALES,))
+    if dtype not in _DTYPES:
+        raise TypeError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
+    if weight.dim() != 2 or 0 in weight.shape:
+        raise ValueError(f"weight must be [out, in], got shape {tuple(weight.shape)}")
+    n, k = weight.shape
+    if x.dim() < 1 or x.shape[-1] != k:
+        raise ValueError(f"x must be [..., {k}] for weight {(n, k)}, got shape {tuple(x.shape)}")
+    if k % 16:
+        raise ValueError(f"the inputs of a projection must be a multiple of 16, got {k}")
+    if x_scale.shape != (*x.shape[:-1], _blocks(k)):
+        raise ValueError(f"x_scale must have shape {(*x.shape[:-1], _blocks(k))}, got {tuple(x_scale.shape)}")
+    if weight_scale.shape != (_blocks(n), _blocks(k)):
+        raise ValueError(f"weight_scale must have shape {(_blocks(n), _blocks(k))}, got {tuple(weight_scale.shape)}")
+    device = _on_gpu(x=x, x_scale=x_scale, weight=weight, weight_scale=weight_scale)
+    rows = x.numel() // k
+    y = x.new_empty((*x.shape[:-1], n), dtype=dtype)
+    if rows:
+        x, weight = _aligned(x), _aligned(weight)
+        ws, size = _scratch(y, "fm_linear_fp8_workspace_bytes", rows, k, n)
+        _run(device, "fm_linear_fp8", x, x_scale.contiguous(), weight, weight_scale.contiguous(), rows, k, n, _DTYPES[dtype], y,
+             ws, size)
+    return y
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous, from a 16-byte address on."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t

@@ -1,11 +1,12 @@
-"""Operators with gradients: LayerNorm, sliding-window attention, codebook embedding.
+"""Operators with gradients: norms, rotary positions, attention, codebook embedding.
 
 What a transformer over codec frames and the codebooks below it need to be
 trained, on the HIP kernels of ``libfast_mimi_amd.so``:
 
-* :func:`layer_norm`, :func:`window_attention` and :func:`code_embedding` are
-  differentiable (``torch.autograd``, reverse mode, first order: dual tensors
-  raise ``NotImplementedError``);
+* :func:`layer_norm`, :func:`rms_norm`, :func:`rotary`, :func:`window_attention`,
+  :func:`cross_attention` and :func:`code_embedding` are differentiable
+  (``torch.autograd``, reverse mode, first order: dual tensors raise
+  ``NotImplementedError``);
 * ``*_forward`` / ``*_backward`` are the same without autograd, for a training
   loop that keeps its own tape, or that records its step in a hipGraph.
 
@@ -41,6 +42,13 @@ __all__ = [
     "layer_norm",
     "layer_norm_backward",
     "layer_norm_forward",
+    "rms_norm",
+    "rms_norm_backward",
+    "rms_norm_forward",
+    "rotary",
+    "rotary_backward",
+    "rotary_forward",
+    "rotary_frequencies",
     "window_attention",
     "window_attention_backward",
     "window_attention_forward",
@@ -145,7 +153,7 @@ def _apply(function, inputs, *args):
                            "and is still alive: drop the eager graph (and what else holds the leaf's gradient accumulator), "
                            "make it on another stream, or capture the *_forward and *_backward functions")
     out = function.apply(*args)
-    default = torch._C._cuda_getCurrentRawStream(out.device.index) == 0
+    default = torch._C._cuda_getCurrentRawStream((out[0] if isinstance(out, tuple) else out).device.index) == 0
     for node in _accumulators(inputs):
         node.metadata.setdefault(_DEFAULT_STREAM, default)
     return out
@@ -246,6 +254,254 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
     if not _differentiable(x, weight, bias):
         return layer_norm_forward(x, weight, bias, eps)[0]
     return _apply(_LayerNorm, (x, weight, bias), x, weight, bias, eps)
+
+
+# ----------------------------------------------------------------- RMS norm
+def _branch(x, residual, eps):
+    """A branch and its residual stream, checked."""
+    x = _tensor("x", x)
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"x must have a last dimension to normalise, got shape {tuple(x.shape)}")
+    if residual is not None:
+        residual = _tensor("residual", residual, (x.dtype,) if x.dtype == torch.float32 else (x.dtype, torch.float32))
+        if residual.shape != x.shape:
+            raise ValueError(f"residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    return x, residual
+
+
+def rms_norm_forward(x, weight=None, residual=None, eps: float = 1e-5):
+    """``(y, h, rstd)`` of the RMS norm over the last dimension of ``h = x + residual``.
+
+    ``y = h * rstd * weight`` has ``x``'s type; ``h``, the stream's next value, that of
+    ``residual``: ``x``'s, or FP32.  ``y`` is formed from the sum before it is rounded.
+    Without a residual ``h`` is ``x`` itself.  ``weight`` (optional) has ``x``'s type or
+    FP32; ``rstd`` is FP32, one per row, for :func:`rms_norm_backward`.
+    """
+    x, residual = _branch(x, residual, eps)
+    weight, _, wtype = _norm_weights(x, weight, None)
+    device = _on_gpu(x=x, residual=residual, weight=weight)
+    rows_x, pitch = _rows(x)
+    rows_r, pitch_r = (None, 0) if residual is None else _rows(residual)
+    y = x.new_empty(x.shape)
+    h = x if residual is None else residual.new_empty(x.shape)
+    rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    rows = rstd.numel()
+    if rows:
+        _run(device, "fm_rms_norm_forward", rows_x, pitch, rows_r, pitch_r, weight, rows, x.shape[-1], float(eps), _DTYPES[x.dtype],
+             _DTYPES[h.dtype], _DTYPES[wtype], y, None if residual is None else h, rstd)
+    return y, h, rstd
+
+
+def rms_norm_backward(grad, x, rstd, weight=None, residual=None, grad_h=None):
+    """``(dx, dresidual, dweight)`` for the gradients ``grad`` of ``y`` and ``grad_h`` (optional)
+    of ``h``, the outputs of :func:`rms_norm_forward` for ``x`` and ``residual``.
+
+    In the place of both, ``x`` may be the forward's ``h``: of an FP32 stream that says the
+    same and is one tensor less to keep; of a 16-bit one its rounding shows in the gradients.
+    ``dx`` has ``grad``'s type, ``dresidual`` the stream's; where these are one, both are
+    the same tensor.  ``dweight`` is ``None`` without a weight.
+    """
+    grad = _tensor("grad", grad)
+    wide = (grad.dtype,) if grad.dtype == torch.float32 else (grad.dtype, torch.float32)
+    x = _tensor("x", x, wide if residual is None else (grad.dtype,))
+    residual = None if residual is None else _tensor("residual", residual, wide)
+    rstd = _tensor("rstd", rstd, (torch.float32,))
+    if x.dim() < 1 or x.shape[-1] == 0 or grad.shape != x.shape:
+        raise ValueError(f"grad must have x's shape {tuple(x.shape)}, got {tuple(grad.shape)}")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
+    if rstd.shape != x.shape[:-1] or not rstd.is_contiguous():
+        raise ValueError("rstd must be what rms_norm_forward returned for x")
+    weight, _, wtype = _norm_weights(grad, weight, None)
+    stream = x.dtype if residual is None else residual.dtype
+    if grad_h is not None:
+        grad_h = _tensor("grad_h", grad_h, (stream,))
+        if grad_h.shape != x.shape:
+            raise ValueError(f"grad_h must have x's shape {tuple(x.shape)}, got {tuple(grad_h.shape)}")
+    device = _on_gpu(x=x, residual=residual, grad=grad, rstd=rstd, grad_h=grad_h, weight=weight)
+    dresidual = x.new_empty(x.shape, dtype=stream)
+    dx = dresidual if grad.dtype == stream else grad.new_empty(x.shape)
+    dw = None if weight is None else torch.empty_like(weight)
+    rows, c = rstd.numel(), x.shape[-1]
+    ws, size = (None, 0) if dw is None else _scratch(x, "fm_rms_norm_backward_workspace_bytes", rows, c)
+    (x, ld_x), (grad, ld_dy) = _rows(x), _rows(grad)
+    residual, ld_r = (None, 0) if residual is None else _rows(residual)
+    grad_h, ld_dh = (None, 0) if grad_h is None else _rows(grad_h)
+    # The sum alone stands in the stream's place.
+    parts = (x, ld_x, residual, ld_r) if residual is not None or x.dtype == grad.dtype else (None, 0, x, ld_x)
+    _run(device, "fm_rms_norm_backward", grad, ld_dy, *parts, weight, rstd, grad_h, ld_dh, rows, c, _DTYPES[grad.dtype],
+         _DTYPES[stream], _DTYPES[wtype], None if dx is dresidual else dx, dresidual, dw, ws, size)
+    return dx, dresidual, dw
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        ctx.set_materialize_grads(False)
+        y, h, rstd = rms_norm_forward(x, weight, residual, eps)
+        # An FP32 stream's sum is all that the backward pass needs of it.
+        parts = (h, None) if h.dtype == torch.float32 else (x, residual)
+        ctx.save_for_backward(*parts, weight, rstd)
+        ctx.branch = x.dtype
+        return y if residual is None else (y, h)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, grad_h=None):
+        x, residual, weight, rstd = ctx.saved_tensors
+        if grad is None and grad_h is None:
+            return None, None, None, None
+        if grad is None:
+            grad = torch.zeros(x.shape, dtype=ctx.branch, device=x.device)
+        dx, dresidual, dw = rms_norm_backward(grad, x, rstd, weight, residual, grad_h)
+        return tuple(g if need else None for g, need in zip((dx, dw, dresidual, None), ctx.needs_input_grad))
+
+
+def rms_norm(x, weight=None, residual=None, eps: float = 1e-5):
+    """RMS norm over the last dimension, differentiable: ``y``, or with a residual ``(y, h)``,
+    ``h = x + residual`` being the stream that the next branch is added to (see
+    :func:`rms_norm_forward` for the types)."""
+    if not _differentiable(x, weight, residual):
+        y, h, _ = rms_norm_forward(x, weight, residual, eps)
+        return y if residual is None else (y, h)
+    return _apply(_RmsNorm, (x, weight, residual), x, weight, residual, eps)
+
+
+# --------------------------------------------------------- rotary positions
+def rotary_frequencies(dim: int, base: float = 10_000.0, factor: float = 1.0, method: str = "linear", context: int | None = None,
+                       fast: float = 32.0, slow: float = 1.0, device=None) -> torch.Tensor:
+    """Radians per position of ``dim / 2`` channel pairs, ``base ** (-2 i / dim)``, in float64.
+
+    ``factor`` stretches them for contexts that many times as long:
+
+    * ``"linear"``: every frequency divided by it;
+    * ``"base"``: the base raised, such that the slowest pair is slower by it and the fastest as it was;
+    * ``"ramp"``: pairs with more than ``fast`` turns within ``context`` positions, the length that the model knows, as
+      they were, those with fewer than ``slow`` slower by it, linearly in the turns between.
+    """
+    if not isinstance(dim, int) or isinstance(dim, bool) or dim <= 0 or dim % 2:
+        raise ValueError(f"dim must be positive and even, got {dim!r}")
+    if not (base > 0 and factor > 0 and math.isfinite(base) and math.isfinite(factor)):
+        raise ValueError(f"base and factor must be positive and finite, got {base} and {factor}")
+    if method not in ("linear", "base", "ramp"):
+        raise ValueError(f"method must be linear, base or ramp, got {method!r}")
+    if method == "base" and factor != 1.0:
+        if dim == 2:
+            raise ValueError("one pair has no slower one: method base needs dim of 4 or more")
+        base = base * factor ** (dim / (dim - 2))
+    f = float(base) ** (-torch.arange(0, dim, 2, dtype=torch.float64) / dim)
+    if method == "linear":
+        f = f / factor
+    elif method == "ramp":
+        if context is None or not context > 0 or not fast > slow:
+            raise ValueError(f"method ramp needs a positive context and fast > slow, got {context}, {fast} and {slow}")
+        keep = ((context * f / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+        f = f * keep + f / factor * (1 - keep)
+    return f if device is None else f.to(device)
+
+
+def _rotary_input(q, k, frequencies, positions, scale):
+    q = _tensor("q", q)
+    k = None if k is None else _tensor("k", k, (q.dtype,))
+    for name, t in (("q", q), ("k", k)):
+        if t is not None and t.dim() != 4:
+            raise ValueError(f"{name} must be [batch, positions, heads, head_dim], got shape {tuple(t.shape)}")
+    b, t, _, d = q.shape
+    if k is not None and (k.shape[:2] != (b, t) or k.shape[3] != d):
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} do not belong together")
+    if not 0 < d <= 512:
+        raise ValueError(f"head_dim must be from 1 to 512, got {d}")
+    frequencies = _tensor("frequencies", frequencies, (torch.float64,))
+    if frequencies.dim() != 1 or not 0 < 2 * frequencies.numel() <= d:
+        raise ValueError(f"frequencies must be [pairs], at most {d // 2} for heads of {d}, got shape {tuple(frequencies.shape)}")
+    first = 0
+    if isinstance(positions, int) and not isinstance(positions, bool):
+        first, positions = positions, None
+        if not -(1 << 62) < first < 1 << 62:
+            raise ValueError(f"positions must start within 62 bits, got {first}")
+    if positions is not None:
+        positions = _tensor("positions", positions, (torch.int32, torch.int64))
+        if positions.shape not in ((t,), (b, t)):
+            raise ValueError(f"positions must have shape {(t,)} or {(b, t)}, got {tuple(positions.shape)}")
+        positions = positions.contiguous()
+    if b * t > 1 << 24:
+        raise ValueError(f"at most {1 << 24} positions in all, got {b * t}")
+    scale = float(scale)
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite, got {scale}")
+    return q, k, frequencies.contiguous(), positions, first, scale
+
+
+def _rotate(q, k, frequencies, positions, interleaved, scale, inverse):
+    q, k, frequencies, positions, first, scale = _rotary_input(q, k, frequencies, positions, scale)
+    device = _on_gpu(q=q, k=k, frequencies=frequencies, positions=positions)
+    b, t, _, d = q.shape
+
+    def heads(x):
+        if x is None:
+            return None, 0, 0, 0, 0
+        if x.stride(3) != 1 and d > 1:
+            x = x.contiguous()
+        return x, *x.stride()[:3], x.shape[2]
+
+    q_out = q.new_empty(q.shape)
+    k_out = None if k is None else k.new_empty(k.shape)
+    if b and t and q.shape[2] + (0 if k is None else k.shape[2]):
+        batch, size = (0, 8) if positions is None else (t if positions.dim() == 2 else 0, positions.element_size())
+        _run(device, "fm_rotary", *heads(q), *heads(k), frequencies, positions, batch, size, first, b, t, d,
+             2 * frequencies.numel(), int(bool(interleaved)), scale, inverse, _DTYPES[q.dtype], q_out, k_out)
+    return q_out, k_out
+
+
+def rotary_forward(q, k, frequencies, positions=None, interleaved: bool = False, scale: float = 1.0):
+    """``(q, k)`` turned by their positions, in one launch.
+
+    ``q`` is ``[batch, positions, heads, head_dim]``, ``k`` ``[batch, positions, kv_heads,
+    head_dim]`` or ``None`` (any strides; slices of a packed projection are read in place).
+    ``frequencies`` (float64 ``[pairs]``, see :func:`rotary_frequencies`) are radians per
+    position: the first ``2 * pairs`` channels of a head are turned, pair ``i`` being
+    channels ``(i, i + pairs)`` or, ``interleaved``, ``(2 i, 2 i + 1)``, and come ``scale`` times
+    as large; the others are copied.  ``positions``: int32 or int64 ``[positions]`` or
+    ``[batch, positions]``, or the first position (``None``: 0).
+
+    Angles are formed in 64 bits: positions of any size are as exact as small ones.  At
+    most 2^24 positions in all, heads of 512.
+    """
+    return _rotate(q, k, frequencies, positions, interleaved, scale, 0)
+
+
+def rotary_backward(dq, dk, frequencies, positions=None, interleaved: bool = False, scale: float = 1.0):
+    """``(dq, dk)`` before the rotation for the gradients of :func:`rotary_forward`'s outputs
+    (``dk`` may be ``None``): the same rotation backwards."""
+    return _rotate(dq, dk, frequencies, positions, interleaved, scale, 1)
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, frequencies, positions, interleaved, scale):
+        tensor = isinstance(positions, torch.Tensor)
+        ctx.save_for_backward(frequencies, positions if tensor else None)
+        ctx.how = None if tensor else positions, interleaved, scale
+        q, k = rotary_forward(q, k, frequencies, positions, interleaved, scale)
+        return q if k is None else (q, k)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq, dk=None):
+        frequencies, positions = ctx.saved_tensors
+        first, interleaved, scale = ctx.how
+        dq, dk = rotary_backward(dq, dk, frequencies, first if positions is None else positions, interleaved, scale)
+        return tuple(g if need else None for g, need in zip((dq, dk, None, None, None, None), ctx.needs_input_grad))
+
+
+def rotary(q, k, frequencies, positions=None, interleaved: bool = False, scale: float = 1.0):
+    """``(q, k)`` turned by their positions, differentiable in both (see :func:`rotary_forward`)."""
+    if not _differentiable(q, k):
+        return rotary_forward(q, k, frequencies, positions, interleaved, scale)
+    out = _apply(_Rotary, (q, k), q, k, frequencies, positions, interleaved, scale)
+    return out if k is not None else (out, None)
 
 
 # ---------------------------------------------------------------- attention

@@ -645,6 +645,94 @@ int fm_code_embedding_backward(const void* dout, long ld_dout, const int64_t* co
                                int entries, int dim, float scale, int dtype, void* dtable,
                                void* workspace, size_t workspace_bytes, hipStream_t stream);
 
+/*
+ * RMS norm of a branch added to its residual stream: h = x + residual, rstd = 1 /
+ * sqrt(mean of h^2 + eps), y = h rstd gamma, from the sum before it is rounded to
+ * stream_dtype.  x has rows of `channels` elements at a pitch of ld_x elements, residual
+ * (of stream_dtype: dtype, or FP32) at ld_residual; rows may start at any element.
+ * residual NULL: y of x alone, h (then NULL) is not written.  y (dtype), h
+ * (stream_dtype) and rstd [rows] are contiguous; h may be residual itself.  gamma
+ * (weight_dtype: dtype, or FP32) may be NULL (one).  Fewer than 2^31 - 1 rows, at most
+ * 2^26 channels.
+ * Stands where a model over the codes has it in the place of nn.LayerNorm
+ * (model.py:2028-2061) and the residual's addition behind it.
+ */
+int fm_rms_norm_forward(const void* x, long ld_x, const void* residual, long ld_residual,
+                        const void* gamma, long rows, int channels, float eps, int dtype,
+                        int stream_dtype, int weight_dtype, void* y, void* h, float* rstd,
+                        hipStream_t stream);
+
+/*
+ * Its gradients, of the forward's x and residual: with hh = (x + residual) rstd and g = dy
+ * gamma, dresidual = dh + rstd (g - hh mean(g hh)) in stream_dtype, dx the same in dtype
+ * (NULL where the types are one and the caller takes dresidual), dgamma = the sum over
+ * rows of dy hh (weight_dtype; NULL to leave it).  dh (stream_dtype; NULL for none) is the
+ * gradient that h has from elsewhere.  Either x or residual may be NULL: of an FP32 stream
+ * the forward's h as the residual says the same and is one tensor less to read.
+ * dx and dresidual are contiguous.  The workspace holds the row blocks' partial sums
+ * and is needed where dgamma is given.
+ */
+size_t fm_rms_norm_backward_workspace_bytes(long rows, int channels);
+int fm_rms_norm_backward(const void* dy, long ld_dy, const void* x, long ld_x, const void* residual,
+                         long ld_residual, const void* gamma, const float* rstd, const void* dh,
+                         long ld_dh, long rows, int channels, int dtype, int stream_dtype,
+                         int weight_dtype, void* dx, void* dresidual, void* dgamma,
+                         float* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * Rotary positions of queries [batch][length][heads][head_dim] and keys
+ * [..][kv_heads][..] (either may have no heads): of each head's first `rotated`
+ * channels, pair i - channels (i, i + rotated / 2), or (2 i, 2 i + 1) with interleaved -
+ * goes (a, b) -> scale (a cos - b sin, b cos + a sin) at the angle position *
+ * frequencies[i]; the others are copied.  frequencies are rotated / 2 doubles, radians
+ * per position.  positions holds [length] per batch item, positions_batch apart (0: the
+ * same for all), of positions_bytes 4 or 8; NULL: first, first + 1, ...  inverse turns
+ * back (the gradient).  q / k are strided (elements; channels adjacent), q_out / k_out
+ * contiguous, other memory than q / k.  head_dim <= 512, batch * length <= 2^24.
+ * Replaces MimiRotaryEmbedding and its use in MimiAttention (model.py:1484-1535, :1870-1961) where the
+ * transformer is trained, with positions, pairings and frequencies of its own.
+ */
+int fm_rotary(const void* q, long q_batch, long q_row, long q_head, int heads, const void* k,
+              long k_batch, long k_row, long k_head, int kv_heads, const double* frequencies,
+              const void* positions, long positions_batch, int positions_bytes, long first,
+              int batch, int length, int head_dim, int rotated, int interleaved, float scale,
+              int inverse, int dtype, void* q_out, void* k_out, hipStream_t stream);
+
+/*
+ * 8 bits.  Values are e4m3 (no infinities, largest 448); each block of 128 of them along
+ * a row of activations, or of 128 x 128 weights, shares a scale 2^(byte - 127) (e8m0,
+ * the least that keeps the block's largest value at or below 448; 255, NaN, for a block
+ * that holds an infinity or NaN).  Last blocks may be shorter.
+ *
+ * fm_rms_norm_quantized is fm_rms_norm_forward with y in 8 bits: y [rows][channels],
+ * scales [rows][ceil(channels / 128)], rounded once, from FP32.  fm_quantize_rows does the
+ * same to rows as they are, fm_quantize_weight to weights [out_features][in_features]
+ * (contiguous; scales [ceil(out_features / 128)][ceil(in_features / 128)]).
+ */
+int fm_rms_norm_quantized(const void* x, long ld_x, const void* residual, long ld_residual,
+                          const void* gamma, long rows, int channels, float eps, int dtype,
+                          int stream_dtype, int weight_dtype, void* y, void* scales, void* h,
+                          hipStream_t stream);
+int fm_quantize_rows(const void* x, long ld_x, long rows, int channels, int dtype, void* y,
+                     void* scales, hipStream_t stream);
+int fm_quantize_weight(const void* weight, int out_features, int in_features, int dtype,
+                       void* values, void* scales, hipStream_t stream);
+
+/*
+ * y [rows][out_features] (dtype) = x weight^T of 8-bit x [rows][in_features] and weight
+ * [out_features][in_features] with their scales (above): every product times both
+ * powers of two, summed in FP32, rounded once.  All contiguous, x and weight 16-byte
+ * aligned, in_features a multiple of 16, rows at most 2097120.  The workspace holds the parts of calls
+ * whose in_features are split over blocks; NULL where its size is 0.
+ * Stands beside fm_linear (nn.Linear of the transformer layers, model.py:1870-2061)
+ * where a model over the codes is served in 8 bits.
+ */
+size_t fm_linear_fp8_workspace_bytes(long rows, int in_features, int out_features);
+int fm_linear_fp8(const void* x, const void* x_scales, const void* weight,
+                  const void* weight_scales, long rows, int in_features, int out_features,
+                  int dtype, void* y, float* workspace, size_t workspace_bytes,
+                  hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
