@@ -1,0 +1,209 @@
+// Attention to the states of another sequence, forward and backward, for training
+// and for single tokens: every query sees keys 0 .. key_lengths[b] - 1, whatever its
+// position.  FP32, bfloat16 and float16; grouped query heads; padded queries and keys.
+//
+//   S = Q K^T c, P = exp2(S - max), O = P V / sum P      (c = scale log2 e)
+//   P = exp2(S - lse), D = rowsum(dO O), dS = P (dO V^T - D)
+//   dQ = dS K scale, dV = P^T dO, dK = dS^T Q scale
+//
+// The tiles, operands and loops are the causal kernels' (fm_attention.h) without their
+// window.  What differs is the shape of the calls: the two lengths have nothing to do
+// with each other, so either may be too short to fill the chip.  A forward or dQ block
+// walks the keys and a dK / dV block the rows of its sequence; where there are few blocks and a
+// long walk, it is cut, and the parts are joined in their order.
+
+#include "fm_attention.h"
+
+namespace {
+
+// dQ, or dK and dV, from the parts of a cut walk: one wave per row of DT columns,
+// eight parts in flight.
+template <typename T, int DT, bool KEYS>
+__global__ __launch_bounds__(256) void cross_join_kernel(Attn a) {
+  const int lane = threadIdx.x & 63, R = a.T * a.G;
+  const long seqs = (long)a.B * a.KV, rows = KEYS ? 2 * seqs * a.S : seqs * R;
+  const long at = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= rows) return;
+  float sum[DT / 64] = {};
+  constexpr int AHEAD = 8;
+  for (int s = 0; s < a.splits; s += AHEAD) {
+    float v[AHEAD][DT / 64];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+      for (int d = 0; d < DT / 64; ++d) v[u][d] = a.part_o[(min(s + u, a.splits - 1) * rows + at) * DT + 64 * d + lane];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+      for (int d = 0; d < DT / 64; ++d) sum[d] += s + u < a.splits ? v[u][d] : 0.0f;
+  }
+  T* out;
+  if constexpr (KEYS) {
+    const long which = at / (seqs * a.S), row = at - which * seqs * a.S, seq = row / a.S, key = row - seq * a.S;
+    const long b = seq / a.KV, kh = seq - b * a.KV;
+    out = static_cast<T*>(which ? a.dv : a.dk) + ((b * a.S + key) * a.KV + kh) * a.D;
+  } else {
+    const int seq = (int)(at / R), r = (int)(at - (long)seq * R), b = seq / a.KV, kh = seq - b * a.KV, t = (int)fm_div(r, a.by_g);
+    const long row = ((long)b * a.T + t) * a.H + kh * a.G + (r - t * a.G);
+    out = static_cast<T*>(a.out) + row * a.D;
+    // The sum of dS puts rowsum(dO O) from the rounded O right (see attention_dq_kernel).
+    if (sizeof(T) == 2) {
+      float rest = lane < a.splits ? a.part_ml[lane * rows + at] : 0.0f;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) rest += __shfl_xor(rest, o, 64);
+      if (lane == 0) a.stats[(long)a.B * a.T * a.H + row] += rest;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < DT / 64; ++u)
+    if (64 * u + lane < a.D) out[64 * u + lane] = (T)sum[u];
+}
+
+// Into how many parts a walk of `tiles` is cut that `blocks` blocks make: until some 512
+// blocks run, at least four tiles each.
+int cut(long blocks, int tiles) { return (int)std::max<long>(1, std::min<long>({tiles / 4, 512 / std::max<long>(blocks, 1), 64})); }
+
+long sequences(const Attn& a) { return (long)a.B * a.KV; }
+int row_splits(const Attn& a) {  // forward, dQ
+  const long rows = (long)a.T * a.G;
+  return cut(sequences(a) * fm_ceil_div(rows, 32), fm_ceil_div(a.S, 128));
+}
+int key_splits(const Attn& a) {  // dK / dV
+  return cut(sequences(a) * fm_ceil_div(a.S, 32), fm_ceil_div((long)a.T * a.G, 128));
+}
+
+size_t backward_floats(const Attn& a) {
+  const size_t dt = a.D > 64 ? 128 : 64;
+  const size_t q = row_splits(a), k = key_splits(a);
+  return std::max(q > 1 ? q * sequences(a) * a.T * a.G * (dt + 1) : 0, k > 1 ? k * 2 * sequences(a) * a.S * dt : 0);
+}
+
+#define FM_CROSS_LAUNCH(kernel, own, rows, z)                                                                \
+  do {                                                                                                       \
+    const dim3 grid((unsigned)sequences(a), fm_ceil_div(rows, 32 * (own)), z);                               \
+    if ((own) == 4) hipLaunchKernelGGL((kernel<T, DT, 4, 1, true>), grid, dim3(256), 0, stream, a);          \
+    else if ((own) == 2) hipLaunchKernelGGL((kernel<T, DT, 2, 2, true>), grid, dim3(256), 0, stream, a);     \
+    else hipLaunchKernelGGL((kernel<T, DT, 1, 4, true>), grid, dim3(256), 0, stream, a);                     \
+  } while (0)
+
+template <typename T, int DT>
+int cross_forward(Attn a, hipStream_t stream) {
+  const long rows = (long)a.T * a.G;
+  const int waves = a.splits > 1 ? 1 : own_waves(a, rows);
+  FM_CROSS_LAUNCH(attention_forward_kernel, waves, rows, a.splits);
+  if (a.splits > 1)
+    hipLaunchKernelGGL((attention_join_kernel<T, DT, true>), dim3(fm_ceil_div(sequences(a) * rows, 4)), dim3(256), 0, stream, a);
+  return (int)hipGetLastError();
+}
+
+template <typename T, int DT>
+int cross_backward(Attn a, float* workspace, hipStream_t stream) {
+  const long rows = (long)a.T * a.G;
+  a.part_o = workspace;
+  if (rows > 0) {
+    a.splits = row_splits(a);
+    a.part_ml = workspace + (size_t)a.splits * sequences(a) * rows * DT;
+    const int waves = a.splits > 1 ? 1 : own_waves(a, rows);
+    FM_CROSS_LAUNCH(attention_dq_kernel, waves, rows, a.splits);
+    if (a.splits > 1)
+      hipLaunchKernelGGL((cross_join_kernel<T, DT, false>), dim3(fm_ceil_div(sequences(a) * rows, 4)), dim3(256), 0, stream, a);
+  }
+  if (a.S > 0) {
+    a.splits = key_splits(a);
+    if constexpr (HELD<T, DT>) {
+      const dim3 grid((unsigned)sequences(a), fm_ceil_div(a.S, 64), a.splits);
+      if ((long)grid.x * grid.y * grid.z > 512)
+        hipLaunchKernelGGL((attention_dkv_kernel<T, DT, 2, 2, true>), grid, dim3(256), 0, stream, a);
+      else hipLaunchKernelGGL((attention_dkv_kernel<T, DT, 2, 4, true>), grid, dim3(512), 0, stream, a);
+    } else {
+      const int waves = a.splits > 1 ? 1 : own_waves(a, a.S);
+      FM_CROSS_LAUNCH(attention_dkv_kernel, waves, a.S, a.splits);
+    }
+    if (a.splits > 1)
+      hipLaunchKernelGGL((cross_join_kernel<T, DT, true>), dim3(fm_ceil_div(2 * sequences(a) * a.S, 4)), dim3(256), 0, stream, a);
+  }
+  return (int)hipGetLastError();
+}
+
+int cross_check(const Attn& a, int dtype) {
+  if (const int status = check(a, dtype, true)) return status;
+  // A join has four rows to a block.
+  if (sequences(a) * std::max<long>((long)a.T * a.G, 2l * a.S) > 4l * INT_MAX) return FM_UNSUPPORTED;
+  return FM_OK;
+}
+
+Attn cross_sizes(int batch, int queries, int keys, int heads, int kv_heads, int head_dim, float scale) {
+  Attn a{};
+  a.B = batch, a.T = queries, a.S = keys, a.H = heads, a.KV = kv_heads, a.D = head_dim;
+  a.G = kv_heads > 0 && heads > 0 ? heads / kv_heads : 1;
+  a.window = 1, a.scale = scale, a.scale2 = scale * LOG2E, a.splits = 1;
+  a.by_g = fm_divisor((unsigned)std::max(a.G, 1));
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fm_cross_attention_forward_workspace_bytes(int batch, int queries, int keys, int heads, int kv_heads, int head_dim) {
+  const Attn a = cross_sizes(batch, queries, keys, heads, kv_heads, head_dim, 1.0f);
+  if (cross_check(a, DT_F32) != FM_OK && cross_check(a, DT_BF16) != FM_OK) return 0;
+  return batch == 0 || queries == 0 ? 0 : workspace_floats(a, row_splits(a)) * sizeof(float);
+}
+
+int fm_cross_attention_forward(const void* q, long q_batch, long q_row, long q_head, const void* k, long k_batch, long k_row,
+                               long k_head, const void* v, long v_batch, long v_row, long v_head, const int* key_lengths,
+                               const int* query_lengths, int batch, int queries, int keys, int heads, int kv_heads,
+                               int head_dim, float scale, int dtype, void* out, float* lse, float* workspace,
+                               size_t workspace_bytes, hipStream_t stream) {
+  Attn a = cross_sizes(batch, queries, keys, heads, kv_heads, head_dim, scale);
+  a.q = View{q, q_batch, q_row, q_head}, a.k = View{k, k_batch, k_row, k_head}, a.v = View{v, v_batch, v_row, v_head};
+  a.lengths = key_lengths, a.query_lengths = query_lengths, a.out = out, a.lse = lse;
+  if (const int status = cross_check(a, dtype)) return status;
+  if (batch == 0 || queries == 0) return FM_OK;
+  if (!q || !out || !lse || (keys > 0 && (!k || !v))) return FM_BAD_ARGUMENT;
+  if (reinterpret_cast<uintptr_t>(out) & 15) return FM_UNSUPPORTED;
+  a.splits = row_splits(a);
+  if (a.splits > 1) {
+    if (!workspace || workspace_bytes < workspace_floats(a, a.splits) * sizeof(float)) return FM_WORKSPACE_TOO_SMALL;
+    if (reinterpret_cast<uintptr_t>(workspace) & 15) return FM_UNSUPPORTED;
+    a.part_o = workspace;
+    a.part_ml = workspace + (size_t)a.splits * sequences(a) * a.T * a.G * (a.D > 64 ? 128 : 64);
+  }
+  return FM_ATTENTION_TYPES(cross_forward);
+}
+
+size_t fm_cross_attention_backward_workspace_bytes(int batch, int queries, int keys, int heads, int kv_heads, int head_dim) {
+  const Attn a = cross_sizes(batch, queries, keys, heads, kv_heads, head_dim, 1.0f);
+  if (cross_check(a, DT_F32) != FM_OK && cross_check(a, DT_BF16) != FM_OK) return 0;
+  return batch == 0 || queries == 0 ? 0 : backward_floats(a) * sizeof(float);
+}
+
+int fm_cross_attention_backward(const void* dout, long dout_batch, long dout_row, long dout_head, const void* q, long q_batch,
+                                long q_row, long q_head, const void* k, long k_batch, long k_row, long k_head, const void* v,
+                                long v_batch, long v_row, long v_head, const void* out, const float* lse,
+                                const int* key_lengths, const int* query_lengths, int batch, int queries, int keys, int heads,
+                                int kv_heads, int head_dim, float scale, int dtype, void* dq, void* dk, void* dv, float* stats,
+                                float* workspace, size_t workspace_bytes, hipStream_t stream) {
+  Attn a = cross_sizes(batch, queries, keys, heads, kv_heads, head_dim, scale);
+  a.q = View{q, q_batch, q_row, q_head}, a.k = View{k, k_batch, k_row, k_head}, a.v = View{v, v_batch, v_row, v_head};
+  a.dout = View{dout, dout_batch, dout_row, dout_head};
+  a.o = out, a.lengths = key_lengths, a.query_lengths = query_lengths, a.lse = const_cast<float*>(lse);
+  a.out = dq, a.dk = dk, a.dv = dv, a.stats = stats;
+  if (const int status = cross_check(a, dtype)) return status;
+  if (batch == 0 || queries == 0) return batch == 0 || keys == 0 ? FM_OK : FM_BAD_ARGUMENT;
+  if (!dout || !q || !out || !lse || !dq || !stats || (keys > 0 && (!k || !v || !dk || !dv))) return FM_BAD_ARGUMENT;
+  for (const void* p : {out, (const void*)dq, (const void*)dk, (const void*)dv})
+    if (reinterpret_cast<uintptr_t>(p) & 15) return FM_UNSUPPORTED;
+  if (const size_t need = backward_floats(a) * sizeof(float)) {
+    if (!workspace || workspace_bytes < need) return FM_WORKSPACE_TOO_SMALL;
+    if (reinterpret_cast<uintptr_t>(workspace) & 15) return FM_UNSUPPORTED;
+  }
+  const auto run = [&](auto kernel) { return kernel(a, workspace, stream); };
+  const bool wide = a.D > 64;
+  if (dtype == DT_F32) return wide ? run(cross_backward<float, 128>) : run(cross_backward<float, 64>);
+  if (dtype == DT_BF16) return wide ? run(cross_backward<__bf16, 128>) : run(cross_backward<__bf16, 64>);
+  return wide ? run(cross_backward<_Float16, 128>) : run(cross_backward<_Float16, 64>);
+}
+
+}  // extern "C"

@@ -110,6 +110,10 @@ _SIGNATURES = {
     "fm_quantize_weight": ([_P, _I, _I, _I, _P, _P, _P], _I),
     "fm_linear_fp8_workspace_bytes": ([_L, _I, _I], _S),
     "fm_linear_fp8": ([_P, _P, _P, _P, _L, _I, _I, _I, _P, _P, _S, _P], _I),
+    "fm_cross_attention_forward_workspace_bytes": ([_I, _I, _I, _I, _I, _I], _S),
+    "fm_cross_attention_forward": ([_P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P, _S, _P], _I),
+    "fm_cross_attention_backward_workspace_bytes": ([_I, _I, _I, _I, _I, _I], _S),
+    "fm_cross_attention_backward": ([_P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P, _P, _P, _S, _P], _I),
     "fm_rotary": ([_P, _L, _L, _L, _I, _P, _L, _L, _L, _I, _P, _P, _L, _I, _L, _I, _I, _I, _I, _I, _F, _I, _I, _P, _P, _P], _I),
     "fm_code_embedding_backward": ([_P, _L, _P, _L, _L, _I, _I, _I, _I, _I, _F, _I, _P, _P, _S, _P], _I),
 }

@@ -69,6 +69,8 @@ SPECS = {
     "fm_quantize_rows": "in:x i:ld_x i:rows i:channels i:dtype out:y out:scales",
     "fm_quantize_weight": "in:weight i:out_features i:in_features i:dtype out:values out:scales",
     "fm_linear_fp8": "in:x in:x_scales in:weight in:weight_scales i:rows i:in_features i:out_features i:dtype out:y out:workspace i:workspace_bytes",
+    "fm_cross_attention_forward": "in:q i:q_batch i:q_row i:q_head in:k i:k_batch i:k_row i:k_head in:v i:v_batch i:v_row i:v_head in:key_lengths in:query_lengths i:batch i:queries i:keys i:heads i:kv_heads i:head_dim f:scale i:dtype out:out out:lse out:workspace i:workspace_bytes",
+    "fm_cross_attention_backward": "in:dout i:dout_batch i:dout_row i:dout_head in:q i:q_batch i:q_row i:q_head in:k i:k_batch i:k_row i:k_head in:v i:v_batch i:v_row i:v_head in:out in:lse in:key_lengths in:query_lengths i:batch i:queries i:keys i:heads i:kv_heads i:head_dim f:scale i:dtype out:dq out:dk out:dv out:stats out:workspace i:workspace_bytes",
     "fm_rotary": "in:q i:q_batch i:q_row i:q_head i:heads in:k i:k_batch i:k_row i:k_head i:kv_heads in:frequencies in:positions i:positions_batch i:positions_bytes i:first i:batch i:length i:head_dim i:rotated i:interleaved f:scale i:inverse i:dtype out:q_out out:k_out",
 }
 

@@ -39,6 +39,9 @@ __all__ = [
     "code_embedding",
     "code_embedding_backward",
     "code_embedding_forward",
+    "cross_attention",
+    "cross_attention_backward",
+    "cross_attention_forward",
     "layer_norm",
     "layer_norm_backward",
     "layer_norm_forward",
@@ -505,37 +508,46 @@ def rotary(q, k, frequencies, positions=None, interleaved: bool = False, scale: 
 
 
 # ---------------------------------------------------------------- attention
-def _attention_input(q, k, v, window, scale, lengths):
+def _attention_operands(q, k, v, scale):
     q = _tensor("q", q)
     k, v = _tensor("k", k, (q.dtype,)), _tensor("v", v, (q.dtype,))
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 4:
             raise ValueError(f"{name} must be [batch, positions, heads, head_dim], got shape {tuple(t.shape)}")
-    b, t, h, d = q.shape
+    b, _, h, d = q.shape
     s, kv = k.shape[1], k.shape[2]
     if k.shape != (b, s, kv, d) or v.shape != k.shape:
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
-    if t > s:
-        raise ValueError(f"{t} queries over {s} keys: the queries are the last positions of the keys")
     if h == 0 or kv == 0 or h % kv:
         raise ValueError(f"{h} query heads are not a multiple of {kv} key heads")
     unit = 4 if q.dtype == torch.float32 else 8
     if not 0 < d <= 128 or d % unit:
         raise ValueError(f"head_dim must be a multiple of {unit} up to 128 for {q.dtype}, got {d}")
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0 < scale < math.inf:
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    return q, k, v, scale
+
+
+def _lengths(name, lengths, b):
+    if lengths is None:
+        return None
+    lengths = _tensor(name, lengths, (torch.int32,))
+    if lengths.shape != (b,):
+        raise ValueError(f"{name} must have shape ({b},), got {tuple(lengths.shape)}")
+    return lengths.contiguous()
+
+
+def _attention_input(q, k, v, window, scale, lengths):
+    q, k, v, scale = _attention_operands(q, k, v, scale)
+    t, s = q.shape[1], k.shape[1]
+    if t > s:
+        raise ValueError(f"{t} queries over {s} keys: the queries are the last positions of the keys")
     if window is None:
         window = max(s, 1)
     if not isinstance(window, int) or isinstance(window, bool) or window <= 0:
         raise ValueError(f"window must be a positive integer or None, got {window!r}")
-    window = min(window, max(s, 1))
-    scale = d ** -0.5 if scale is None else float(scale)
-    if not 0 < scale < math.inf:
-        raise ValueError(f"scale must be positive and finite, got {scale}")
-    if lengths is not None:
-        lengths = _tensor("lengths", lengths, (torch.int32,))
-        if lengths.shape != (b,):
-            raise ValueError(f"lengths must have shape ({b},), got {tuple(lengths.shape)}")
-        lengths = lengths.contiguous()
-    return q, k, v, window, scale, lengths
+    return q, k, v, min(window, max(s, 1)), scale, _lengths("lengths", lengths, q.shape[0])
 
 
 def _heads(t: torch.Tensor, group: int = 1) -> tuple[torch.Tensor, int, int, int]:
@@ -632,6 +644,87 @@ def window_attention(q, k, v, window: int | None = None, scale: float | None = N
     if not _differentiable(q, k, v):
         return window_attention_forward(q, k, v, window, scale, lengths)[0]
     return _apply(_WindowAttention, (q, k, v), q, k, v, window, scale, lengths)
+
+
+# ---------------------------------------------------------- cross attention
+def _cross_input(q, k, v, scale, key_lengths, query_lengths):
+    q, k, v, scale = _attention_operands(q, k, v, scale)
+    b = q.shape[0]
+    return q, k, v, scale, _lengths("key_lengths", key_lengths, b), _lengths("query_lengths", query_lengths, b)
+
+
+def cross_attention_forward(q, k, v, scale: float | None = None, key_lengths=None, query_lengths=None):
+    """``(out, lse)`` of attention to another sequence: every query sees every key of its batch item.
+
+    ``q`` is ``[batch, queries, heads, head_dim]``, ``k`` and ``v`` are ``[batch, keys, kv_heads,
+    head_dim]`` (any strides; slices of a packed projection are read in place); neither length
+    bounds the other.  ``key_lengths`` and ``query_lengths`` (int32 ``[batch]``): what lies behind
+    them is padding; it is never read, and its rows of ``out`` are zeros, as are all of an item without
+    keys.  ``scale`` defaults to ``head_dim ** -0.5``.  ``lse`` (FP32 ``[batch, queries, heads]``,
+    base 2) is for :func:`cross_attention_backward`.
+
+    An infinity or NaN may reach other rows near it; what padding holds reaches nothing.  At
+    most 2097120 keys, and queries times heads per key head.
+    """
+    q, k, v, scale, key_lengths, query_lengths = _cross_input(q, k, v, scale, key_lengths, query_lengths)
+    device = _on_gpu(q=q, k=k, v=v, key_lengths=key_lengths, query_lengths=query_lengths)
+    b, t, h, d = q.shape
+    s, kv = k.shape[1], k.shape[2]
+    out = q.new_empty((b, t, h, d))
+    lse = q.new_empty((b, t, h), dtype=torch.float32)
+    if b and t:
+        ws, size = _scratch(q, "fm_cross_attention_forward_workspace_bytes", b, t, s, h, kv, d)
+        _run(device, "fm_cross_attention_forward", *_heads(q, h // kv), *_heads(k), *_heads(v), key_lengths, query_lengths, b, t, s,
+             h, kv, d, scale, _DTYPES[out.dtype], out, lse, ws, size)
+    return out, lse
+
+
+def cross_attention_backward(grad, q, k, v, out, lse, scale: float | None = None, key_lengths=None, query_lengths=None):
+    """``(dq, dk, dv)`` for the gradient ``grad`` of the output of :func:`cross_attention_forward`
+    (``out``, ``lse``: what it returned)."""
+    q, k, v, scale, key_lengths, query_lengths = _cross_input(q, k, v, scale, key_lengths, query_lengths)
+    grad, out, lse = _tensor("grad", grad, (q.dtype,)), _tensor("out", out, (q.dtype,)), _tensor("lse", lse, (torch.float32,))
+    b, t, h, d = q.shape
+    s, kv = k.shape[1], k.shape[2]
+    if grad.shape != q.shape:
+        raise ValueError(f"grad must have q's shape {tuple(q.shape)}, got {tuple(grad.shape)}")
+    if out.shape != q.shape or lse.shape != (b, t, h) or not lse.is_contiguous():
+        raise ValueError("out and lse must be what cross_attention_forward returned for q, k and v")
+    device = _on_gpu(q=q, k=k, v=v, grad=grad, out=out, lse=lse, key_lengths=key_lengths, query_lengths=query_lengths)
+    dq, dk, dv = q.new_empty((b, t, h, d)), q.new_empty((b, s, kv, d)), q.new_empty((b, s, kv, d))
+    if b and t == 0:
+        return dq, dk.zero_(), dv.zero_()
+    if b:
+        out = _heads(out.contiguous())[0]
+        stats = lse.new_empty((2, b, t, h))
+        ws, size = _scratch(q, "fm_cross_attention_backward_workspace_bytes", b, t, s, h, kv, d)
+        _run(device, "fm_cross_attention_backward", *_heads(grad, h // kv), *_heads(q, h // kv), *_heads(k), *_heads(v), out, lse,
+             key_lengths, query_lengths, b, t, s, h, kv, d, scale, _DTYPES[q.dtype], dq, dk, dv, stats, ws, size)
+    return dq, dk, dv
+
+
+class _CrossAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, scale, key_lengths, query_lengths):
+        out, lse = cross_attention_forward(q, k, v, scale, key_lengths, query_lengths)
+        ctx.save_for_backward(q, k, v, out, lse, key_lengths, query_lengths)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        q, k, v, out, lse, *lengths = ctx.saved_tensors
+        grads = cross_attention_backward(grad, q, k, v, out, lse, ctx.scale, *lengths)
+        return tuple(g if need else None for g, need in zip((*grads, None, None, None), ctx.needs_input_grad))
+
+
+def cross_attention(q, k, v, scale: float | None = None, key_lengths=None, query_lengths=None):
+    """Attention to another sequence, differentiable in ``q``, ``k`` and ``v`` (see
+    :func:`cross_attention_forward` for the layouts and the padding)."""
+    if not _differentiable(q, k, v):
+        return cross_attention_forward(q, k, v, scale, key_lengths, query_lengths)[0]
+    return _apply(_CrossAttention, (q, k, v), q, k, v, scale, key_lengths, query_lengths)
 
 
 # ------------------------------------------------------- codebook embedding

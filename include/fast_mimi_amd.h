@@ -699,6 +699,37 @@ int fm_rotary(const void* q, long q_batch, long q_row, long q_head, int heads, c
               int inverse, int dtype, void* q_out, void* k_out, hipStream_t stream);
 
 /*
+ * Attention to the states of another sequence: fm_attention_forward without its mask, each
+ * of the queries seeing keys 0 .. key_lengths[b] - 1 (int [batch]; NULL: all).  queries and
+ * keys do not bound each other.  Queries from query_lengths[b] on (NULL: none) are padding: like
+ * those of an item without keys they give zeros and an lse of -inf, and nothing behind
+ * either length is used.  Everything else, limits included, is as in fm_attention_forward.
+ * The workspace holds the parts of calls that are cut over their keys (forward, dq) or
+ * rows (dk, dv); NULL where its size is 0.  lse, out and stats as there.
+ * A conditioned model over the codes has this beside MimiAttention (model.py:1870-1961).
+ */
+size_t fm_cross_attention_forward_workspace_bytes(int batch, int queries, int keys, int heads,
+                                                  int kv_heads, int head_dim);
+int fm_cross_attention_forward(const void* q, long q_batch, long q_row, long q_head, const void* k,
+                               long k_batch, long k_row, long k_head, const void* v, long v_batch,
+                               long v_row, long v_head, const int* key_lengths,
+                               const int* query_lengths, int batch, int queries, int keys,
+                               int heads, int kv_heads, int head_dim, float scale, int dtype,
+                               void* out, float* lse, float* workspace, size_t workspace_bytes,
+                               hipStream_t stream);
+size_t fm_cross_attention_backward_workspace_bytes(int batch, int queries, int keys, int heads,
+                                                   int kv_heads, int head_dim);
+int fm_cross_attention_backward(const void* dout, long dout_batch, long dout_row, long dout_head,
+                                const void* q, long q_batch, long q_row, long q_head,
+                                const void* k, long k_batch, long k_row, long k_head,
+                                const void* v, long v_batch, long v_row, long v_head,
+                                const void* out, const float* lse, const int* key_lengths,
+                                const int* query_lengths, int batch, int queries, int keys,
+                                int heads, int kv_heads, int head_dim, float scale, int dtype,
+                                void* dq, void* dk, void* dv, float* stats, float* workspace,
+                                size_t workspace_bytes, hipStream_t stream);
+
+/*
  * 8 bits.  Values are e4m3 (no infinities, largest 448); each block of 128 of them along
  * a row of activations, or of 128 x 128 weights, shares a scale 2^(byte - 127) (e8m0,
  * the least that keeps the block's largest value at or below 448; 255, NaN, for a block

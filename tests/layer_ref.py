@@ -108,7 +108,10 @@ def cross(q, k, v, grad, scale, key_lengths, query_lengths, pieces=1):
             DS = P * (DP - D)
             edp = (d + 2) * H * (G.abs() @ V.abs().T)
             eD = (G.abs() * (du * O.abs() + eo + step0(t) + (d + 2) * H * O.abs())).sum(1, keepdim=True)
-            eds = ep * (DP - D).abs() + P * (edp + eD + 2 * H * (DP.abs() + D.abs())) + (up + 2 * H) * DS.abs() + eta
+            # A probability below 2^-126 is zero (eta): dS = P (dP - D) loses up to eta |dP - D| with it.  (Scores of
+            # 739 under a largest of 826 have P = 1.1e-38 and dP - D = 17.)  Its own rounding near zero is the other eta.
+            eds = ep * (DP - D).abs() + P * (edp + eD + 2 * H * (DP.abs() + D.abs())) + (up + 2 * H) * DS.abs() \
+                + eta * ((DP - D).abs() + 1)
             val["out"][i, :rows, a] = O
             err["out"][i, :rows, a] = eo + u * O.abs() + step0(t)
             val["dq"][i, :rows, a] = DS @ K * scale
