@@ -54,27 +54,27 @@ FM_DEVICE unsigned two(float a, float b) {
 }
 
 // ------------------------------------------------------------ many rows
-// A block forms BM rows of x by BN of w, waves of WM x WN.  128-deep tiles of both
-// travel global -> LDS (16 bytes a lane) in two stages, the next one on its way during
-// the products.  A row of a tile is 128 bytes, its 16-byte chunk c at chunk c ^ (row / 2 % 8): a fragment
-// read takes the same chunk of 16 rows, 256 bytes over all banks.  The weights are the A operand, so that
-// a lane ends with runs of four outputs of one row.
+// A block forms BM rows of x by BN of w, four waves of WM x WN.  128-deep tiles of both
+// travel global -> LDS (16 bytes a lane) in two stages, and from there, half a tile at a
+// time, into one of two sets of registers: while the products of one half run, the other
+// half's (or the next tile's) operands are read.  A tile's second half is in registers before
+// its one barrier, so behind it the next but one tile takes its place, and the products go
+// on at once; its loads go out one by one between them (16 in a row hold the wave up: 8192^3
+// 442 us, so 412).
 //
-// Of a 64-deep product lane l holds chunks l / 32 and l / 32 + 2: which values of k does not
-// matter as long as both operands hold the same.
-template <typename T, int BM, int BN, int WM, int WN>
-struct Tile {
-  static constexpr int WAVES = (BM / WM) * (BN / WN), STAGE = (BM + BN) * 128;
-};
-
-template <typename T, int BM, int BN, int WM, int WN, int BLOCKS>
-__global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), BLOCKS) void linear_tile_kernel(Linear a) {
-  constexpr int WAVES = (BM / WM) * (BN / WN), MT = WM / 32, NT = WN / 32, STAGE = (BM + BN) * 128;
-  constexpr int LOADS = (BM + BN) / 8 / WAVES;  // instructions of 8 rows each, a wave
-  static_assert((BM / 8) % LOADS == 0, "a wave loads rows of one operand");
+// A row of a tile is 128 bytes, its 16-byte chunk c at chunk c ^ (row / 2 % 8): a fragment read takes
+// the same chunk of 16 rows, 256 bytes over all banks.  Of a 64-deep half lane l holds chunks
+// l / 32 and l / 32 + 2 of its row: which values of k does not matter as long as both operands
+// hold the same.  The weights are the A operand, so that a lane ends with runs of four outputs of one row.
+template <typename T, int BM, int BN, int BLOCKS>
+__global__ __launch_bounds__(256, BLOCKS) void linear_tile_kernel(Linear a) {
+  constexpr int WM = BM / 2, WN = BN / 2, MT = WM / 32, NT = WN / 32, STAGE = (BM + BN) * 128;
+  constexpr int LOADS = (BM + BN) / 32, P = MT * NT, F = MT + NT;  // a wave's loads of 8 rows, products and operands
+  static_assert(LOADS % 2 == 0 && 128 % WN == 0, "pairs of loads; a wave's rows of w share their scales");
   __shared__ __attribute__((aligned(1024))) unsigned char lds[2 * STAGE];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, half = lane >> 5;
-  const int wm = wave % (BM / WM), wn = wave / (BM / WM);
+  // The wave's number as a scalar: its loads' bases are, too.
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5, r = lane & 31;
+  const int wm = wave & 1, wn = wave >> 1;
 
   // Blocks of one XCD (block % 8) take neighbouring tiles: eight tiles of rows by as
   // many of columns as follow, so that both operands come from its L2 several times.
@@ -84,37 +84,29 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), BLOCKS) void linear_til
   const int band = 8 * a.tiles_n, first = at / band * 8, rows = min(8, a.tiles_m - first), in = at % band;
   const int m0 = (first + in % rows) * BM, n0 = in / rows * BN;
 
+  // This block's part of K, in blocks of 128 values.
   const int split = blockIdx.y, per_split = (a.KB + a.splits - 1) / a.splits;
-  const int b_lo = split * per_split, b_hi = min(a.KB, b_lo + per_split);
+  const int b_lo = min(a.KB, split * per_split), b_hi = min(a.KB, b_lo + per_split);
 
-  // This wave's loads: rows of x, or of w.
-  const bool of_w = wave * LOADS * 8 >= BM;
-  const int limit = of_w ? a.N - n0 : a.M - m0;
-  const __amdgpu_buffer_rsrc_t buf = fm_buffer(of_w ? a.w + (long)n0 * a.K : a.x + (long)m0 * a.K, INT_MAX);
+  // This wave's loads: rows of x (the first two waves, where the tile is square), or of w.
+  const __amdgpu_buffer_rsrc_t buf_x = fm_buffer(a.x + (long)m0 * a.K, INT_MAX), buf_w = fm_buffer(a.w + (long)n0 * a.K, INT_MAX);
   int offset[LOADS];
 #pragma unroll
   for (int u = 0; u < LOADS; ++u) {
-    const int r = (wave * LOADS + u) * 8 + lane / 8, row = of_w ? r - BM : r;
-    offset[u] = row < limit ? row * a.K + (((lane & 7) ^ ((r >> 1) & 7)) << 4) : INT_MIN;
+    const int i = wave * LOADS + u, row = 8 * i + lane / 8, own = row - (8 * i < BM ? 0 : BM);
+    offset[u] = own < (8 * i < BM ? a.M - m0 : a.N - n0) ? own * a.K + (((lane & 7) ^ ((row >> 1) & 7)) << 4) : INT_MIN;
   }
-  const int chunk[2] = {((lane & 7) ^ ((lane >> 4) & 3)) << 4, ((lane & 7) ^ (((lane >> 4) & 3) + 4)) << 4};
-  auto load = [&](int b, int stage) {
-    const int left = a.K - b * 128;  // a chunk past the end reads zeros
-#pragma unroll
-    for (int u = 0; u < LOADS; ++u) {
-      const int i = wave * LOADS + u;
-      fm_buf_load_lds16(buf, lds + stage * STAGE + i * 1024, chunk[i & 1] < left ? offset[u] : INT_MIN, b * 128);
-    }
+  const int chunk[2] = {((lane & 7) ^ (lane >> 4)) << 4, ((lane & 7) ^ ((lane >> 4) + 4)) << 4};  // of even and odd loads
+  auto load = [&](int b, int stage, int u) {
+    const int i = wave * LOADS + u, left = b < b_hi ? a.K - b * 128 : 0;  // a chunk past the end reads zeros
+    fm_buf_load_lds16(8 * i < BM ? buf_x : buf_w, lds + stage * STAGE + i * 1024, chunk[u & 1] < left ? offset[u] : INT_MIN, b * 128);
   };
 
-  // Scales: a lane's own row of each tile of x, one byte for all of the wave's rows of w
-  // (or 32 of them, where a block's are not whole 128s).
-  const unsigned char* sx[MT];
+  // Scales: of a lane's own row of each 32 of x, and one byte for all of the wave's rows of w.
+  const unsigned char *sx[MT], *sw = a.sw + (long)(min(n0 + wn * WN, a.N - 1) / 128) * a.KB;
 #pragma unroll
-  for (int i = 0; i < MT; ++i) sx[i] = a.sx + (long)min(m0 + wm * WM + 32 * i + (lane & 31), a.M - 1) * a.KB;
-  const unsigned char* sw = a.sw + (long)(min(n0 + wn * WN, a.N - 1) / 128) * a.KB;
-  static_assert(WN <= 128 && 128 % WN == 0 && BN % WN == 0, "a wave's rows of w share their scales");
-  int next_x[MT], next_w = 0;
+  for (int i = 0; i < MT; ++i) sx[i] = a.sx + (long)min(m0 + wm * WM + 32 * i + r, a.M - 1) * a.KB;
+  int next_x[MT], next_w;
   auto scales = [&](int b) {
 #pragma unroll
     for (int i = 0; i < MT; ++i) next_x[i] = sx[i][b];
@@ -122,47 +114,76 @@ __global__ __launch_bounds__(64 * (BM / WM) * (BN / WN), BLOCKS) void linear_til
   };
 
   const unsigned base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
-  const int r = lane & 31;
   const unsigned lane_at = base + r * 128 + ((half ^ ((r >> 1) & 7)) << 4);
-  auto fragment = [&](unsigned at, int s) {
-    const auto p = [&](int u) { return *(const __attribute__((address_space(3))) intx4*)(at ^ (64 * s + 32 * u)); };
-    return join(p(0), p(1));
+  struct Operands {
+    intx8 f[F];  // of x, of w
+  } first_half, second_half;
+  auto fetch = [&](Operands& o, int stage, int s, int p) {
+    typedef const __attribute__((address_space(3))) intx4 Chunk;
+    const unsigned from = lane_at + stage * STAGE + (p < MT ? wm * WM + 32 * p : BM + wn * WN + 32 * (p - MT)) * 128;
+    o.f[p] = join(*(Chunk*)(from ^ (64 * s)), *(Chunk*)(from ^ (64 * s + 32)));
   };
 
   floatx16 acc[NT][MT] = {};
-  if (b_lo < b_hi) load(b_lo, 0), scales(b_lo);
-  for (int b = b_lo; b < b_hi; ++b) {
+  int x_scale[MT], w_scale;
+  // All products of a half, with something between one and the next.
+  auto products = [&](const Operands& o, auto between) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            acc[j][i] = fm_mfma32_bf16(to_bf16(o.f[MT + j], c, scale_of(w_scale)), to_bf16(o.f[i], c, scale_of(x_scale[i])), acc[j][i]);
+        } else {
+          acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(o.f[MT + j], o.f[i], acc[j][i], 0, 0, 0, w_scale, 0, x_scale[i]);
+        }
+        between(j * MT + i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  };
+  // Operands go between the products one each, a little behind them, or all that are due.
+  auto due = [](int p, auto fetch_one) {
+#pragma unroll
+    for (int u = P >= F + 2 ? p - 2 : p * F / P; u < (P >= F + 2 ? p - 1 : (p + 1) * F / P); ++u)
+      if (u >= 0 && u < F) fetch_one(u);
+  };
+  auto barrier = [&]() {
+    __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    int x_scale[MT], w_scale = next_w;
+    __builtin_amdgcn_sched_barrier(0);
+  };
+
+  if (b_lo < b_hi) {
+    scales(b_lo);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) x_scale[i] = next_x[i];
-    const int stage = (b - b_lo) & 1;
-    if (b + 1 < b_hi) load(b + 1, stage ^ 1), scales(b + 1);
-    const unsigned x_at = lane_at + stage * STAGE + wm * WM * 128, w_at = lane_at + stage * STAGE + (BM + wn * WN) * 128;
+    for (int u = 0; u < LOADS; ++u) load(b_lo, 0, u);
+    barrier();
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      intx8 xf[MT];
+    for (int u = 0; u < LOADS; ++u) load(b_lo + 1, 1, u);
 #pragma unroll
-      for (int i = 0; i < MT; ++i) xf[i] = fragment(x_at + i * 4096, s);
+    for (int p = 0; p < F; ++p) fetch(first_half, 0, 0, p);
+    for (int b = b_lo; b < b_hi; ++b) {
+      const int stage = (b - b_lo) & 1;
+      w_scale = next_w;
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const intx8 wf = fragment(w_at + j * 4096, s);
-        if constexpr (sizeof(T) == 4) {
+      for (int i = 0; i < MT; ++i) x_scale[i] = next_x[i];
+      products(first_half, [&](int p) { due(p, [&](int u) { fetch(second_half, stage, 1, u); }); });
+      barrier();
+      // Ahead of the tile's loads: waiting for one behind them would be waiting for all.
+      scales(min(b + 1, b_hi - 1));
+      __builtin_amdgcn_sched_barrier(0);
+      products(second_half, [&](int p) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const bf16x8 f = to_bf16(wf, c, scale_of(w_scale));
-#pragma unroll
-            for (int i = 0; i < MT; ++i) acc[j][i] = fm_mfma32_bf16(f, to_bf16(xf[i], c, scale_of(x_scale[i])), acc[j][i]);
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-            acc[j][i] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wf, xf[i], acc[j][i], 0, 0, 0, w_scale, 0, x_scale[i]);
-        }
-      }
+        for (int u = p * LOADS / P; u < (p + 1) * LOADS / P; ++u) load(b + 2, stage, u);
+        due(p, [&](int u) { fetch(first_half, stage ^ 1, 0, u); });
+      });
     }
+    // The copies of the two tiles past the end (zeros) must not outlive the block's LDS.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
 
   // Lane l: row l % 32 of x, rows 8 g + 4 (l / 32) .. + 3 of w.
@@ -233,48 +254,79 @@ __global__ __launch_bounds__(256) void linear_join_kernel(Linear a) {
 }
 
 // ------------------------------------------------------------- few rows
-// Up to 16 MT rows of x by 16 of w a block, whose waves take every WAVES-th 128-deep block
-// of K, operands straight from memory (each weight is read once in all), and add their
-// sums through LDS in order.
-template <typename T, int MT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(Linear a) {
-  __shared__ float sums[WAVES][MT][4][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, quarter = lane >> 4;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
-  const unsigned char* w = a.w + (long)min(n0 + r, a.N - 1) * a.K;
-  const unsigned char* sw = a.sw + (long)(n0 / 128) * a.KB;
-  const unsigned char *x[MT], *sx[MT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    const long m = min(m0 + 16 * i + r, a.M - 1);
-    x[i] = a.x + m * a.K, sx[i] = a.sx + m * a.KB;
+// The bytes of up to four scales from `from` on, of `left` that the row still has; zeros
+// (2^-127, of zero values) behind them.  Nothing past the scales' `total` bytes is read.
+FM_DEVICE unsigned four_scales(const unsigned char* scales, long total, long from, int left) {
+  if (left <= 0) return 0;
+  unsigned v = 0;
+  if (total >= 4) {
+    const long there = min(from, total - 4);
+    __builtin_memcpy(&v, scales + there, 4);
+    v >>= 8 * (int)(from - there);
+  } else {
+    for (int i = 0; i < 3; ++i)
+      if (from + i < total) v |= (unsigned)scales[from + i] << (8 * i);
   }
+  return left >= 4 ? v : v & ((1u << (8 * left)) - 1);
+}
+
+// Up to 16 MT rows of x by 16 of w a block, operands straight from memory: each weight is
+// read once in all.  The waves take four blocks of 128 values each in turn, with
+// all of their loads on the way at once, and add their sums through LDS in order.
+template <typename T, int MT>
+__global__ __launch_bounds__(512) void linear_rows_kernel(Linear a) {
+  constexpr int WAVES = 8, U = 4;  // blocks of a wave
+  __shared__ float sums[WAVES][MT][4][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, quarter = lane >> 4;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MT;
+  const __amdgpu_buffer_rsrc_t buf_w = fm_buffer(a.w + (long)n0 * a.K, INT_MAX), buf_x = fm_buffer(a.x + (long)m0 * a.K, INT_MAX);
   // Lane l holds chunks l / 16 and l / 16 + 4 of a block.
-  auto two_chunks = [&](const unsigned char* row, int b) {
-    intx4 p{}, q{};
-    const int k = b * 128 + quarter * 16;
-    if (k < a.K) p = *reinterpret_cast<const intx4*>(row + k);
-    if (k + 64 < a.K) q = *reinterpret_cast<const intx4*>(row + k + 64);
-    return join(p, q);
-  };
+  const int at_w = n0 + r < a.N ? r * a.K + quarter * 16 : INT_MIN;
+  int at_x[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) at_x[i] = m0 + 16 * i + r < a.M ? (16 * i + r) * a.K + quarter * 16 : INT_MIN;
+  const long sw = (long)(n0 / 128) * a.KB, sw_total = (long)((a.N + 127) / 128) * a.KB, sx_total = (long)a.M * a.KB;
   floatx4 acc[MT] = {};
-#pragma unroll 4
-  for (int b = wave; b < a.KB; b += WAVES) {
-    const intx8 wf = two_chunks(w, b);
-    const int w_scale = sw[b];
+  for (int b0 = 4 * wave; b0 < a.KB; b0 += 4 * WAVES) {
+    intx4 wf[U][2], xf[U][MT][2];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const intx8 xf = two_chunks(x[i], b);
-      const int x_scale = sx[i][b];
-      if constexpr (sizeof(T) == 4) {
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16(wf, c, scale_of(w_scale)), to_bf16(xf, c, scale_of(x_scale)),
-                                                           acc[i], 0, 0, 0);
-      } else {
-        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf, xf, acc[i], 0, 0, 0, w_scale, 0, x_scale);
+      for (int h = 0; h < 2; ++h) {
+        const int k = (b0 + u) * 128 + 64 * h;
+        const bool there = quarter * 16 < a.K - k;
+        auto get = [&](__amdgpu_buffer_rsrc_t buf, int at) {
+          return __builtin_bit_cast(intx4, __builtin_amdgcn_raw_buffer_load_b128(buf, there ? at : INT_MIN, k, 0));
+        };
+        wf[u][h] = get(buf_w, at_w);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) xf[u][i][h] = get(buf_x, at_x[i]);
       }
-    }
+    // Behind the operands, so that those do not wait for them.
+    __builtin_amdgcn_sched_barrier(0);
+    const unsigned w_scale = four_scales(a.sw, sw_total, sw + b0, a.KB - b0);
+    unsigned x_scale[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+      x_scale[i] = four_scales(a.sx, sx_total, (long)min(m0 + 16 * i + r, a.M - 1) * a.KB + b0, a.KB - b0);
+    auto product = [&](auto which) {
+      constexpr int B = decltype(which)::value;
+      const intx8 w8 = join(wf[B][0], wf[B][1]);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const intx8 x8 = join(xf[B][i][0], xf[B][i][1]);
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16(w8, c, scale_of(w_scale >> (8 * B) & 255)),
+                                                             to_bf16(x8, c, scale_of(x_scale[i] >> (8 * B) & 255)), acc[i], 0, 0, 0);
+        } else {
+          acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, x8, acc[i], 0, 0, B, w_scale, B, x_scale[i]);
+        }
+      }
+    };
+    product(std::integral_constant<int, 0>{}), product(std::integral_constant<int, 1>{});
+    product(std::integral_constant<int, 2>{}), product(std::integral_constant<int, 3>{});
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i)
@@ -291,34 +343,47 @@ __global__ __launch_bounds__(64 * WAVES) void linear_rows_kernel(Linear a) {
   }
 }
 
-constexpr int FEW = 64;  // rows that the few-row kernel takes
-
+// How a call runs.  Rows a block (0: the few-row kernel), columns a block, parts of K.
+//
+// Few rows up to 16, and up to 32 where the weights are 2 MB or less and latency is all
+// (us, few rows / 64 x 64 tiles: 1 x 4096 to 6144 8.1 / 9.9, 16 x 8192 to 2048 10.5 / 11.4, 32 x
+// 1008 to 1000 3.9 / 4.8, 32 x 4096 to 6144 14 / 11.9).
+//
+// 256 x 256 tiles, one block to a CU, where their last round of 256 is nearly full: they
+// read the least per product (4096^3 60 us; 128 x 128 83, 64 x 128 96, 64 x 64 116).  Else
+// 128 x 128 (two to a CU) from 400 tiles on (1001 x 2048 to 8192 23.6; 64 x 128 28.1), 64
+// x 128 from 300 on (500 x 4096 to 6144 24.1; 128 x 128 26.6, 64 x 64 27.7), else 64 x 64
+// (256 x 2048 to 8192 11.6; 64 x 128 12.9), whose K is split, up to 512 blocks of eight or more of its
+// 128s: the parts go through memory (256 x 8192 to 2048, in 2 / 4 / 8: 19.8 / 17.2 / 21; 300 x
+// 1040 to 200, in 1 / 2: 5.1 / 6.4).  None was more than 8% behind the best of 20-40 tried at 20 sizes.
 struct LinearPlan {
   int bm, bn, splits;
 };
 LinearPlan linear_plan(long M, int N, int K) {
-  if (M <= FEW) return {0, 0, 1};
-  if (fm_ceil_div(M, 256) * fm_ceil_div(N, 256) >= 224) return {256, 256, 1};
-  const long tiles = (long)fm_ceil_div(M, 128) * fm_ceil_div(N, 128);
-  const int blocks = fm_ceil_div(K, 128);
-  int splits = 1;
-  while (tiles * splits * 2 <= 512 && blocks / (splits * 2) >= 4) splits *= 2;
-  return {128, 128, splits};
+  if (M <= 16 || (M <= 32 && (long)N * K <= 1 << 21)) return {0, 0, 1};
+  auto tiles = [&](int bm, int bn) { return (long)fm_ceil_div(M, bm) * fm_ceil_div(N, bn); };
+  const long large = tiles(256, 256);
+  if (4 * large >= 3 * ((large + 255) / 256 * 256)) return {256, 256, 1};
+  if (tiles(128, 128) >= 400) return {128, 128, 1};
+  if (tiles(64, 128) >= 300) return {64, 128, 1};
+  const long small = tiles(64, 64);
+  return {64, 64, (int)std::max<long>(1, std::min<long>({512 / small, fm_ceil_div(K, 128) / 8, 8}))};
 }
 
 template <typename T>
 int run(Linear a, const LinearPlan& p, hipStream_t stream) {
   if (p.bm == 0) {
     const dim3 grid(fm_ceil_div(a.N, 16));
-    if (a.M <= 16) hipLaunchKernelGGL((linear_rows_kernel<T, 1, 8>), grid, dim3(512), 0, stream, a);
-    else if (a.M <= 32) hipLaunchKernelGGL((linear_rows_kernel<T, 2, 8>), grid, dim3(512), 0, stream, a);
-    else hipLaunchKernelGGL((linear_rows_kernel<T, 4, 8>), grid, dim3(512), 0, stream, a);
+    if (a.M <= 16) hipLaunchKernelGGL((linear_rows_kernel<T, 1>), grid, dim3(512), 0, stream, a);
+    else hipLaunchKernelGGL((linear_rows_kernel<T, 2>), grid, dim3(512), 0, stream, a);
     return (int)hipGetLastError();
   }
   a.splits = p.splits, a.tiles_m = fm_ceil_div(a.M, p.bm), a.tiles_n = fm_ceil_div(a.N, p.bn);
   const dim3 grid(fm_ceil_div((long)a.tiles_m * a.tiles_n, 8) * 8, p.splits);
-  if (p.bm == 256) hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, 64, 128, 1>), grid, dim3(512), 0, stream, a);
-  else hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 64, 64, 2>), grid, dim3(256), 0, stream, a);
+  if (p.bm == 256) hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, 1>), grid, dim3(256), 0, stream, a);
+  else if (p.bm == 128) hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 2>), grid, dim3(256), 0, stream, a);
+  else if (p.bn == 128) hipLaunchKernelGGL((linear_tile_kernel<T, 64, 128, 3>), grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL((linear_tile_kernel<T, 64, 64, 4>), grid, dim3(256), 0, stream, a);
   if (p.splits > 1)
     hipLaunchKernelGGL(linear_join_kernel<T>, dim3(fm_ceil_div((long)a.M * a.N, 1024)), dim3(256), 0, stream, a);
   return (int)hipGetLastError();
@@ -338,7 +403,9 @@ int fm_linear_fp8(const void* x, const void* x_scales, const void* weight, const
                   int in_features, int out_features, int dtype, void* y, float* workspace, size_t workspace_bytes,
                   hipStream_t stream) {
   if (rows < 0 || in_features <= 0 || out_features <= 0 || dtype < DT_F32 || dtype > DT_F16) return FM_BAD_ARGUMENT;
-  if (in_features % 16 || in_features > 1 << 22 || rows > 1 << 24 || out_features > 1 << 24) return FM_UNSUPPORTED;
+  // A tile's rows within 32-bit offsets, tiles and joined outputs within a grid.
+  if (in_features % 16 || in_features > 1 << 22 || rows > 1 << 24 || out_features > 1 << 24 || rows * out_features > 1l << 40)
+    return FM_UNSUPPORTED;
   if (rows == 0) return FM_OK;
   if (!x || !x_scales || !weight || !weight_scales || !y) return FM_BAD_ARGUMENT;
   if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(weight) | reinterpret_cast<uintptr_t>(y)) & 15)
