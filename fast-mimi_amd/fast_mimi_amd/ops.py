@@ -125,6 +125,11 @@ def op(entry: str):
     return getattr(torch.ops.fast_mimi_amd, entry[3:])
 
 
+# Looked up once: a call asks all of them.
+_dispatch_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
+_tracing, _functorch_level = torch._C._get_tracing_state, torch._C._functorch.peek_interpreter_stack
+_profiling = torch._C._autograd._profiler_enabled
+
 _POINTERS = {entry: tuple(i for i, item in enumerate(spec.split()) if item[:3] in ("in:", "out", "res"))
              for entry, spec in SPECS.items()}
 
@@ -136,11 +141,8 @@ def _observed() -> bool:
     trace observer without the profiler cannot be asked for: it does not see
     direct calls.)"""
     # torch.compile first: it folds this to a constant and could not trace the rest.
-    return bool(torch.compiler.is_compiling()
-                or torch._C._len_torch_dispatch_stack() or torch._C._len_torch_function_stack()
-                or torch._C._get_tracing_state() is not None
-                or torch._C._functorch.peek_interpreter_stack() is not None
-                or torch._C._autograd._profiler_enabled())
+    return bool(torch.compiler.is_compiling() or _dispatch_modes() or _function_modes() or _tracing() is not None
+                or _functorch_level() is not None or _profiling())
 
 
 def call(entry: str, *args) -> None:

@@ -21,7 +21,7 @@ from __future__ import annotations
 
 import torch
 
-from .training import _DTYPES, _branch, _differentiable, _norm_weights, _on_gpu, _rows, _run, _scratch, _tensor
+from .training import _DTYPES, _branch, _differentiable, _on_gpu, _rows, _run, _scratch, _tensor
 
 __all__ = ["BLOCK", "linear", "quantize", "quantize_weight", "rms_norm"]
 
@@ -79,18 +79,19 @@ def rms_norm(x, weight=None, residual=None, eps: float = 1e-5):
     """``(values, scales, h)``: the ``y`` of :func:`fast_mimi_amd.training.rms_norm_forward` as
     :func:`quantize` gives it, rounded once, from FP32, and its ``h``."""
     _no_gradient(x, weight, residual)
-    x, residual = _branch(x, residual, eps)
-    weight, _, wtype = _norm_weights(x, weight, None)
-    device = _on_gpu(x=x, residual=residual, weight=weight)
-    c = x.shape[-1]
-    values = x.new_empty(x.shape, dtype=_VALUES)
-    scales = x.new_empty((*x.shape[:-1], _blocks(c)), dtype=_SCALES)
-    h = x if residual is None else residual.new_empty(x.shape)
+    x, weight, residual, device = _branch(x, weight, residual, eps)
+    shape, c, dtype = x.shape, x.shape[-1], _DTYPES[x.dtype]
+    values = x.new_empty(shape, dtype=_VALUES)
+    scales = x.new_empty((*shape[:-1], _blocks(c)), dtype=_SCALES)
+    rows, pitch = _rows(x)
+    rows_r, pitch_r, h, stream, out = None, 0, x, dtype, None
+    if residual is not None:
+        rows_r, pitch_r = _rows(residual)
+        h = out = residual.new_empty(shape)
+        stream = _DTYPES[h.dtype]
     if x.numel():
-        rows_x, pitch = _rows(x)
-        rows_r, pitch_r = (None, 0) if residual is None else _rows(residual)
-        _run(device, "fm_rms_norm_quantized", rows_x, pitch, rows_r, pitch_r, weight, x.numel() // c, c, float(eps),
-             _DTYPES[x.dtype], _DTYPES[h.dtype], _DTYPES[wtype], values, scales, None if residual is None else h)
+        _run(device, "fm_rms_norm_quantized", rows, pitch, rows_r, pitch_r, weight, x.numel() // c, c, float(eps), dtype, stream,
+             dtype if weight is None else _DTYPES[weight.dtype], values, scales, out)
     return values, scales, h
 
 
@@ -120,10 +121,9 @@ def linear(x, x_scale, weight, weight_scale, dtype: torch.dtype = torch.bfloat16
     rows = x.numel() // k
     y = x.new_empty((*x.shape[:-1], n), dtype=dtype)
     if rows:
-        x, weight = _aligned(x), _aligned(weight)
         ws, size = _scratch(y, "fm_linear_fp8_workspace_bytes", rows, k, n)
-        _run(device, "fm_linear_fp8", x, x_scale.contiguous(), weight, weight_scale.contiguous(), rows, k, n, _DTYPES[dtype], y,
-             ws, size)
+        _run(device, "fm_linear_fp8", _aligned(x), x_scale.contiguous(), _aligned(weight), weight_scale.contiguous(), rows, k, n,
+             _DTYPES[dtype], y, ws, size)
     return y
 
 

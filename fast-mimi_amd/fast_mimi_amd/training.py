@@ -59,6 +59,8 @@ __all__ = [
 
 _DEFAULT_STREAM = "fast_mimi_amd.default_stream"
 _DTYPES = {torch.float32: nat.DTYPE_F32, torch.bfloat16: nat.DTYPE_BF16, torch.float16: nat.DTYPE_F16}
+# What may stand beside a type: itself, or FP32.
+_WIDER = {torch.float32: (torch.float32,), torch.bfloat16: (torch.bfloat16, torch.float32), torch.float16: (torch.float16, torch.float32)}
 
 
 # ------------------------------------------------------------------- checks
@@ -99,7 +101,7 @@ def _on_gpu(**tensors) -> torch.device:
 
 def _run(device: torch.device, entry: str, *args) -> None:
     """The entry point, with its tensors' device as the current one."""
-    if device.index == torch.cuda.current_device():
+    if device.index == torch._C._cuda_getDevice():
         ops.call(entry, *args)
     else:
         with torch.cuda.device(device):
@@ -260,18 +262,27 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
 
 
 # ----------------------------------------------------------------- RMS norm
-def _branch(x, residual, eps):
-    """A branch and its residual stream, checked."""
+def _branch(x, weight, residual, eps):
+    """A branch, the norm's weight and the residual stream, checked; the device."""
     x = _tensor("x", x)
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"x must have a last dimension to normalise, got shape {tuple(x.shape)}")
     if residual is not None:
-        residual = _tensor("residual", residual, (x.dtype,) if x.dtype == torch.float32 else (x.dtype, torch.float32))
+        residual = _tensor("residual", residual, _WIDER[x.dtype])
         if residual.shape != x.shape:
             raise ValueError(f"residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    return x, residual
+    return x, _norm_weight(weight, x), residual, _on_gpu(x=x, residual=residual, weight=weight)
+
+
+def _norm_weight(weight, x):
+    if weight is None:
+        return None
+    weight = _tensor("weight", weight, _WIDER[x.dtype])
+    if weight.shape != x.shape[-1:]:
+        raise ValueError(f"weight must have shape {tuple(x.shape[-1:])}, got {tuple(weight.shape)}")
+    return weight.contiguous()
 
 
 def rms_norm_forward(x, weight=None, residual=None, eps: float = 1e-5):
@@ -282,18 +293,19 @@ def rms_norm_forward(x, weight=None, residual=None, eps: float = 1e-5):
     Without a residual ``h`` is ``x`` itself.  ``weight`` (optional) has ``x``'s type or
     FP32; ``rstd`` is FP32, one per row, for :func:`rms_norm_backward`.
     """
-    x, residual = _branch(x, residual, eps)
-    weight, _, wtype = _norm_weights(x, weight, None)
-    device = _on_gpu(x=x, residual=residual, weight=weight)
-    rows_x, pitch = _rows(x)
-    rows_r, pitch_r = (None, 0) if residual is None else _rows(residual)
-    y = x.new_empty(x.shape)
-    h = x if residual is None else residual.new_empty(x.shape)
-    rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
-    rows = rstd.numel()
-    if rows:
-        _run(device, "fm_rms_norm_forward", rows_x, pitch, rows_r, pitch_r, weight, rows, x.shape[-1], float(eps), _DTYPES[x.dtype],
-             _DTYPES[h.dtype], _DTYPES[wtype], y, None if residual is None else h, rstd)
+    x, weight, residual, device = _branch(x, weight, residual, eps)
+    shape, dtype = x.shape, _DTYPES[x.dtype]
+    y = x.new_empty(shape)
+    rstd = x.new_empty(shape[:-1], dtype=torch.float32)
+    rows, pitch = _rows(x)
+    rows_r, pitch_r, h, stream, out = None, 0, x, dtype, None
+    if residual is not None:
+        rows_r, pitch_r = _rows(residual)
+        h = out = residual.new_empty(shape)
+        stream = _DTYPES[h.dtype]
+    if rstd.numel():
+        _run(device, "fm_rms_norm_forward", rows, pitch, rows_r, pitch_r, weight, rstd.numel(), shape[-1], float(eps), dtype, stream,
+             dtype if weight is None else _DTYPES[weight.dtype], y, out, rstd)
     return y, h, rstd
 
 
@@ -307,7 +319,7 @@ def rms_norm_backward(grad, x, rstd, weight=None, residual=None, grad_h=None):
     the same tensor.  ``dweight`` is ``None`` without a weight.
     """
     grad = _tensor("grad", grad)
-    wide = (grad.dtype,) if grad.dtype == torch.float32 else (grad.dtype, torch.float32)
+    wide = _WIDER[grad.dtype]
     x = _tensor("x", x, wide if residual is None else (grad.dtype,))
     residual = None if residual is None else _tensor("residual", residual, wide)
     rstd = _tensor("rstd", rstd, (torch.float32,))
@@ -317,7 +329,7 @@ def rms_norm_backward(grad, x, rstd, weight=None, residual=None, grad_h=None):
         raise ValueError(f"residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
     if rstd.shape != x.shape[:-1] or not rstd.is_contiguous():
         raise ValueError("rstd must be what rms_norm_forward returned for x")
-    weight, _, wtype = _norm_weights(grad, weight, None)
+    weight = _norm_weight(weight, grad)
     stream = x.dtype if residual is None else residual.dtype
     if grad_h is not None:
         grad_h = _tensor("grad_h", grad_h, (stream,))
@@ -334,8 +346,9 @@ def rms_norm_backward(grad, x, rstd, weight=None, residual=None, grad_h=None):
     grad_h, ld_dh = (None, 0) if grad_h is None else _rows(grad_h)
     # The sum alone stands in the stream's place.
     parts = (x, ld_x, residual, ld_r) if residual is not None or x.dtype == grad.dtype else (None, 0, x, ld_x)
-    _run(device, "fm_rms_norm_backward", grad, ld_dy, *parts, weight, rstd, grad_h, ld_dh, rows, c, _DTYPES[grad.dtype],
-         _DTYPES[stream], _DTYPES[wtype], None if dx is dresidual else dx, dresidual, dw, ws, size)
+    dtype = _DTYPES[grad.dtype]
+    _run(device, "fm_rms_norm_backward", grad, ld_dy, *parts, weight, rstd, grad_h, ld_dh, rows, c, dtype, _DTYPES[stream],
+         dtype if weight is None else _DTYPES[weight.dtype], None if dx is dresidual else dx, dresidual, dw, ws, size)
     return dx, dresidual, dw
 
 
