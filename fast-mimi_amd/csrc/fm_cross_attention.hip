@@ -59,9 +59,16 @@ __global__ __launch_bounds__(256) void cross_join_kernel(Attn a) {
     if (64 * u + lane < a.D) out[64 * u + lane] = (T)sum[u];
 }
 
-// Into how many parts a walk of `tiles` is cut that `blocks` blocks make: until some 512
-// blocks run, at least four tiles each.
-int cut(long blocks, int tiles) { return (int)std::max<long>(1, std::min<long>({tiles / 4, 512 / std::max<long>(blocks, 1), 64})); }
+// Into how many parts a walk of `tiles` (of 128) is cut that `blocks` blocks make: until some 512
+// blocks run, at least two tiles each (backward, in 1 / 6 / 16 parts: 2 x 3000 queries over 20 keys, 8
+// heads of 64, FP32: 143 / 48 / 40 us; 4000 over 64, bfloat16, in 1 / 8 / 16: 59 / 23 / 21).
+int cut(long blocks, int tiles) { return (int)std::max<long>(1, std::min<long>({tiles / 2, 512 / std::max<long>(blocks, 1), 64})); }
+
+// A block's waves with rows (or keys) of their own, as own_waves has it for their number, but that
+// the waves which share them have two tiles of 32 each at least to walk (own_waves' / four of
+// their own: forward 2 x 3000 over 20 keys, FP32: 17.5 / 13.1 us, 13 over 7: 8.9 / 7.5; 16 x 200 over 100, 8 / 2
+// heads of 128, bfloat16, backward: 41 / 38; dK / dV of 3000 keys from 2 x 20 rows, 8 heads: 26.5 / 22.9 in all).
+int waves_apart(const Attn& a, long own, long walked) { return std::max(own_waves(a, own), walked < 128 ? 4 : walked < 256 ? 2 : 1); }
 
 long sequences(const Attn& a) { return (long)a.B * a.KV; }
 int row_splits(const Attn& a) {  // forward, dQ
@@ -89,7 +96,7 @@ size_t backward_floats(const Attn& a) {
 template <typename T, int DT>
 int cross_forward(Attn a, hipStream_t stream) {
   const long rows = (long)a.T * a.G;
-  const int waves = a.splits > 1 ? 1 : own_waves(a, rows);
+  const int waves = a.splits > 1 ? 1 : waves_apart(a, rows, a.S);
   FM_CROSS_LAUNCH(attention_forward_kernel, waves, rows, a.splits);
   if (a.splits > 1)
     hipLaunchKernelGGL((attention_join_kernel<T, DT, true>), dim3(fm_ceil_div(sequences(a) * rows, 4)), dim3(256), 0, stream, a);
@@ -103,7 +110,7 @@ int cross_backward(Attn a, float* workspace, hipStream_t stream) {
   if (rows > 0) {
     a.splits = row_splits(a);
     a.part_ml = workspace + (size_t)a.splits * sequences(a) * rows * DT;
-    const int waves = a.splits > 1 ? 1 : own_waves(a, rows);
+    const int waves = a.splits > 1 ? 1 : waves_apart(a, rows, a.S);
     FM_CROSS_LAUNCH(attention_dq_kernel, waves, rows, a.splits);
     if (a.splits > 1)
       hipLaunchKernelGGL((cross_join_kernel<T, DT, false>), dim3(fm_ceil_div(sequences(a) * rows, 4)), dim3(256), 0, stream, a);
@@ -116,7 +123,7 @@ int cross_backward(Attn a, float* workspace, hipStream_t stream) {
         hipLaunchKernelGGL((attention_dkv_kernel<T, DT, 2, 2, true>), grid, dim3(256), 0, stream, a);
       else hipLaunchKernelGGL((attention_dkv_kernel<T, DT, 2, 4, true>), grid, dim3(512), 0, stream, a);
     } else {
-      const int waves = a.splits > 1 ? 1 : own_waves(a, a.S);
+      const int waves = a.splits > 1 ? 1 : waves_apart(a, a.S, rows);
       FM_CROSS_LAUNCH(attention_dkv_kernel, waves, a.S, a.splits);
     }
     if (a.splits > 1)

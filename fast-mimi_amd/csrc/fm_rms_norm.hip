@@ -17,6 +17,11 @@
 
 namespace {
 
+// Elements of a lane's vector: 16 bytes of the stream, so that the stores of neighbouring
+// lanes lie side by side.
+template <typename S>
+constexpr int VEC = 16 / (int)sizeof(S);
+
 // E consecutive elements at any address.
 template <typename T, int E>
 using AnyVec = typename Vec<T, E>::type __attribute__((aligned(sizeof(T))));
@@ -26,7 +31,7 @@ struct Rms {
   void *y, *sum, *scales, *dx, *dres, *dw;
   float *rstd, *part;  // part: [blocks][C]
   long rows, ld_x, ld_res, ld_dy, ld_dh;
-  int C, blocks;
+  int C, blocks, wide;  // wide: FP32 weights
   float eps;
 };
 
@@ -44,16 +49,46 @@ FM_DEVICE typename Vec<T, E>::type row_load(const T* row, int i, int C) {
   }
   return t;
 }
-template <typename T, int E>
+// PAST: past the L2.
+template <typename T, int E, bool PAST = false>
 FM_DEVICE void row_store(T* row, int i, int C, typename Vec<T, E>::type t) {
   T* at = row + i * E;
   if ((i + 1) * E <= C) {
-    *reinterpret_cast<AnyVec<T, E>*>(at) = t;
+    auto to = reinterpret_cast<AnyVec<T, E>*>(at);
+    if constexpr (PAST) __builtin_nontemporal_store(t, to);
+    else *to = t;
   } else {
 #pragma unroll
     for (int e = 0; e < E - 1; ++e)
       if (i * E + e < C) at[e] = t[e];
   }
+}
+
+// Vector i of the weights, of T or FP32; ones without any.
+template <typename T, int E>
+FM_DEVICE void weight_load(const Rms& a, int i, float (&w)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) w[e] = 1.0f;
+  if (!a.w) return;
+  if (sizeof(T) == 4 || a.wide) {
+    const typename Vec<float, E>::type t = row_load<float, E>(static_cast<const float*>(a.w), i, a.C);
+#pragma unroll
+    for (int e = 0; e < E; ++e) w[e] = t[e];
+  } else {
+    const typename Vec<T, E>::type t = row_load<T, E>(static_cast<const T*>(a.w), i, a.C);
+#pragma unroll
+    for (int e = 0; e < E; ++e) w[e] = widen(t[e]);
+  }
+}
+template <typename T>
+FM_DEVICE float one_weight(const Rms& a, int c) {
+  if (!a.w) return 1.0f;
+  return sizeof(T) == 4 || a.wide ? static_cast<const float*>(a.w)[c] : widen(static_cast<const T*>(a.w)[c]);
+}
+template <typename T>
+FM_DEVICE void store_weight_gradient(const Rms& a, long c, float v) {
+  if (sizeof(T) == 4 || a.wide) static_cast<float*>(a.dw)[c] = v;
+  else static_cast<T*>(a.dw)[c] = (T)v;
 }
 
 // The scale byte of 128 values whose largest magnitude is `most`: 255 (NaN) for an
@@ -94,17 +129,16 @@ FM_DEVICE void store_8_bits(const float (&v)[E], unsigned char* row, unsigned ch
 }
 
 // Lane p of a row holds vectors p, p + LPR, ... (NV of them, E elements each).
-template <typename T, typename S, typename W, int NV, int LPR, bool BITS8>
+template <typename T, typename S, int NV, int LPR, bool BITS8, bool PAST>
 __global__ __launch_bounds__(256) void rms_forward_kernel(Rms a) {
-  constexpr int E = 16 / (int)sizeof(T);
+  constexpr int E = VEC<S>;
   __shared__ float waves[4];
   const int p = threadIdx.x % LPR;
   const long row = (long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
   if (row >= a.rows) return;
   const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
   const S* res = a.res ? static_cast<const S*>(a.res) + row * a.ld_res : nullptr;
-  float v[NV][E];
-  typename Vec<W, E>::type wv[NV];
+  float v[NV][E], w[NV][E];
   float s = 0.0f;
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
@@ -116,9 +150,8 @@ __global__ __launch_bounds__(256) void rms_forward_kernel(Rms a) {
     for (int e = 0; e < E; ++e) v[u][e] = widen(t[e]) + widen(r[e]);
   }
   // The weights are on their way during the sum.
-  const W* w = static_cast<const W*>(a.w);
 #pragma unroll
-  for (int u = 0; u < NV; ++u) wv[u] = w ? row_load<W, E>(w, p + u * LPR, a.C) : typename Vec<W, E>::type{};
+  for (int u = 0; u < NV; ++u) weight_load<T, E>(a, p + u * LPR, w[u]);
 #pragma unroll
   for (int u = 0; u < NV; ++u)
 #pragma unroll
@@ -130,7 +163,7 @@ __global__ __launch_bounds__(256) void rms_forward_kernel(Rms a) {
       typename Vec<S, E>::type t;
 #pragma unroll
       for (int e = 0; e < E; ++e) t[e] = (S)v[u][e];
-      row_store<S, E>(h, p + u * LPR, a.C, t);
+      row_store<S, E, PAST>(h, p + u * LPR, a.C, t);
     }
   }
   const float rstd = 1.0f / sqrtf(row_sum<LPR>(s, waves) / (float)a.C + a.eps);
@@ -140,7 +173,7 @@ __global__ __launch_bounds__(256) void rms_forward_kernel(Rms a) {
     const int i = p + u * LPR;
     float y[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) y[e] = v[u][e] * rstd * (w ? widen(wv[u][e]) : 1.0f);
+    for (int e = 0; e < E; ++e) y[e] = v[u][e] * rstd * w[u][e];
     if constexpr (BITS8) {
       const int blocks = (a.C + 127) / 128;
       store_8_bits<E, (128 / E < LPR ? 128 / E : LPR)>(y, static_cast<unsigned char*>(a.y) + row * a.C,
@@ -149,29 +182,43 @@ __global__ __launch_bounds__(256) void rms_forward_kernel(Rms a) {
       typename Vec<T, E>::type t;
 #pragma unroll
       for (int e = 0; e < E; ++e) t[e] = (T)y[e];
-      row_store<T, E>(static_cast<T*>(a.y) + row * a.C, i, a.C, t);
+      row_store<T, E, PAST>(static_cast<T*>(a.y) + row * a.C, i, a.C, t);
     }
   }
+}
+
+// The sum over a row's lanes; with more than 64, its waves, through `waves` (of its own
+// for each sum between two barriers).
+template <int LPR>
+FM_DEVICE float lanes_sum(float v, float* waves) {
+  v = row_sum<(LPR < 64 ? LPR : 64)>(v);
+  if constexpr (LPR > 64) {
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.0f;
+#pragma unroll
+    for (int u = 0; u < LPR / 64; ++u) v += waves[u];
+  }
+  return v;
 }
 
 // dh, and this block's share of dw: a row group walks rows blockIdx * groups + g,
 // + gridDim * groups, ... with the columns' sums in registers; the block joins its
 // groups through LDS in order and writes one partial row (or, when it is the only
 // block, the gradient itself).
-template <typename T, typename S, typename W, int NV, int LPR>
-__global__ __launch_bounds__(256) void rms_backward_kernel(Rms a) {
-  constexpr int E = 16 / (int)sizeof(T), GROUPS = 256 / LPR;
+template <typename T, typename S, int NV, int LPR, bool PAST>
+__global__ __launch_bounds__(LPR < 256 ? 256 : LPR) void rms_backward_kernel(Rms a) {
+  constexpr int E = VEC<S>, GROUPS = LPR < 256 ? 256 / LPR : 1;
   typedef typename Vec<T, E>::type VT;
   typedef typename Vec<S, E>::type VS;
-  __shared__ float joined[256 * E], waves[2][4];
+  __shared__ float joined[GROUPS > 1 ? 256 * E : 1], waves[2][LPR > 64 ? LPR / 64 : 1];
   const int p = threadIdx.x % LPR, g = threadIdx.x / LPR;
   float wv[NV][E], dw[NV][E];
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
-    typename Vec<W, E>::type t{};
-    if (a.w) t = row_load<W, E>(static_cast<const W*>(a.w), p + u * LPR, a.C);
+    weight_load<T, E>(a, p + u * LPR, wv[u]);
 #pragma unroll
-    for (int e = 0; e < E; ++e) wv[u][e] = a.w ? widen(t[e]) : 1.0f, dw[u][e] = 0.0f;
+    for (int e = 0; e < E; ++e) dw[u][e] = 0.0f;
   }
   const float inv = 1.0f / (float)a.C;
   VT xv[NV], xn[NV], gv[NV], gn[NV];
@@ -209,7 +256,7 @@ __global__ __launch_bounds__(256) void rms_backward_kernel(Rms a) {
         s = fmaf(d * wv[u][e], hh, s);
         dw[u][e] = fmaf(d, hh, dw[u][e]);
       }
-    s = row_sum<LPR>(s, waves[turn]) * inv, turn ^= 1;
+    s = lanes_sum<LPR>(s, waves[turn]) * inv, turn ^= 1;
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
       VS t;
@@ -220,40 +267,44 @@ __global__ __launch_bounds__(256) void rms_backward_kernel(Rms a) {
         const float dh = fmaf(rstd, fmaf(widen(gv[u][e]), wv[u][e], -hh * s), widen(sv[u][e]));
         t[e] = (S)dh, b[e] = (T)dh;
       }
-      row_store<S, E>(static_cast<S*>(a.dres) + row * a.C, p + u * LPR, a.C, t);
+      row_store<S, E, PAST>(static_cast<S*>(a.dres) + row * a.C, p + u * LPR, a.C, t);
       if constexpr (!std::is_same<T, S>::value)
-        if (a.dx) row_store<T, E>(static_cast<T*>(a.dx) + row * a.C, p + u * LPR, a.C, b);
+        if (a.dx) row_store<T, E, PAST>(static_cast<T*>(a.dx) + row * a.C, p + u * LPR, a.C, b);
     }
   }
   if (!a.dw) return;
 #pragma unroll
   for (int u = 0; u < NV; ++u) {
-    __syncthreads();
+    if constexpr (GROUPS > 1) {
+      __syncthreads();
 #pragma unroll
-    for (int e = 0; e < E; ++e) joined[e * 256 + threadIdx.x] = dw[u][e];
-    __syncthreads();
-    if (g != 0) continue;
+      for (int e = 0; e < E; ++e) joined[e * 256 + threadIdx.x] = dw[u][e];
+      __syncthreads();
+      if (g != 0) continue;
+    }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int c = (p + u * LPR) * E + e;
       if (c >= a.C) continue;
-      float s = 0.0f;
-      for (int j = 0; j < GROUPS; ++j) s += joined[e * 256 + j * LPR + p];
+      float s = dw[u][e];
+      if constexpr (GROUPS > 1) {
+        s = 0.0f;
+        for (int j = 0; j < GROUPS; ++j) s += joined[e * 256 + j * LPR + p];
+      }
       if (a.blocks > 1) a.part[(long)blockIdx.x * a.C + c] = s;
-      else static_cast<W*>(a.dw)[c] = (W)s;
+      else store_weight_gradient<T>(a, c, s);
     }
   }
 }
 
 // Any number of channels: one block per row (forward) or per run of rows
 // (backward), the row read again for each step.
-template <typename T, typename S, typename W, bool BITS8>
+template <typename T, typename S, bool BITS8>
 __global__ __launch_bounds__(256) void rms_forward_any_kernel(Rms a) {
   __shared__ float waves[4];
   const long row = blockIdx.x;
   const T* x = static_cast<const T*>(a.x) + row * a.ld_x;
   const S* res = a.res ? static_cast<const S*>(a.res) + row * a.ld_res : nullptr;
-  const W* w = static_cast<const W*>(a.w);
   auto h = [&](int c) { return widen(x[c]) + (res ? widen(res[c]) : 0.0f); };
   float s = 0.0f;
   for (int c = threadIdx.x; c < a.C; c += 256) {
@@ -272,21 +323,20 @@ __global__ __launch_bounds__(256) void rms_forward_any_kernel(Rms a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int c = 4 * i + e;
-        y[e] = c < a.C ? h(c) * rstd * (w ? widen(w[c]) : 1.0f) : 0.0f;
+        y[e] = c < a.C ? h(c) * rstd * one_weight<T>(a, c) : 0.0f;
       }
       store_8_bits<4, 32>(y, static_cast<unsigned char*>(a.y) + row * a.C, static_cast<unsigned char*>(a.scales) + row * blocks,
                           i, a.C);
     }
   } else {
     for (int c = threadIdx.x; c < a.C; c += 256)
-      static_cast<T*>(a.y)[row * a.C + c] = (T)(h(c) * rstd * (w ? widen(w[c]) : 1.0f));
+      static_cast<T*>(a.y)[row * a.C + c] = (T)(h(c) * rstd * one_weight<T>(a, c));
   }
 }
 
-template <typename T, typename S, typename W>
+template <typename T, typename S>
 __global__ __launch_bounds__(256) void rms_backward_any_kernel(Rms a) {
   __shared__ float waves[2][4];
-  const W* w = static_cast<const W*>(a.w);
   float* part = a.part + (long)blockIdx.x * a.C;
   bool first = true;
   int turn = 0;
@@ -300,13 +350,13 @@ __global__ __launch_bounds__(256) void rms_backward_any_kernel(Rms a) {
     float s = 0.0f;
     for (int c = threadIdx.x; c < a.C; c += 256) {
       const float hh = h(c) * rstd, d = widen(dy[c]);
-      s = fmaf(d * (w ? widen(w[c]) : 1.0f), hh, s);
+      s = fmaf(d * one_weight<T>(a, c), hh, s);
       if (a.dw) part[c] = first ? d * hh : fmaf(d, hh, part[c]);
     }
     s = row_sum<256>(s, waves[turn]) / (float)a.C;
     for (int c = threadIdx.x; c < a.C; c += 256) {
       const float hh = h(c) * rstd;
-      const float v = fmaf(rstd, fmaf(widen(dy[c]), w ? widen(w[c]) : 1.0f, -hh * s), dh ? widen(dh[c]) : 0.0f);
+      const float v = fmaf(rstd, fmaf(widen(dy[c]), one_weight<T>(a, c), -hh * s), dh ? widen(dh[c]) : 0.0f);
       static_cast<S*>(a.dres)[row * a.C + c] = (S)v;
       if constexpr (!std::is_same<T, S>::value)
         if (a.dx) static_cast<T*>(a.dx)[row * a.C + c] = (T)v;
@@ -316,7 +366,7 @@ __global__ __launch_bounds__(256) void rms_backward_any_kernel(Rms a) {
 
 // dw from the blocks' partial rows: 32 columns a block, 32 threads to a column, each
 // summing every 32nd row in order, then joined in order.
-template <typename W>
+template <typename T>
 __global__ __launch_bounds__(1024) void rms_join_kernel(Rms a) {
   __shared__ float sums[32][33];
   const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
@@ -333,14 +383,14 @@ __global__ __launch_bounds__(1024) void rms_join_kernel(Rms a) {
   float total = 0.0f;
 #pragma unroll
   for (int j = 0; j < 32; ++j) total += sums[j][c];
-  static_cast<W*>(a.dw)[col] = (W)total;
+  store_weight_gradient<T>(a, col, total);
 }
 
 // No rows: a zero gradient.
-template <typename W>
+template <typename T>
 __global__ __launch_bounds__(256) void rms_zero_kernel(Rms a) {
   const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c < a.C) static_cast<W*>(a.dw)[c] = (W)0.0f;
+  if (c < a.C) store_weight_gradient<T>(a, c, 0.0f);
 }
 
 // Rows as they are, in 8 bits: a lane a vector.  A row has whole 128-channel blocks of
@@ -395,6 +445,9 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(const T* w, int N,
 
 constexpr int MOST_CHANNELS = 1 << 26;
 constexpr long MOST_ROWS = 1 << 23;  // of a launch: a grid has at most 2^32 threads
+// Bytes of the stream from which on results go past the L2, whose eight parts hold 32 MB (bfloat16, through / past:
+// forward 40000 x 2048 93 / 70 us, 16000 x 2048 31 / 30, 40000 x 4096 with an FP32 stream 335 / 326).
+constexpr long PAST_FROM = 32l << 20;
 
 int rms_check(const Rms& a, int dtype, int stype, int wtype) {
   if (a.rows < 0 || a.C <= 0 || dtype < DT_F32 || dtype > DT_F16 || (stype != dtype && stype != DT_F32) ||
@@ -405,45 +458,63 @@ int rms_check(const Rms& a, int dtype, int stype, int wtype) {
   return FM_OK;
 }
 
-// The lanes and vectors of a row: the rule of plan(), rows being whole vectors here.
-Plan rms_plan(int C, int size) {
-  const int e = 16 / size;
-  return plan((C + e - 1) / e * e, size, true);
-}
-
 enum Pass { FORWARD, BITS8, BACKWARD };
 
-template <typename T, typename S, typename W, int NV, int LPR, Pass PASS>
+// The lanes and vectors of a row: the rule of plan(), rows being whole vectors here, but for
+// forward rows that leave a block a vector each or half that (us, 2048 bfloat16 channels in 8 bits, a
+// wave / a block a row: 13 rows 4.5 / 3.4, 1001 5.3 / 4.8, 4000 12.1 / 12.2, 16000 36 / 35; 1024, half
+// of the lanes idle: 16000 19 / 25).
+Plan forward_plan(int C, int e) {
+  const int n = (C + e - 1) / e;
+  return n > 128 && n <= 256 ? Plan{e, 1, 256} : plan(n * e, 16 / e, true);
+}
+// The backward pass holds three or four tensors' vectors twice (a row and the next), so at most
+// two of each a lane: four leave one wave to a SIMD (4000 x 2048 bfloat16, four in a wave / one in a
+// block a row: 29 / 19 us; 40000 x 4096 with an FP32 stream, four / two / one in 256 / 512 / 1024
+// lanes: 506 / 520 / 475).
+Plan backward_plan(int C, int e) {
+  const int n = (C + e - 1) / e;
+  if (n <= 16) return {e, 1, 16};
+  if (n <= 128) return {e, n <= 64 ? 1 : 2, 64};
+  if (n <= 512) return {e, n <= 256 ? 1 : 2, 256};
+  if (n <= 1024) return {e, 1, 1024};
+  return n <= 2048 && e == 4 ? Plan{e, 2, 1024} : Plan{e, 0, 64};
+}
+
+template <typename T, typename S, int NV, int LPR, Pass PASS, bool PAST>
 void launch(const Rms& a, hipStream_t stream) {
   if constexpr (PASS == BACKWARD)
-    hipLaunchKernelGGL((rms_backward_kernel<T, S, W, NV, LPR>), dim3(a.blocks), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((rms_backward_kernel<T, S, NV, LPR, PAST>), dim3(a.blocks), dim3(std::max(256, LPR)), 0, stream, a);
   else
-    hipLaunchKernelGGL((rms_forward_kernel<T, S, W, NV, LPR, PASS == BITS8>), dim3(fm_ceil_div(a.rows, 256 / LPR)), dim3(256),
+    hipLaunchKernelGGL((rms_forward_kernel<T, S, NV, LPR, PASS == BITS8, PAST>), dim3(fm_ceil_div(a.rows, 256 / LPR)), dim3(256),
                        0, stream, a);
 }
 
-// False where the plan has no kernel (none of plan()'s).
-template <typename T, typename S, typename W, Pass PASS>
+// False where the plan has no kernel (none of those above).
+template <typename T, typename S, Pass PASS, bool PAST>
 bool launch_plan(const Rms& a, const Plan& p, hipStream_t stream) {
-  if (p.lpr == 16) return launch<T, S, W, 1, 16, PASS>(a, stream), true;
-  if (p.lpr == 64) {
-    if (p.nv == 1) return launch<T, S, W, 1, 64, PASS>(a, stream), true;
-    if (p.nv == 2) return launch<T, S, W, 2, 64, PASS>(a, stream), true;
-    if (p.nv == 4) return launch<T, S, W, 4, 64, PASS>(a, stream), true;
+  if (p.lpr == 16) return launch<T, S, 1, 16, PASS, PAST>(a, stream), true;
+  if (p.lpr == 64 && p.nv == 1) return launch<T, S, 1, 64, PASS, PAST>(a, stream), true;
+  if (p.lpr == 64 && p.nv == 2) return launch<T, S, 2, 64, PASS, PAST>(a, stream), true;
+  if (p.lpr == 256 && p.nv == 1) return launch<T, S, 1, 256, PASS, PAST>(a, stream), true;
+  if (p.lpr == 256 && p.nv == 2) return launch<T, S, 2, 256, PASS, PAST>(a, stream), true;
+  if constexpr (PASS == BACKWARD) {
+    if (p.lpr == 1024 && p.nv == 1) return launch<T, S, 1, 1024, PASS, PAST>(a, stream), true;
+    if constexpr (sizeof(S) == 4)
+      if (p.lpr == 1024) return launch<T, S, 2, 1024, PASS, PAST>(a, stream), true;
   } else {
-    if (p.nv == 2) return launch<T, S, W, 2, 256, PASS>(a, stream), true;
-    if (p.nv == 4) return launch<T, S, W, 4, 256, PASS>(a, stream), true;
-    if constexpr (sizeof(T) == 4)
-      if (p.nv == 8) return launch<T, S, W, 8, 256, PASS>(a, stream), true;
+    if (p.nv == 4) return launch<T, S, 4, 256, PASS, PAST>(a, stream), true;
+    if constexpr (sizeof(S) == 4)
+      if (p.nv == 8) return launch<T, S, 8, 256, PASS, PAST>(a, stream), true;
   }
   return false;
 }
 
-template <typename T, typename S, typename W, Pass PASS>
+template <typename T, typename S, Pass PASS>
 int run(Rms a, hipStream_t stream) {
-  const Plan p = rms_plan(a.C, sizeof(T));
+  const Plan p = PASS == BACKWARD ? backward_plan(a.C, VEC<S>) : forward_plan(a.C, VEC<S>);
   if (PASS == BACKWARD && a.rows == 0) {
-    hipLaunchKernelGGL((rms_zero_kernel<W>), dim3(fm_ceil_div(a.C, 256)), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL((rms_zero_kernel<T>), dim3(fm_ceil_div(a.C, 256)), dim3(256), 0, stream, a);
     return (int)hipGetLastError();
   }
   if (PASS != BACKWARD && a.rows > MOST_ROWS) {
@@ -456,36 +527,32 @@ int run(Rms a, hipStream_t stream) {
       part.y = static_cast<char*>(a.y) + first * a.C * (PASS == BITS8 ? 1 : sizeof(T));
       if (a.scales) part.scales = static_cast<char*>(a.scales) + first * ((a.C + 127) / 128);
       if (a.rstd) part.rstd = a.rstd + first;
-      if (const int status = run<T, S, W, PASS>(part, stream)) return status;
+      if (const int status = run<T, S, PASS>(part, stream)) return status;
     }
     return FM_OK;
   }
   a.blocks = PASS == BACKWARD ? backward_blocks(a.rows, p, sizeof(T)) : 0;
   if (p.nv == 0) {
     if constexpr (PASS == BACKWARD)
-      hipLaunchKernelGGL((rms_backward_any_kernel<T, S, W>), dim3(a.blocks), dim3(256), 0, stream, a);
+      hipLaunchKernelGGL((rms_backward_any_kernel<T, S>), dim3(a.blocks), dim3(256), 0, stream, a);
     else
-      hipLaunchKernelGGL((rms_forward_any_kernel<T, S, W, PASS == BITS8>), dim3((unsigned)a.rows), dim3(256), 0, stream, a);
-  } else if (!launch_plan<T, S, W, PASS>(a, p, stream)) {
-    return FM_UNSUPPORTED;
+      hipLaunchKernelGGL((rms_forward_any_kernel<T, S, PASS == BITS8>), dim3((unsigned)a.rows), dim3(256), 0, stream, a);
+  } else if (PASS != BITS8 && a.rows * a.C * (long)sizeof(S) >= PAST_FROM) {
+    if (!launch_plan<T, S, PASS, PASS != BITS8>(a, p, stream)) return FM_UNSUPPORTED;
+  } else {
+    if (!launch_plan<T, S, PASS, false>(a, p, stream)) return FM_UNSUPPORTED;
   }
   if (PASS == BACKWARD && a.dw && (a.blocks > 1 || p.nv == 0))
-    hipLaunchKernelGGL((rms_join_kernel<W>), dim3(fm_ceil_div(a.C, 32)), dim3(1024), 0, stream, a);
+    hipLaunchKernelGGL((rms_join_kernel<T>), dim3(fm_ceil_div(a.C, 32)), dim3(1024), 0, stream, a);
   return (int)hipGetLastError();
 }
 
-template <typename T, Pass PASS>
-int run_types(const Rms& a, bool wide_stream, bool wide_weight, hipStream_t stream) {
-  if constexpr (std::is_same<T, float>::value) return run<float, float, float, PASS>(a, stream);
-  else if (wide_stream) return wide_weight ? run<T, float, float, PASS>(a, stream) : run<T, float, T, PASS>(a, stream);
-  else return wide_weight ? run<T, T, float, PASS>(a, stream) : run<T, T, T, PASS>(a, stream);
-}
-
 template <Pass PASS>
-int dispatch(const Rms& a, int dtype, int stype, int wtype, hipStream_t stream) {
-  const bool s = stype == DT_F32, w = wtype == DT_F32;
-  if (dtype == DT_F32) return run_types<float, PASS>(a, s, w, stream);
-  return dtype == DT_BF16 ? run_types<__bf16, PASS>(a, s, w, stream) : run_types<_Float16, PASS>(a, s, w, stream);
+int dispatch(Rms a, int dtype, int stype, int wtype, hipStream_t stream) {
+  a.wide = wtype == DT_F32;
+  if (dtype == DT_F32) return run<float, float, PASS>(a, stream);
+  if (stype == DT_F32) return dtype == DT_BF16 ? run<__bf16, float, PASS>(a, stream) : run<_Float16, float, PASS>(a, stream);
+  return dtype == DT_BF16 ? run<__bf16, __bf16, PASS>(a, stream) : run<_Float16, _Float16, PASS>(a, stream);
 }
 
 template <typename T>

@@ -25,10 +25,10 @@ struct Rotary {
   Part q, k;  // k.heads may be 0
   const double* frequencies;
   const void* positions;  // [batch or 1][length] of 4 or 8 bytes, or NULL: first + 0, 1, ...
-  long positions_batch, first;
-  int wide, B, T, D, half, units, per_block, group;
+  long positions_batch, first, start;  // start: of this launch's positions
+  int wide, B, T, D, half, turns, units, per_block, group, groups;  // units of a position: the first `turns` turn pairs
   float scale, sign;
-  FmDivisor by_units, by_length;
+  FmDivisor by_units, by_length, by_groups;
 };
 
 template <typename T, int E>
@@ -43,9 +43,11 @@ template <typename T, int E>
 FM_DEVICE typename Vec<T, E>::type any_load(const T* at) {
   return *reinterpret_cast<const typename AnyVec<T, E>::type*>(at);
 }
-template <typename T, int E>
+template <bool PAST, typename T, int E>
 FM_DEVICE void any_store(T* at, typename Vec<T, E>::type v) {
-  *reinterpret_cast<typename AnyVec<T, E>::type*>(at) = v;
+  auto to = reinterpret_cast<typename AnyVec<T, E>::type*>(at);
+  if constexpr (PAST && E > 1) __builtin_nontemporal_store(v, to);
+  else *to = v;
 }
 
 // Sine and cosine of position * frequency.  1 / (2 pi) is the sum of two doubles; with
@@ -76,14 +78,27 @@ FM_DEVICE void turn(double position, double frequency, float& sine, float& cosin
   cosine = (q + 1) & 2 ? -cosine : cosine;
 }
 
-template <typename T, int E, bool INTERLEAVED>
+// A unit is a thread's two vectors within a head, neighbouring threads' side by side in
+// memory.  Pairs apart: one vector of the first partners and one of the second, or two that
+// are copied.  Pairs side by side (whole pairs in a vector): two vectors half a head
+// apart, each turned or copied.  PAST: results go past the L2.
+template <typename T, int E, bool INTERLEAVED, bool PAST>
 __global__ __launch_bounds__(256) void rotary_kernel(Rotary a) {
+  constexpr bool WITHIN = INTERLEAVED && E > 1;
   const int local = (int)fm_div(threadIdx.x, a.by_units), unit = threadIdx.x - local * a.units;
-  const long n = (long)blockIdx.x * a.per_block + local;
+  // Neighbouring blocks take the heads of the same positions: whole rows are read at a time.
+  const int block = (int)fm_div(blockIdx.x, a.by_groups), h0 = (blockIdx.x - block * a.groups) * a.group;
+  const long n = a.start + (long)block * a.per_block + local;
   if (local >= a.per_block || n >= (long)a.B * a.T) return;
   const int b = (int)fm_div((unsigned)n, a.by_length), t = (int)(n - (long)b * a.T);
-  const int pair = unit * E;
-  const bool turns = pair < a.half;
+  const bool turns = WITHIN || unit < a.turns;
+  int first = unit * E, second = first + a.units * E;
+  if constexpr (!WITHIN) {
+    if (!turns) first = 2 * a.half + (unit - a.turns) * E, second = first + (a.units - a.turns) * E;
+    else if (INTERLEAVED) first = 2 * unit, second = first + 1;
+    else second = a.half + first;
+  }
+  const bool both = second < a.D;
   float sine[E], cosine[E];
   if (turns) {
     double position = (double)(a.first + t);
@@ -93,16 +108,12 @@ __global__ __launch_bounds__(256) void rotary_kernel(Rotary a) {
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      turn(position, a.frequencies[pair + e], sine[e], cosine[e]);
-      sine[e] *= a.sign, cosine[e] *= a.scale;
+      const int pair = !WITHIN ? unit * E + e : 2 * e < E ? first / 2 + e : second / 2 + e - E / 2;
+      if (WITHIN && pair >= a.half) sine[e] = 0.0f, cosine[e] = 1.0f;  // copied, below
+      else turn(position, a.frequencies[pair], sine[e], cosine[e]), sine[e] *= a.sign, cosine[e] *= a.scale;
     }
   }
-  // The unit's two vectors within a head; of the copied channels the last may have one.
-  const int rest = 2 * a.half + 2 * (pair - a.half);
-  const int first = turns ? (INTERLEAVED ? 2 * pair : pair) : rest;
-  const int second = turns && !INTERLEAVED ? a.half + pair : first + E;
-  const bool both = second < a.D;
-  const int heads = a.q.heads + a.k.heads, h0 = blockIdx.y * a.group;
+  const int heads = a.q.heads + a.k.heads;
   for (int h = h0; h < min(h0 + a.group, heads); ++h) {
     const bool key = h >= a.q.heads;
     const Part& p = key ? a.k : a.q;
@@ -112,51 +123,63 @@ __global__ __launch_bounds__(256) void rotary_kernel(Rotary a) {
     typename Vec<T, E>::type u = any_load<T, E>(x + first), v{}, ou = u, ov;
     if (both) v = any_load<T, E>(x + second);
     ov = v;
-    if (turns) {
+    if constexpr (WITHIN) {
+      auto turned = [&](const auto& from, auto& to, int e0) {
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) {
+          const float x0 = (float)from[2 * e], x1 = (float)from[2 * e + 1];
+          to[2 * e] = (T)(x0 * cosine[e0 + e] - x1 * sine[e0 + e]);
+          to[2 * e + 1] = (T)(x1 * cosine[e0 + e] + x0 * sine[e0 + e]);
+        }
+      };
+      if (first < 2 * a.half) turned(u, ou, 0);
+      if (second < 2 * a.half) turned(v, ov, E / 2);
+    } else if (turns) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        if constexpr (INTERLEAVED && E > 1) {
-          // Pairs 2 e and 2 e + 1 of the two vectors' values in a row.
-          const float x0 = (float)(2 * e < E ? u[2 * e % E] : v[2 * e % E]);
-          const float x1 = (float)(2 * e < E ? u[(2 * e + 1) % E] : v[(2 * e + 1) % E]);
-          const float y0 = x0 * cosine[e] - x1 * sine[e], y1 = x1 * cosine[e] + x0 * sine[e];
-          if (2 * e < E) ou[2 * e % E] = (T)y0, ou[(2 * e + 1) % E] = (T)y1;
-          else ov[2 * e % E] = (T)y0, ov[(2 * e + 1) % E] = (T)y1;
-        } else {
-          const float x0 = (float)u[e], x1 = (float)v[e];
-          ou[e] = (T)(x0 * cosine[e] - x1 * sine[e]);
-          ov[e] = (T)(x1 * cosine[e] + x0 * sine[e]);
-        }
+        const float x0 = (float)u[e], x1 = (float)v[e];
+        ou[e] = (T)(x0 * cosine[e] - x1 * sine[e]);
+        ov[e] = (T)(x1 * cosine[e] + x0 * sine[e]);
       }
     }
-    any_store<T, E>(y + first, ou);
-    if (both) any_store<T, E>(y + second, ov);
+    any_store<PAST, T, E>(y + first, ou);
+    if (both) any_store<PAST, T, E>(y + second, ov);
   }
 }
 
 template <typename T, int E>
-void launch(const Rotary& a, int interleaved, hipStream_t stream) {
+void launch(Rotary a, int interleaved, hipStream_t stream) {
   const long positions = (long)a.B * a.T;
-  const dim3 grid(fm_ceil_div(positions, a.per_block), fm_ceil_div(a.q.heads + a.k.heads, a.group));
-  if (interleaved) hipLaunchKernelGGL((rotary_kernel<T, E, true>), grid, dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL((rotary_kernel<T, E, false>), grid, dim3(256), 0, stream, a);
+  const int heads = a.q.heads + a.k.heads;
+  // A grid has fewer than 2^32 threads.
+  const long most = std::max(1, ((1 << 24) - 1) / a.groups) * (long)a.per_block;
+  // Results of 128 MB or more, half of the last-level cache, go past the L2, where neighbouring
+  // threads' stores fill 64 bytes at a time (16-bit, caches / past: 8 x 4095 positions, 20 heads of 128,
+  // 168 MB 78 / 52 us; 32 x 2500, 24 of 64, 246 MB 122 / 92; 16 x 2500, 123 MB 41 / 48; 20 of 80, 102 MB 26 / 50).
+  const int side_by_side = (interleaved ? a.units : a.units > a.turns ? std::min(a.turns, a.units - a.turns) : a.turns) * E;
+  const bool past = E > 1 && positions * heads * a.D * (long)sizeof(T) >= 128l << 20 && side_by_side * sizeof(T) % 64 == 0;
+  for (; a.start < positions; a.start += most) {
+    const dim3 grid(fm_ceil_div(std::min(most, positions - a.start), a.per_block) * a.groups);
+    if (past && interleaved) hipLaunchKernelGGL((rotary_kernel<T, E, true, true>), grid, dim3(256), 0, stream, a);
+    else if (past) hipLaunchKernelGGL((rotary_kernel<T, E, false, true>), grid, dim3(256), 0, stream, a);
+    else if (interleaved) hipLaunchKernelGGL((rotary_kernel<T, E, true, false>), grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((rotary_kernel<T, E, false, false>), grid, dim3(256), 0, stream, a);
+  }
 }
 
-// Pairs of a thread: 16 bytes of each of its two vectors where both the rotated and the
-// copied channels are whole vectors, 8, or single elements.
-int pairs(const Rotary& a, int size) {
+// Elements of a vector: 16 bytes where turned and copied channels are whole vectors (and
+// whole pairs), 8, or one.
+int elements(const Rotary& a, int size, bool interleaved) {
+  const int turned = interleaved ? 2 * a.half : a.half;
   for (int e : {16 / size, 4})
-    if (a.half % e == 0 && (a.D - 2 * a.half) % e == 0) return e;
+    if (turned % e == 0 && (a.D - 2 * a.half) % e == 0) return e;
   return 1;
 }
 
-// Heads of a thread: as many as leave some 2048 threads a CU, at most 8.
+// Heads of a thread: two share its sines and cosines, where some 2048 threads a CU remain
+// (8 x 4095 positions, 20 heads of 128, one / two / four / eight: 56 / 52 / 53 / 54 us; 250, one / two: 3.7 / 4.0).
 int heads_of_a_thread(const Rotary& a) {
-  const long threads = (long)a.B * a.T * a.units;
-  const int heads = a.q.heads + a.k.heads;
-  int group = 1;
-  while (group < 8 && group < heads && threads * fm_ceil_div(heads, 2 * group) >= 256l * 2048) group *= 2;
-  return group;
+  return (long)a.B * a.T * a.units * fm_ceil_div(a.q.heads + a.k.heads, 2) >= 256l * 2048 ? 2 : 1;
 }
 
 }  // namespace
@@ -178,11 +201,13 @@ int fm_rotary(const void* q, long q_batch, long q_row, long q_head, int heads, c
   a.frequencies = frequencies, a.positions = positions, a.positions_batch = positions_batch, a.first = first;
   a.wide = positions_bytes == 8, a.B = batch, a.T = length, a.D = head_dim, a.half = rotated / 2;
   a.scale = scale, a.sign = inverse ? -scale : scale;
-  const int e = pairs(a, dtype == DT_F32 ? 4 : 2);
-  a.units = a.half / e + fm_ceil_div(head_dim - rotated, 2 * e);
+  const int e = elements(a, dtype == DT_F32 ? 4 : 2, interleaved != 0);
+  a.turns = a.half / e, a.units = a.turns + fm_ceil_div(head_dim - rotated, 2 * e);
+  if (interleaved && e > 1) a.units = fm_ceil_div(head_dim, 2 * e);
   a.per_block = 256 / a.units;
   a.by_units = fm_divisor((unsigned)a.units), a.by_length = fm_divisor((unsigned)length);
-  a.group = heads_of_a_thread(a);
+  a.group = heads_of_a_thread(a), a.groups = fm_ceil_div(heads + kv_heads, a.group);
+  a.by_groups = fm_divisor((unsigned)a.groups);
   if (dtype == DT_F32) {
     e == 4 ? launch<float, 4>(a, interleaved, stream) : launch<float, 1>(a, interleaved, stream);
   } else if (dtype == DT_BF16) {

@@ -63,7 +63,7 @@ constexpr int ONE_BLOCK = 8;  // rows of a group that are left to one block
 // partial sums are two FP32 rows to write and to join: beyond two blocks a CU they
 // are held to a quarter of an input (8191 x 2048 bfloat16 34 -> 27 us).
 int backward_blocks(long rows, const Plan& p, int size) {
-  const int groups = p.nv ? 256 / p.lpr : 1;
+  const int groups = p.nv && p.lpr < 256 ? 256 / p.lpr : 1;
   if (p.nv && rows <= ONE_BLOCK * groups) return 1;
   const long most = std::min<long>(1024, std::max<long>(512, rows * size / 32));
   return (int)std::max<long>(1, std::min<long>(most, (rows + 2 * groups - 1) / (2 * groups)));
