@@ -163,6 +163,12 @@ def call(name: str, *args) -> None:
         check(status, name)
 
 
+def query(name: str, *args) -> int:
+    """What a host-only entry point returns (a size, a yes or no)."""
+    lib = _lib if _lib is not None else library()
+    return getattr(lib, name)(*args)
+
+
 def last_gemm_plan() -> str:
     """Kernel, tiles and K splits of the last GEMM-engine call on this thread."""
     buf = ctypes.create_string_buffer(160)

@@ -129,6 +129,7 @@ def op(entry: str):
 _dispatch_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
 _tracing, _functorch_level = torch._C._get_tracing_state, torch._C._functorch.peek_interpreter_stack
 _profiling = torch._C._autograd._profiler_enabled
+_raw_stream, _Tensor = getattr(torch._C, "_cuda_getCurrentRawStream", None), torch.Tensor
 
 _POINTERS = {entry: tuple(i for i, item in enumerate(spec.split()) if item[:3] in ("in:", "out", "res"))
              for entry, spec in SPECS.items()}
@@ -160,13 +161,13 @@ def call(entry: str, *args) -> None:
             t = values[i]
             if t is None:
                 continue
-            if type(t) is not torch.Tensor or t.requires_grad:
+            if type(t) is not _Tensor or t.requires_grad:
                 break
             if device is None:
                 device = t.device
             values[i] = t.data_ptr()
         else:
             if device is not None and device.type == "cuda":
-                nat.call(entry, *values, torch._C._cuda_getCurrentRawStream(device.index))
+                nat.call(entry, *values, _raw_stream(device.index))
                 return
     getattr(torch.ops.fast_mimi_amd, entry[3:])(*args)

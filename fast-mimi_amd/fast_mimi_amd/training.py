@@ -78,7 +78,8 @@ def _tensor(name: str, t, dtypes=tuple(_DTYPES)) -> torch.Tensor:
         raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}, got {t.dtype}")
-    _reverse_mode(t)
+    if forward_ad._current_level >= 0:
+        _reverse_mode(t)
     if t.requires_grad:
         t = t.detach()
     return t.resolve_neg() if t.is_neg() else t
@@ -110,7 +111,7 @@ def _run(device: torch.device, entry: str, *args) -> None:
 
 def _scratch(like: torch.Tensor, entry: str, *args) -> tuple[torch.Tensor | None, int]:
     """Workspace for a call: what its size query asks for."""
-    size = getattr(nat.library(), entry)(*args)
+    size = nat.query(entry, *args)
     return (like.new_empty((size + 3) // 4, dtype=torch.float32) if size else None), size
 
 
@@ -414,7 +415,7 @@ def rotary_frequencies(dim: int, base: float = 10_000.0, factor: float = 1.0, me
         if context is None or not context > 0 or not fast > slow:
             raise ValueError(f"method ramp needs a positive context and fast > slow, got {context}, {fast} and {slow}")
         keep = ((context * f / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
-        f = f * keep + f / factor * (1 - keep)
+        f = f * (keep + (1 - keep) / factor)
     return f if device is None else f.to(device)
 
 
