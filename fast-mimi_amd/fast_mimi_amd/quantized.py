@@ -21,7 +21,7 @@ from __future__ import annotations
 
 import torch
 
-from .training import _DTYPES, _branch, _differentiable, _on_gpu, _rows, _run, _scratch, _tensor
+from .training import _DTYPES, _branch, _differentiable, _like, _on_gpu, _rows, _run, _scratch, _tensor
 
 __all__ = ["BLOCK", "linear", "quantize", "quantize_weight", "rms_norm"]
 
@@ -87,7 +87,7 @@ def rms_norm(x, weight=None, residual=None, eps: float = 1e-5):
     rows_r, pitch_r, h, stream, out = None, 0, x, dtype, None
     if residual is not None:
         rows_r, pitch_r = _rows(residual)
-        h = out = residual.new_empty(shape)
+        h = out = _like(residual)
         stream = _DTYPES[h.dtype]
     if x.numel():
         _run(device, "fm_rms_norm_quantized", rows, pitch, rows_r, pitch_r, weight, x.numel() // c, c, float(eps), dtype, stream,

@@ -109,6 +109,11 @@ def _run(device: torch.device, entry: str, *args) -> None:
             ops.call(entry, *args)
 
 
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous memory of ``t``'s shape and type (``empty_like`` takes less of the host than ``new_empty``)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _scratch(like: torch.Tensor, entry: str, *args) -> tuple[torch.Tensor | None, int]:
     """Workspace for a call: what its size query asks for."""
     size = nat.query(entry, *args)
@@ -296,13 +301,13 @@ def rms_norm_forward(x, weight=None, residual=None, eps: float = 1e-5):
     """
     x, weight, residual, device = _branch(x, weight, residual, eps)
     shape, dtype = x.shape, _DTYPES[x.dtype]
-    y = x.new_empty(shape)
+    y = _like(x)
     rstd = x.new_empty(shape[:-1], dtype=torch.float32)
     rows, pitch = _rows(x)
     rows_r, pitch_r, h, stream, out = None, 0, x, dtype, None
     if residual is not None:
         rows_r, pitch_r = _rows(residual)
-        h = out = residual.new_empty(shape)
+        h = out = _like(residual)
         stream = _DTYPES[h.dtype]
     if rstd.numel():
         _run(device, "fm_rms_norm_forward", rows, pitch, rows_r, pitch_r, weight, rstd.numel(), shape[-1], float(eps), dtype, stream,
@@ -337,8 +342,8 @@ def rms_norm_backward(grad, x, rstd, weight=None, residual=None, grad_h=None):
         if grad_h.shape != x.shape:
             raise ValueError(f"grad_h must have x's shape {tuple(x.shape)}, got {tuple(grad_h.shape)}")
     device = _on_gpu(x=x, residual=residual, grad=grad, rstd=rstd, grad_h=grad_h, weight=weight)
-    dresidual = x.new_empty(x.shape, dtype=stream)
-    dx = dresidual if grad.dtype == stream else grad.new_empty(x.shape)
+    dresidual = _like(x if residual is None else residual)
+    dx = dresidual if grad.dtype == stream else _like(grad)
     dw = None if weight is None else torch.empty_like(weight)
     rows, c = rstd.numel(), x.shape[-1]
     ws, size = (None, 0) if dw is None else _scratch(x, "fm_rms_norm_backward_workspace_bytes", rows, c)
@@ -463,8 +468,8 @@ def _rotate(q, k, frequencies, positions, interleaved, scale, inverse):
             x = x.contiguous()
         return x, *x.stride()[:3], x.shape[2]
 
-    q_out = q.new_empty(q.shape)
-    k_out = None if k is None else k.new_empty(k.shape)
+    q_out = _like(q)
+    k_out = None if k is None else _like(k)
     if b and t and q.shape[2] + (0 if k is None else k.shape[2]):
         batch, size = (0, 8) if positions is None else (t if positions.dim() == 2 else 0, positions.element_size())
         _run(device, "fm_rotary", *heads(q), *heads(k), frequencies, positions, batch, size, first, b, t, d,
@@ -684,7 +689,7 @@ def cross_attention_forward(q, k, v, scale: float | None = None, key_lengths=Non
     device = _on_gpu(q=q, k=k, v=v, key_lengths=key_lengths, query_lengths=query_lengths)
     b, t, h, d = q.shape
     s, kv = k.shape[1], k.shape[2]
-    out = q.new_empty((b, t, h, d))
+    out = _like(q)
     lse = q.new_empty((b, t, h), dtype=torch.float32)
     if b and t:
         ws, size = _scratch(q, "fm_cross_attention_forward_workspace_bytes", b, t, s, h, kv, d)
@@ -705,7 +710,7 @@ def cross_attention_backward(grad, q, k, v, out, lse, scale: float | None = None
     if out.shape != q.shape or lse.shape != (b, t, h) or not lse.is_contiguous():
         raise ValueError("out and lse must be what cross_attention_forward returned for q, k and v")
     device = _on_gpu(q=q, k=k, v=v, grad=grad, out=out, lse=lse, key_lengths=key_lengths, query_lengths=query_lengths)
-    dq, dk, dv = q.new_empty((b, t, h, d)), q.new_empty((b, s, kv, d)), q.new_empty((b, s, kv, d))
+    dq, dk, dv = _like(q), _like(k), _like(v)
     if b and t == 0:
         return dq, dk.zero_(), dv.zero_()
     if b:
