@@ -296,7 +296,7 @@ def rms_norm_forward(x, weight=None, residual=None, eps: float = 1e-5):
 
     ``y = h * rstd * weight`` has ``x``'s type; ``h``, the stream's next value, that of
     ``residual``: ``x``'s, or FP32.  ``y`` is formed from the sum before it is rounded.
-    Without a residual ``h`` is ``x`` itself.  ``weight`` (optional) has ``x``'s type or
+    Without a residual ``h`` is ``x`` itself.  Squares and sums are FP32's.  ``weight`` (optional) has ``x``'s type or
     FP32; ``rstd`` is FP32, one per row, for :func:`rms_norm_backward`.
     """
     x, weight, residual, device = _branch(x, weight, residual, eps)
@@ -441,8 +441,8 @@ def _rotary_input(q, k, frequencies, positions, scale):
     first = 0
     if isinstance(positions, int) and not isinstance(positions, bool):
         first, positions = positions, None
-        if not -(1 << 62) < first < 1 << 62:
-            raise ValueError(f"positions must start within 62 bits, got {first}")
+        if not -(1 << 53) <= first <= (1 << 53) - t:
+            raise ValueError(f"positions must lie within 53 bits, got {first} and the {t} from there on")
     if positions is not None:
         positions = _tensor("positions", positions, (torch.int32, torch.int64))
         if positions.shape not in ((t,), (b, t)):
@@ -488,8 +488,8 @@ def rotary_forward(q, k, frequencies, positions=None, interleaved: bool = False,
     as large; the others are copied.  ``positions``: int32 or int64 ``[positions]`` or
     ``[batch, positions]``, or the first position (``None``: 0).
 
-    Angles are formed in 64 bits: positions of any size are as exact as small ones.  At
-    most 2^24 positions in all, heads of 512.
+    Angles are formed in 64 bits, with what those round off beside them: positions up to 2^53 are
+    as exact as small ones.  At most 2^24 positions in all, heads of 512.
     """
     return _rotate(q, k, frequencies, positions, interleaved, scale, 0)
 

@@ -651,9 +651,9 @@ int fm_code_embedding_backward(const void* dout, long ld_dout, const int64_t* co
  * stream_dtype.  x has rows of `channels` elements at a pitch of ld_x elements, residual
  * (of stream_dtype: dtype, or FP32) at ld_residual; rows may start at any element.
  * residual NULL: y of x alone, h (then NULL) is not written.  y (dtype), h
- * (stream_dtype) and rstd [rows] are contiguous; h may be residual itself.  gamma
- * (weight_dtype: dtype, or FP32) may be NULL (one).  Fewer than 2^31 - 1 rows, at most
- * 2^26 channels.
+ * (stream_dtype) and rstd [rows] are contiguous, other memory than x and residual.  gamma
+ * (weight_dtype: dtype, or FP32) may be NULL (one).  Squares and sums are FP32's.  Fewer
+ * than 2^31 - 1 rows, at most 2^26 channels.
  * Stands where a model over the codes has it in the place of nn.LayerNorm
  * (model.py:2028-2061) and the residual's addition behind it.
  */
@@ -686,7 +686,7 @@ int fm_rms_norm_backward(const void* dy, long ld_dy, const void* x, long ld_x, c
  * goes (a, b) -> scale (a cos - b sin, b cos + a sin) at the angle position *
  * frequencies[i]; the others are copied.  frequencies are rotated / 2 doubles, radians
  * per position.  positions holds [length] per batch item, positions_batch apart (0: the
- * same for all), of positions_bytes 4 or 8; NULL: first, first + 1, ...  inverse turns
+ * same for all), of positions_bytes 4 or 8 (exact up to 2^53); NULL: first, first + 1, ...  inverse turns
  * back (the gradient).  q / k are strided (elements; channels adjacent), q_out / k_out
  * contiguous, other memory than q / k.  head_dim <= 512, batch * length <= 2^24.
  * Replaces MimiRotaryEmbedding and its use in MimiAttention (model.py:1484-1535, :1870-1961) where the
@@ -752,9 +752,12 @@ int fm_quantize_weight(const void* weight, int out_features, int in_features, in
 /*
  * y [rows][out_features] (dtype) = x weight^T of 8-bit x [rows][in_features] and weight
  * [out_features][in_features] with their scales (above): every product times both
- * powers of two, summed in FP32, rounded once.  All contiguous, x and weight 16-byte
- * aligned, in_features a multiple of 16, rows at most 2097120.  The workspace holds the parts of calls
- * whose in_features are split over blocks; NULL where its size is 0.
+ * powers of two, summed in FP32, rounded once.  For 16-bit results the matrix cores line up
+ * eight products by their largest and drop what lies 2^-13 below it; FP32 results are sums of
+ * exact products.  Values below 2^-126 with their scale may count as zero.  All contiguous, x, weight and
+ * y 16-byte aligned, in_features a multiple of 16 up to 2^22, rows and out_features up to 2^24,
+ * 2^40 results.  The workspace holds the parts of calls whose in_features are split over
+ * blocks; NULL where its size is 0.
  * Stands beside fm_linear (nn.Linear of the transformer layers, model.py:1870-2061)
  * where a model over the codes is served in 8 bits.
  */

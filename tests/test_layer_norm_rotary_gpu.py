@@ -158,7 +158,7 @@ def test_rotary(t, interleaved, b, n, h, kv, d, rotated):
             assert_within(name, y, want, bound)
 
 
-@pytest.mark.parametrize("positions", [0, 7, -3, 1_000_000, 1 << 40, torch.tensor([5, 0, 1 << 45, -9]),
+@pytest.mark.parametrize("positions", [0, 7, -3, 1_000_000, 1 << 40, (1 << 53) - 4, -(1 << 53), torch.tensor([5, 0, 1 << 45, -9]),
                                        torch.tensor([3, 1, 2, 2_000_000_000], dtype=torch.int32)])
 def test_rotary_positions(positions):
     """Far positions are as exact as near ones; no positions start at 0."""

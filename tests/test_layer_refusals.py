@@ -59,7 +59,8 @@ XS, WS = scales(4, 2), scales(1, 2)
     (TypeError, "positions must be a tensor", lambda: tr.rotary(Q, None, F, True)),
     (TypeError, "positions must be a tensor", lambda: tr.rotary(Q, None, F, 2.5)),
     (ValueError, "positions must have", lambda: tr.rotary(Q, None, F, torch.arange(4))),
-    (ValueError, "62 bits", lambda: tr.rotary(Q, None, F, 1 << 62)),
+    (ValueError, "53 bits", lambda: tr.rotary(Q, None, F, (1 << 53) - 4)),
+    (ValueError, "53 bits", lambda: tr.rotary(Q, None, F, -(1 << 53) - 1)),
     (ValueError, "head_dim", lambda: tr.rotary(torch.empty(1, 1, 1, 514), None, F)),
     (ValueError, "scale", lambda: tr.rotary(Q, None, F, scale=float("inf"))),
     (ValueError, "positions in all", lambda: tr.rotary(torch.empty(1, 1, 1, 1).expand(4097, 4096, 1, 2), None, F[:1])),

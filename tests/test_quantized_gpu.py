@@ -127,6 +127,11 @@ def test_linear_shapes_and_views():
     wide = torch.zeros(24, 300, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)
     wide[:, 5:261] = x
     assert torch.equal(qz.linear(wide[:, 5:261], xs, w, ws), want)
+    # Scales of a longer row, and of weights kept in another order.
+    far = torch.full((24, 7), 255, dtype=torch.uint8, device=DEV).view(torch.float8_e8m0fnu)
+    far.view(torch.uint8)[:, 3:5] = xs.view(torch.uint8)
+    turned = ws.view(torch.uint8).t().contiguous().t().view(torch.float8_e8m0fnu)
+    assert torch.equal(qz.linear(x, far[:, 3:5], w.view(torch.uint8).t().contiguous().t().view(torch.float8_e4m3fn), turned), want)
     assert qz.linear(x[:0], xs[:0], w, ws).shape == (0, 96)
 
 
