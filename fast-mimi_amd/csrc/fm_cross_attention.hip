@@ -64,24 +64,45 @@ __global__ __launch_bounds__(256) void cross_join_kernel(Attn a) {
 // heads of 64, FP32: 143 / 48 / 40 us; 4000 over 64, bfloat16, in 1 / 8 / 16: 59 / 23 / 21).
 int cut(long blocks, int tiles) { return (int)std::max<long>(1, std::min<long>({tiles / 2, 512 / std::max<long>(blocks, 1), 64})); }
 
-// A block's waves with rows (or keys) of their own, as own_waves has it for their number, but that
-// the waves which share them have two tiles of 32 each at least to walk (own_waves' / four of
-// their own: forward 2 x 3000 over 20 keys, FP32: 17.5 / 13.1 us, 13 over 7: 8.9 / 7.5; 16 x 200 over 100, 8 / 2
-// heads of 128, bfloat16, backward: 41 / 38; dK / dV of 3000 keys from 2 x 20 rows, 8 heads: 26.5 / 22.9 in all).
-int waves_apart(const Attn& a, long own, long walked) { return std::max(own_waves(a, own), walked < 128 ? 4 : walked < 256 ? 2 : 1); }
-
 long sequences(const Attn& a) { return (long)a.B * a.KV; }
-int row_splits(const Attn& a) {  // forward, dQ
-  const long rows = (long)a.T * a.G;
-  return cut(sequences(a) * fm_ceil_div(rows, 32), fm_ceil_div(a.S, 128));
+
+// A block's waves with rows (or keys) of their own: four where that leaves 384 blocks, two where 256
+// are left, else one, but that the waves which share them have two tiles of 32 each at least to walk.  With
+// two / four (us): forward 2 x 4096 over 500, 8 heads of 64 (512 blocks of 128 rows) 21.3 / 20.0, 4 x 2000
+// over 500, 8 / 2 heads of 128 (504) 37 / 31, 2 x 1000 over 1000, 16 / 4 heads of 128 (256) 31.7 / 34.4; short
+// walks, less than four / four: 2 x 3000 over 20, FP32 17.5 / 13.1, 13 over 7 8.9 / 7.5.
+int waves_apart(const Attn& a, long own, long walked) {
+  const long seqs = sequences(a);
+  const int most = seqs * fm_ceil_div(own, 128) >= 384 ? 4 : seqs * fm_ceil_div(own, 64) >= 256 ? 2 : 1;
+  return std::max(most, walked < 128 ? 4 : walked < 256 ? 2 : 1);
 }
-int key_splits(const Attn& a) {  // dK / dV
-  return cut(sequences(a) * fm_ceil_div(a.S, 32), fm_ceil_div((long)a.T * a.G, 128));
+
+struct Shape {
+  int waves, splits;
+};
+Shape row_shape(const Attn& a) {  // forward, dQ
+  const long rows = (long)a.T * a.G;
+  const int splits = cut(sequences(a) * fm_ceil_div(rows, 32), fm_ceil_div(a.S, 128));
+  return {splits > 1 ? 1 : waves_apart(a, rows, a.S), splits};
+}
+// dK / dV.  Where the blocks are no two to a CU, long walks are cut as well, if that fills the
+// rounds of 512 to nine tenths (whole backward, uncut / so, us: 8 x 2500 over 300, 8 heads of 64, FP32 320 / 284,
+// bfloat16 110 / 106, with lengths from 0 to 300 101 / 98; 4 x 2048 over 1024, 8 / 4 heads of 64, FP32 394 / 338).
+Shape key_shape(const Attn& a) {
+  const long rows = (long)a.T * a.G;
+  const int tiles = fm_ceil_div(rows, 128), splits = cut(sequences(a) * fm_ceil_div(a.S, 32), tiles);
+  if (splits > 1) return {1, splits};
+  const int waves = waves_apart(a, a.S, rows);
+  const long blocks = sequences(a) * fm_ceil_div(a.S, 32 * waves);
+  if (blocks < 512 && a.D <= 64)
+    for (int s = 1; s <= tiles / 6; ++s)
+      if (10 * blocks * s >= 9 * ((blocks * s + 511) / 512 * 512)) return {waves, s};
+  return {waves, 1};
 }
 
 size_t backward_floats(const Attn& a) {
   const size_t dt = a.D > 64 ? 128 : 64;
-  const size_t q = row_splits(a), k = key_splits(a);
+  const size_t q = row_shape(a).splits, k = key_shape(a).splits;
   return std::max(q > 1 ? q * sequences(a) * a.T * a.G * (dt + 1) : 0, k > 1 ? k * 2 * sequences(a) * a.S * dt : 0);
 }
 
@@ -96,8 +117,7 @@ size_t backward_floats(const Attn& a) {
 template <typename T, int DT>
 int cross_forward(Attn a, hipStream_t stream) {
   const long rows = (long)a.T * a.G;
-  const int waves = a.splits > 1 ? 1 : waves_apart(a, rows, a.S);
-  FM_CROSS_LAUNCH(attention_forward_kernel, waves, rows, a.splits);
+  FM_CROSS_LAUNCH(attention_forward_kernel, row_shape(a).waves, rows, a.splits);
   if (a.splits > 1)
     hipLaunchKernelGGL((attention_join_kernel<T, DT, true>), dim3(fm_ceil_div(sequences(a) * rows, 4)), dim3(256), 0, stream, a);
   return (int)hipGetLastError();
@@ -108,23 +128,23 @@ int cross_backward(Attn a, float* workspace, hipStream_t stream) {
   const long rows = (long)a.T * a.G;
   a.part_o = workspace;
   if (rows > 0) {
-    a.splits = row_splits(a);
+    const Shape shape = row_shape(a);
+    a.splits = shape.splits;
     a.part_ml = workspace + (size_t)a.splits * sequences(a) * rows * DT;
-    const int waves = a.splits > 1 ? 1 : waves_apart(a, rows, a.S);
-    FM_CROSS_LAUNCH(attention_dq_kernel, waves, rows, a.splits);
+    FM_CROSS_LAUNCH(attention_dq_kernel, shape.waves, rows, a.splits);
     if (a.splits > 1)
       hipLaunchKernelGGL((cross_join_kernel<T, DT, false>), dim3(fm_ceil_div(sequences(a) * rows, 4)), dim3(256), 0, stream, a);
   }
   if (a.S > 0) {
-    a.splits = key_splits(a);
+    const Shape shape = key_shape(a);
+    a.splits = shape.splits;
     if constexpr (HELD<T, DT>) {
       const dim3 grid((unsigned)sequences(a), fm_ceil_div(a.S, 64), a.splits);
       if ((long)grid.x * grid.y * grid.z > 512)
         hipLaunchKernelGGL((attention_dkv_kernel<T, DT, 2, 2, true>), grid, dim3(256), 0, stream, a);
       else hipLaunchKernelGGL((attention_dkv_kernel<T, DT, 2, 4, true>), grid, dim3(512), 0, stream, a);
     } else {
-      const int waves = a.splits > 1 ? 1 : waves_apart(a, a.S, rows);
-      FM_CROSS_LAUNCH(attention_dkv_kernel, waves, a.S, a.splits);
+      FM_CROSS_LAUNCH(attention_dkv_kernel, shape.waves, a.S, a.splits);
     }
     if (a.splits > 1)
       hipLaunchKernelGGL((cross_join_kernel<T, DT, true>), dim3(fm_ceil_div(2 * sequences(a) * a.S, 4)), dim3(256), 0, stream, a);
@@ -155,7 +175,7 @@ extern "C" {
 size_t fm_cross_attention_forward_workspace_bytes(int batch, int queries, int keys, int heads, int kv_heads, int head_dim) {
   const Attn a = cross_sizes(batch, queries, keys, heads, kv_heads, head_dim, 1.0f);
   if (cross_check(a, DT_F32) != FM_OK && cross_check(a, DT_BF16) != FM_OK) return 0;
-  return batch == 0 || queries == 0 ? 0 : workspace_floats(a, row_splits(a)) * sizeof(float);
+  return batch == 0 || queries == 0 ? 0 : workspace_floats(a, row_shape(a).splits) * sizeof(float);
 }
 
 int fm_cross_attention_forward(const void* q, long q_batch, long q_row, long q_head, const void* k, long k_batch, long k_row,
@@ -170,7 +190,7 @@ int fm_cross_attention_forward(const void* q, long q_batch, long q_row, long q_h
   if (batch == 0 || queries == 0) return FM_OK;
   if (!q || !out || !lse || (keys > 0 && (!k || !v))) return FM_BAD_ARGUMENT;
   if (reinterpret_cast<uintptr_t>(out) & 15) return FM_UNSUPPORTED;
-  a.splits = row_splits(a);
+  a.splits = row_shape(a).splits;
   if (a.splits > 1) {
     if (!workspace || workspace_bytes < workspace_floats(a, a.splits) * sizeof(float)) return FM_WORKSPACE_TOO_SMALL;
     if (reinterpret_cast<uintptr_t>(workspace) & 15) return FM_UNSUPPORTED;

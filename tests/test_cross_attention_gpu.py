@@ -87,6 +87,18 @@ def test_long_queries_are_cut(b, t, s, h, kv, d, dtype):
     check(q, k, v, grad, None, None, [7 + 100 * i for i in range(b)])
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("b,t,s,h,kv,d", [(4, 1540, 510, 8, 8, 32), (4, 2309, 300, 8, 8, 64)])
+def test_middling_blocks_are_cut(b, t, s, h, kv, d, dtype):
+    """Blocks for one round, not two, and a long walk: dK's and dV's rows are split over blocks of more waves."""
+    from fast_mimi_amd import _native as nat
+
+    assert nat.library().fm_cross_attention_backward_workspace_bytes(b, t, s, h, kv, d) > 0
+    q, k, v, grad = inputs(b, t, s, h, kv, d, dtype)
+    check(q, k, v, grad)
+    check(q, k, v, grad, 0.3, [s, 0, 1, s - 33], [t, t, 770, 0])
+
+
 def test_views():
     """Slices of packed projections, transposed heads, odd offsets."""
     g = torch.Generator().manual_seed(3)
