@@ -102,7 +102,9 @@ def linear(x, x_scale, weight, weight_scale, dtype: torch.dtype = torch.bfloat16
     ``x`` and ``x_scale`` are what :func:`quantize` or :func:`rms_norm` gave, ``weight`` and
     ``weight_scale`` what :func:`quantize_weight` did.  ``in`` must be a multiple of 16.
     """
+    given = x, weight
     x, weight = _tensor("x", x, (_VALUES,)), _tensor("weight", weight, (_VALUES,))
+    _no_gradient(*given)
     x_scale, weight_scale = _tensor("x_scale", x_scale, (_SCALES,)), _tensor("weight_scale", weight_scale, (_SCALES,))
     if dtype not in _DTYPES:
         raise TypeError(f"dtype must be float32, bfloat16 or float16, got {dtype}")

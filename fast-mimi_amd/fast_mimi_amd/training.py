@@ -520,6 +520,8 @@ class _Rotary(torch.autograd.Function):
 
 def rotary(q, k, frequencies, positions=None, interleaved: bool = False, scale: float = 1.0):
     """``(q, k)`` turned by their positions, differentiable in both (see :func:`rotary_forward`)."""
+    if _differentiable(frequencies):
+        raise ValueError("frequencies take no gradient, but require one")
     if not _differentiable(q, k):
         return rotary_forward(q, k, frequencies, positions, interleaved, scale)
     out = _apply(_Rotary, (q, k), q, k, frequencies, positions, interleaved, scale)

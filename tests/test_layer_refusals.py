@@ -107,6 +107,8 @@ XS, WS = scales(4, 2), scales(1, 2)
     (ValueError, "x_scale must have", lambda: qz.linear(X8, XS[:, :1], W8, WS)),
     (ValueError, "weight_scale must have", lambda: qz.linear(X8, XS, W8, XS)),
     (ValueError, "ROCm GPU", lambda: qz.linear(X8, XS, W8, WS)),
+    (RuntimeError, "no gradient", lambda: qz.linear(X8, XS, W8.detach().requires_grad_(), WS)),
+    (ValueError, "no gradient", lambda: tr.rotary(Q, Q, F.clone().requires_grad_())),
 ])
 def test_python_refusals(error, match, call):
     with pytest.raises(error, match=match):

@@ -135,6 +135,24 @@ def test_linear_shapes_and_views():
     assert qz.linear(x[:0], xs[:0], w, ws).shape == (0, 96)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("m,n,k", [(3, 40, 256), (20, 300, 400), (90, 300, 1040), (300, 520, 256)])
+def test_linear_of_not_a_number(m, n, k, dtype):
+    """A NaN value or scale reaches its row's outputs, or its weights' columns, and no others."""
+    x, xs, w, ws = operands(m, n, k)
+    want = qz.linear(x, xs, w, ws, dtype)
+    bad_x, bad_xs, bad_w, bad_ws = (t.view(torch.uint8).clone() for t in (x, xs, w, ws))
+    bad_x[1, 200], bad_xs[m - 1, 0], bad_w[2, 5], bad_ws[-1, 1] = 127, 255, 255, 255
+    nan = torch.zeros(m, n, dtype=torch.bool)
+    nan[1], nan[m - 1] = True, True
+    f8, e8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+    rows = qz.linear(bad_x.view(f8), bad_xs.view(e8), w, ws, dtype)
+    assert torch.equal(rows.isnan().cpu(), nan) and torch.equal(rows.cpu()[~nan], want.cpu()[~nan])
+    nan[:], nan[:, 2], nan[:, (n - 1) // 128 * 128:] = False, True, True
+    columns = qz.linear(x, xs, bad_w.view(f8), bad_ws.view(e8), dtype)
+    assert torch.equal(columns.isnan().cpu(), nan) and torch.equal(columns.cpu()[~nan], want.cpu()[~nan])
+
+
 def test_linear_scales_reach_far():
     """Scales of both ends: their products, not the partial ones, decide what is finite."""
     x, xs, w, ws = operands(20, 40, 256)
