@@ -11,6 +11,11 @@
 // result's size with normal values, little beside the half step of a 16-bit result (2e-3
 // and 2.4e-4).  FP32 results would lose bits by it, so those are summed from bfloat16 products, which are
 // exact: e4m3 times a power of two is a bfloat16, at half the matrix rate.
+//
+// Many rows are bound by the matrix cores and what feeds them: 8192^3 in 430 us (2560 TFLOP/s; up to 510 as the
+// clock goes, and 413 on another card), FP32 results 916; without its loads from memory it takes a tenth less.
+// Few rows are bound by latency and the weights' bytes: 1 x 4096 to 6144 7.4 us (25 MB), 32 x 8192 to 2048 6.3
+// and the join 2.7.
 
 #include "fm_common.h"
 
