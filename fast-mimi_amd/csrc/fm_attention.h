@@ -866,6 +866,10 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Attn a) {
 // frames 12 / 13 / 13).  Rows of more keys with one large probability keep it (1.4 times at 0.3, 2.2
 // at 0.65): which they are is known after the pass only, and a second one for all
 // would be 12-24% of the backward (16 x 2500, window 250: 201 -> 230 us).
+// In a cross attention of few rows in all there may be little else: with 33 to 130 keys dQ of one to
+// four of them was at 1.2 times at the median of draws and up to 4 times, so those go over their
+// keys twice, whatever their number, where these are not cut (1 x 8 rows over 300, 8 heads of 64: backward 16 -> 19 us).
+constexpr int FEW_RESULTS = 512;
 template <typename T, int DT, int WQ, int WK, bool CROSS>
 struct QueryGradient {
   template <bool SPLITS>
@@ -945,6 +949,7 @@ FM_DEVICE bool QueryGradient<T, DT, WQ, WK, CROSS>::run(const Attn& a, unsigned 
   // With few keys (some row sees fewer than FEW) a first pass makes delta exact.
   constexpr int FEW = 32;
   bool first = sizeof(T) == 2 && tiles > begin && (CROSS ? w.len : min(w.b_lo + 1, a.window)) < FEW;
+  if (CROSS && sizeof(T) == 2 && a.splits <= 1 && (long)a.B * a.T * a.H <= FEW_RESULTS) first = tiles > begin;
   for (;; first = false) {
     for (int i = begin; i < tiles; ++i) {
       tile_barrier();
@@ -1061,6 +1066,8 @@ constexpr bool HELD = sizeof(T) == 2 && DT == 128;
 // in two pieces; a block of that many rows is one or two tiles long (backward of 16 x
 // 13, 100 and 250 positions, never / up to 128 rows / up to 512: 13.0 / 13.4 / 13.4, 16.9 /
 // 17.7 / 17.8, 25.2 / 25.6 / 26.8 us; 16 x 2500 under a window of 100: 172 / 170 / 184).
+// So have cross attention's dV and dK of few keys in all (with 2 keys and 129 to 3000 queries up to
+// 1.8 times otherwise; 2 x 3000 over 16, 8 heads of 64: backward 24 -> 25 us).
 constexpr int FEW_ROWS = 128;
 template <typename T, int DT, int WK, int WR, bool CROSS>
 struct KeyGradients {
@@ -1118,7 +1125,7 @@ FM_DEVICE bool KeyGradients<T, DT, WK, WR, CROSS>::run(const Attn& a, unsigned c
       tiles = r_hi >= r_lo && tiles ? (r_hi - r_lo) / ROWS + 1 : 0;
     }
   }
-  const bool few = sizeof(T) == 2 && r_hi - r_lo < FEW_ROWS;
+  const bool few = sizeof(T) == 2 && (r_hi - r_lo < FEW_ROWS || (CROSS && (long)a.B * a.S * a.KV <= FEW_RESULTS));
 
   const T* qp = static_cast<const T*>(a.q.p) + b * a.q.batch + kh * a.G * a.q.head;
   const T* gp = static_cast<const T*>(a.dout.p) + b * a.dout.batch + kh * a.G * a.dout.head;

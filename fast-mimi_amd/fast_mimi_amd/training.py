@@ -394,7 +394,8 @@ def rms_norm(x, weight=None, residual=None, eps: float = 1e-5):
 # --------------------------------------------------------- rotary positions
 def rotary_frequencies(dim: int, base: float = 10_000.0, factor: float = 1.0, method: str = "linear", context: int | None = None,
                        fast: float = 32.0, slow: float = 1.0, device=None) -> torch.Tensor:
-    """Radians per position of ``dim / 2`` channel pairs, ``base ** (-2 i / dim)``, in float64.
+    """Radians per position of ``dim / 2`` channel pairs, ``base ** (-2 i / dim)``, in float64: made once, on the host, and
+    copied to ``device``.
 
     ``factor`` stretches them for contexts that many times as long:
 

@@ -124,16 +124,17 @@ def test_a_captured_layer():
 
 
 @pytest.mark.parametrize("step", [
-    lambda x: tr.rms_norm(x, None, torch.ones_like(x))[0],
-    lambda x: tr.rotary(x, x, tr.rotary_frequencies(32, device=DEV))[1],
-    lambda x: tr.cross_attention(x, x, x)])
+    lambda x, f: tr.rms_norm(x, None, torch.ones_like(x))[0],
+    lambda x, f: tr.rotary(x, x, f)[1],
+    lambda x, f: tr.cross_attention(x, x, x)])
 def test_a_leaf_in_an_eager_graph_is_not_captured(step):
     x = torch.randn(2, 9, 4, 32, device=DEV, requires_grad=True)
-    y = step(x)  # its graph stays alive
+    f = tr.rotary_frequencies(32, device=DEV)
+    y = step(x, f)  # its graph stays alive
     torch.cuda.synchronize()
     with pytest.raises(RuntimeError, match="eager autograd graph"):
         with torch.cuda.graph(torch.cuda.CUDAGraph()):
-            step(x)
+            step(x, f)
     y.backward(torch.ones_like(y))
     assert x.grad.isfinite().all()
 
