@@ -21,7 +21,7 @@ from __future__ import annotations
 
 import torch
 
-from .training import _DTYPES, _branch, _differentiable, _like, _on_gpu, _rows, _run, _scratch, _tensor
+from .training import _DTYPES, _branch, _like, _on_gpu, _rows, _run, _scratch, _tensor
 
 __all__ = ["BLOCK", "linear", "quantize", "quantize_weight", "rms_norm"]
 
@@ -30,8 +30,9 @@ _VALUES, _SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 
 def _no_gradient(*inputs) -> None:
-    if _differentiable(*inputs):
-        raise RuntimeError("the 8-bit operators have no gradient: an input requires one (call them under torch.no_grad())")
+    for t in inputs:
+        if t is not None and isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("the 8-bit operators have no gradient: an input requires one (call them under torch.no_grad())")
 
 
 def _blocks(n: int) -> int:
@@ -110,18 +111,19 @@ def linear(x, x_scale, weight, weight_scale, dtype: torch.dtype = torch.bfloat16
         raise TypeError(f"dtype must be float32, bfloat16 or float16, got {dtype}")
     if weight.dim() != 2 or 0 in weight.shape:
         raise ValueError(f"weight must be [out, in], got shape {tuple(weight.shape)}")
-    n, k = weight.shape
-    if x.dim() < 1 or x.shape[-1] != k:
-        raise ValueError(f"x must be [..., {k}] for weight {(n, k)}, got shape {tuple(x.shape)}")
+    (n, k), shape = weight.shape, x.shape
+    if not shape or shape[-1] != k:
+        raise ValueError(f"x must be [..., {k}] for weight {(n, k)}, got shape {tuple(shape)}")
     if k % 16:
         raise ValueError(f"the inputs of a projection must be a multiple of 16, got {k}")
-    if x_scale.shape != (*x.shape[:-1], _blocks(k)):
-        raise ValueError(f"x_scale must have shape {(*x.shape[:-1], _blocks(k))}, got {tuple(x_scale.shape)}")
-    if weight_scale.shape != (_blocks(n), _blocks(k)):
-        raise ValueError(f"weight_scale must have shape {(_blocks(n), _blocks(k))}, got {tuple(weight_scale.shape)}")
+    lead, blocks = shape[:-1], _blocks(k)
+    if x_scale.shape != (*lead, blocks):
+        raise ValueError(f"x_scale must have shape {(*lead, blocks)}, got {tuple(x_scale.shape)}")
+    if weight_scale.shape != (_blocks(n), blocks):
+        raise ValueError(f"weight_scale must have shape {(_blocks(n), blocks)}, got {tuple(weight_scale.shape)}")
     device = _on_gpu(x=x, x_scale=x_scale, weight=weight, weight_scale=weight_scale)
     rows = x.numel() // k
-    y = x.new_empty((*x.shape[:-1], n), dtype=dtype)
+    y = x.new_empty((*lead, n), dtype=dtype)
     if rows:
         ws, size = _scratch(y, "fm_linear_fp8_workspace_bytes", rows, k, n)
         _run(device, "fm_linear_fp8", _aligned(x), x_scale.contiguous(), _aligned(weight), weight_scale.contiguous(), rows, k, n,

@@ -124,7 +124,7 @@ def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int]:
     """``t`` as rows of its last dimension at one pitch (a copy where its
     strides allow none), and the pitch."""
     c = t.shape[-1]
-    if t.numel() == 0 or t.is_contiguous():
+    if t.is_contiguous() or t.numel() == 0:
         return t, c
     if t.stride(-1) == 1 or c == 1:
         # Leading dimensions that collapse into one.
@@ -271,23 +271,24 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5):
 def _branch(x, weight, residual, eps):
     """A branch, the norm's weight and the residual stream, checked; the device."""
     x = _tensor("x", x)
-    if x.dim() < 1 or x.shape[-1] == 0:
-        raise ValueError(f"x must have a last dimension to normalise, got shape {tuple(x.shape)}")
+    shape = x.shape
+    if not shape or not shape[-1]:
+        raise ValueError(f"x must have a last dimension to normalise, got shape {tuple(shape)}")
     if residual is not None:
         residual = _tensor("residual", residual, _WIDER[x.dtype])
-        if residual.shape != x.shape:
-            raise ValueError(f"residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
+        if residual.shape != shape:
+            raise ValueError(f"residual must have x's shape {tuple(shape)}, got {tuple(residual.shape)}")
     if not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}")
-    return x, _norm_weight(weight, x), residual, _on_gpu(x=x, residual=residual, weight=weight)
+    return x, _norm_weight(weight, x, shape), residual, _on_gpu(x=x, residual=residual, weight=weight)
 
 
-def _norm_weight(weight, x):
+def _norm_weight(weight, x, shape):
     if weight is None:
         return None
     weight = _tensor("weight", weight, _WIDER[x.dtype])
-    if weight.shape != x.shape[-1:]:
-        raise ValueError(f"weight must have shape {tuple(x.shape[-1:])}, got {tuple(weight.shape)}")
+    if weight.shape != shape[-1:]:
+        raise ValueError(f"weight must have shape {tuple(shape[-1:])}, got {tuple(weight.shape)}")
     return weight.contiguous()
 
 
@@ -329,23 +330,24 @@ def rms_norm_backward(grad, x, rstd, weight=None, residual=None, grad_h=None):
     x = _tensor("x", x, wide if residual is None else (grad.dtype,))
     residual = None if residual is None else _tensor("residual", residual, wide)
     rstd = _tensor("rstd", rstd, (torch.float32,))
-    if x.dim() < 1 or x.shape[-1] == 0 or grad.shape != x.shape:
-        raise ValueError(f"grad must have x's shape {tuple(x.shape)}, got {tuple(grad.shape)}")
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError(f"residual must have x's shape {tuple(x.shape)}, got {tuple(residual.shape)}")
-    if rstd.shape != x.shape[:-1] or not rstd.is_contiguous():
+    shape = x.shape
+    if not shape or not shape[-1] or grad.shape != shape:
+        raise ValueError(f"grad must have x's shape {tuple(shape)}, got {tuple(grad.shape)}")
+    if residual is not None and residual.shape != shape:
+        raise ValueError(f"residual must have x's shape {tuple(shape)}, got {tuple(residual.shape)}")
+    if rstd.shape != shape[:-1] or not rstd.is_contiguous():
         raise ValueError("rstd must be what rms_norm_forward returned for x")
-    weight = _norm_weight(weight, grad)
+    weight = _norm_weight(weight, grad, shape)
     stream = x.dtype if residual is None else residual.dtype
     if grad_h is not None:
         grad_h = _tensor("grad_h", grad_h, (stream,))
-        if grad_h.shape != x.shape:
-            raise ValueError(f"grad_h must have x's shape {tuple(x.shape)}, got {tuple(grad_h.shape)}")
+        if grad_h.shape != shape:
+            raise ValueError(f"grad_h must have x's shape {tuple(shape)}, got {tuple(grad_h.shape)}")
     device = _on_gpu(x=x, residual=residual, grad=grad, rstd=rstd, grad_h=grad_h, weight=weight)
     dresidual = _like(x if residual is None else residual)
     dx = dresidual if grad.dtype == stream else _like(grad)
     dw = None if weight is None else torch.empty_like(weight)
-    rows, c = rstd.numel(), x.shape[-1]
+    rows, c = rstd.numel(), shape[-1]
     ws, size = (None, 0) if dw is None else _scratch(x, "fm_rms_norm_backward_workspace_bytes", rows, c)
     (x, ld_x), (grad, ld_dy) = _rows(x), _rows(grad)
     residual, ld_r = (None, 0) if residual is None else _rows(residual)
