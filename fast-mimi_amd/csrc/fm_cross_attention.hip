@@ -13,8 +13,8 @@
 // long walk, it is cut, and the parts are joined in their order.
 //
 // Long calls are bound by the matrix cores and the exponentials beside them, dK / dV with heads of 128
-// by LDS reads: 2 x 4095 over 4001, 16 / 4 heads of 128, bfloat16: forward 303 us (890 TFLOP/s), dQ 483,
-// dK / dV 737.  2500 over up to 300 keys, 8 heads of 64, 8 items: 23, 41, 44 and the join 8 us.  A token over
+// by LDS reads: 2 x 4095 over 4001, 16 / 4 heads of 128, bfloat16: forward 303 us (890 TFLOP/s), dQ 484,
+// dK / dV 757.  2500 over up to 300 keys, 8 heads of 64, 8 items: 23, 41, 45 and the join 7 us.  A token over
 // 8000 keys by memory: 8 items, 16 / 4 heads of 64, float16, 66 MB in 14 us (4.7 TB/s), the join 4.
 
 #include "fm_attention.h"
