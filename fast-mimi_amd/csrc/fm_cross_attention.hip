@@ -64,38 +64,59 @@ __global__ __launch_bounds__(256) void cross_join_kernel(Attn a) {
   if (col < a.D) *reinterpret_cast<typename Vec<T, 4>::type*>(out + col) = y;
 }
 
-// Into how many parts a walk of `tiles` (of 128) is cut that `blocks` blocks make: until some 512
-// blocks run, at least two tiles each (backward, in 1 / 6 / 16 parts: 2 x 3000 queries over 20 keys, 8
-// heads of 64, FP32: 143 / 48 / 40 us; 4000 over 64, bfloat16, in 1 / 8 / 16: 59 / 23 / 21).
-int cut(long blocks, int tiles) { return (int)std::max<long>(1, std::min<long>({tiles / 2, 512 / std::max<long>(blocks, 1), 64})); }
-
 long sequences(const Attn& a) { return (long)a.B * a.KV; }
 
+// Into how many parts a walk of `tiles` (of 128) is cut that `blocks` blocks, 256 at most, make for `results` rows.
+// What a number of them takes, in half tiles: as many rounds of 256 blocks, or, in 16 bits, one of 256 or some of 512
+// that take half as long again, as they need, and what a second launch and the parts' way through memory cost.
+// Uncut / cut (us): forward 250 over 1000, 8 heads of 64, FP32 31.6 / 17.6, bfloat16 11.7 / 11.0; 1 over 3611, 2 of
+// 128, FP32 (29 parts) 40 / 17; 30 over 300, 4 of 64 (3), FP32 15.9 / 12.8, bfloat16 7.4 / 9.4; 500 over 500, 16 of
+// 128 (2), FP32 31 / 46; 3 x 168 over 3812, 8 of 64 (5), FP32 104 / 77.  256 / 512 blocks: 120 over 4000, 8 of 64, bfloat16
+// 12.7 / 13.7, 4000 over 4000, one of 64, bfloat16 23.5 / 20.8.  Two tiles a part / one: 1 over 8000, 4 key heads of 64,
+// float16 12.3 / 13.4.  dK / dV: 400 over 30, 4 of 64, bfloat16 (4) 20.4 / 17.7, 500 over 500, 8 of 128 (4) 32.7 / 38.1.
+int cut(const Attn& a, long blocks, int tiles, long results, bool wide) {
+  if (blocks == 0 || blocks > 256) return 1;
+  const long most = std::min(64, wide ? tiles : std::max(std::min(tiles, 8), tiles / 2));
+  int best = 1;
+  long least = 2 * tiles + 1;
+  auto consider = [&](long parts) {
+    if (parts < 2) return;
+    const long n = blocks * parts, rounds = wide ? 2 * ((n + 255) / 256) : n <= 256 ? 2 : 3 * ((n + 511) / 512);
+    const long cost = rounds * ((tiles + parts - 1) / parts) + 2 * (!wide ? 3 + parts * results / 4096 : a.D > 64 ? 1 : 2);
+    if (cost < least) least = cost, best = (int)parts;
+  };
+  for (long parts = 2; parts <= std::min(most, 8l); ++parts) consider(parts);
+  consider(std::min(most, 256 / blocks)), consider(std::min(most, 512 / blocks));
+  return best;
+}
+
 // A block's waves with rows (or keys) of their own: four where that leaves 384 blocks, two where 256
-// are left, else one, but that the waves which share them have two tiles of 32 each at least to walk.  With
-// two / four (us): forward 2 x 4096 over 500, 8 heads of 64 (512 blocks of 128 rows) 21.3 / 20.0, 4 x 2000
-// over 500, 8 / 2 heads of 128 (504) 37 / 31, 2 x 1000 over 1000, 16 / 4 heads of 128 (256) 31.7 / 34.4; short
-// walks, less than four / four: 2 x 3000 over 20, FP32 17.5 / 13.1, 13 over 7 8.9 / 7.5.
+// (heads beyond 64: 192) are left, else one, but those that share them have 32 each at least to walk.  With two / four (us):
+// forward 2 x 4096 over 500, 8 heads of 64 (512 blocks of 128 rows) 21.3 / 20.0, 4 x 2000 over 500, 8 / 2 heads
+// of 128 (504) 37 / 31, 2 x 1000 over 1000, 16 / 4 heads of 128 (256) 31.7 / 34.4; with one / two: 2000 over
+// 200, 8 / 2 heads of 128 (250 of 64) 17.0 / 11.4, 7 x 1069 over 1004, 2 of 64 (238) 15.6 / 17.9.  With one / two / four: 13
+// over 7, FP32 9.1 / 8.1 / 7.4; 13 over 40 9.1 / 8.0 / 9.3; 60 over 100, 8 heads of 128, FP32 13.2 / 17.9 / 23.6.
 int waves_apart(const Attn& a, long own, long walked) {
   const long seqs = sequences(a);
-  const int most = seqs * fm_ceil_div(own, 128) >= 384 ? 4 : seqs * fm_ceil_div(own, 64) >= 256 ? 2 : 1;
-  return std::max(most, walked < 128 ? 4 : walked < 256 ? 2 : 1);
+  const int most = seqs * fm_ceil_div(own, 128) >= 384 ? 4 : seqs * fm_ceil_div(own, 64) >= (a.D > 64 ? 192 : 256) ? 2 : 1;
+  return std::max(most, walked <= 32 || (most == 2 && walked < 128) ? 4 : walked <= 64 ? 2 : 1);
 }
 
 struct Shape {
   int waves, splits;
 };
-Shape row_shape(const Attn& a) {  // forward, dQ
+Shape row_shape(const Attn& a, bool wide) {  // forward, dQ; wide: FP32
   const long rows = (long)a.T * a.G;
-  const int splits = cut(sequences(a) * fm_ceil_div(rows, 32), fm_ceil_div(a.S, 128));
+  const int splits = cut(a, sequences(a) * fm_ceil_div(rows, 32), fm_ceil_div(a.S, 128), sequences(a) * rows, wide);
   return {splits > 1 ? 1 : waves_apart(a, rows, a.S), splits};
 }
 // dK / dV.  Where the blocks are no two to a CU, long walks are cut as well, if that fills the
 // rounds of 512 to nine tenths (whole backward, uncut / so, us: 8 x 2500 over 300, 8 heads of 64, FP32 320 / 284,
 // bfloat16 110 / 106, with lengths from 0 to 300 101 / 98; 4 x 2048 over 1024, 8 / 4 heads of 64, FP32 394 / 338).
-Shape key_shape(const Attn& a) {
+Shape key_shape(const Attn& a, bool wide) {
   const long rows = (long)a.T * a.G;
-  const int tiles = fm_ceil_div(rows, 128), splits = cut(sequences(a) * fm_ceil_div(a.S, 32), tiles);
+  const int own = !wide && a.D > 64 ? 64 : 32;  // keys of a block that is cut
+  const int tiles = fm_ceil_div(rows, 128), splits = cut(a, sequences(a) * fm_ceil_div(a.S, own), tiles, sequences(a) * a.S, wide);
   if (splits > 1) return {1, splits};
   const int waves = waves_apart(a, a.S, rows);
   const long blocks = sequences(a) * fm_ceil_div(a.S, 32 * waves);
@@ -105,9 +126,9 @@ Shape key_shape(const Attn& a) {
   return {waves, 1};
 }
 
-size_t backward_floats(const Attn& a) {
+size_t backward_floats(const Attn& a, bool wide) {
   const size_t dt = a.D > 64 ? 128 : 64;
-  const size_t q = row_shape(a).splits, k = key_shape(a).splits;
+  const size_t q = row_shape(a, wide).splits, k = key_shape(a, wide).splits;
   return std::max(q > 1 ? q * sequences(a) * a.T * a.G * (dt + 1) : 0, k > 1 ? k * 2 * sequences(a) * a.S * dt : 0);
 }
 
@@ -122,7 +143,7 @@ size_t backward_floats(const Attn& a) {
 template <typename T, int DT>
 int cross_forward(Attn a, hipStream_t stream) {
   const long rows = (long)a.T * a.G;
-  FM_CROSS_LAUNCH(attention_forward_kernel, row_shape(a).waves, rows, a.splits);
+  FM_CROSS_LAUNCH(attention_forward_kernel, row_shape(a, sizeof(T) == 4).waves, rows, a.splits);
   if (a.splits > 1)
     hipLaunchKernelGGL((attention_join_kernel<T, DT, true>), dim3(fm_ceil_div(sequences(a) * rows, 4)), dim3(256), 0, stream, a);
   return (int)hipGetLastError();
@@ -133,7 +154,7 @@ int cross_backward(Attn a, float* workspace, hipStream_t stream) {
   const long rows = (long)a.T * a.G;
   a.part_o = workspace;
   if (rows > 0) {
-    const Shape shape = row_shape(a);
+    const Shape shape = row_shape(a, sizeof(T) == 4);
     a.splits = shape.splits;
     a.part_ml = workspace + (size_t)a.splits * sequences(a) * rows * DT;
     FM_CROSS_LAUNCH(attention_dq_kernel, shape.waves, rows, a.splits);
@@ -141,7 +162,7 @@ int cross_backward(Attn a, float* workspace, hipStream_t stream) {
       hipLaunchKernelGGL((cross_join_kernel<T, DT, false>), dim3(fm_ceil_div(sequences(a) * rows, 1024 / DT)), dim3(256), 0, stream, a);
   }
   if (a.S > 0) {
-    const Shape shape = key_shape(a);
+    const Shape shape = key_shape(a, sizeof(T) == 4);
     a.splits = shape.splits;
     if constexpr (HELD<T, DT>) {
       const dim3 grid((unsigned)sequences(a), fm_ceil_div(a.S, 64), a.splits);
@@ -180,7 +201,8 @@ extern "C" {
 size_t fm_cross_attention_forward_workspace_bytes(int batch, int queries, int keys, int heads, int kv_heads, int head_dim) {
   const Attn a = cross_sizes(batch, queries, keys, heads, kv_heads, head_dim, 1.0f);
   if (cross_check(a, DT_F32) != FM_OK && cross_check(a, DT_BF16) != FM_OK) return 0;
-  return batch == 0 || queries == 0 ? 0 : workspace_floats(a, row_shape(a).splits) * sizeof(float);
+  if (batch == 0 || queries == 0) return 0;
+  return workspace_floats(a, std::max(row_shape(a, true).splits, row_shape(a, false).splits)) * sizeof(float);
 }
 
 int fm_cross_attention_forward(const void* q, long q_batch, long q_row, long q_head, const void* k, long k_batch, long k_row,
@@ -195,7 +217,7 @@ int fm_cross_attention_forward(const void* q, long q_batch, long q_row, long q_h
   if (batch == 0 || queries == 0) return FM_OK;
   if (!q || !out || !lse || (keys > 0 && (!k || !v))) return FM_BAD_ARGUMENT;
   if (reinterpret_cast<uintptr_t>(out) & 15) return FM_UNSUPPORTED;
-  a.splits = row_shape(a).splits;
+  a.splits = row_shape(a, dtype == DT_F32).splits;
   if (a.splits > 1) {
     if (!workspace || workspace_bytes < workspace_floats(a, a.splits) * sizeof(float)) return FM_WORKSPACE_TOO_SMALL;
     if (reinterpret_cast<uintptr_t>(workspace) & 15) return FM_UNSUPPORTED;
@@ -208,7 +230,7 @@ int fm_cross_attention_forward(const void* q, long q_batch, long q_row, long q_h
 size_t fm_cross_attention_backward_workspace_bytes(int batch, int queries, int keys, int heads, int kv_heads, int head_dim) {
   const Attn a = cross_sizes(batch, queries, keys, heads, kv_heads, head_dim, 1.0f);
   if (cross_check(a, DT_F32) != FM_OK && cross_check(a, DT_BF16) != FM_OK) return 0;
-  return batch == 0 || queries == 0 ? 0 : backward_floats(a) * sizeof(float);
+  return batch == 0 || queries == 0 ? 0 : std::max(backward_floats(a, true), backward_floats(a, false)) * sizeof(float);
 }
 
 int fm_cross_attention_backward(const void* dout, long dout_batch, long dout_row, long dout_head, const void* q, long q_batch,
@@ -227,7 +249,7 @@ int fm_cross_attention_backward(const void* dout, long dout_batch, long dout_row
   if (!dout || !q || !out || !lse || !dq || !stats || (keys > 0 && (!k || !v || !dk || !dv))) return FM_BAD_ARGUMENT;
   for (const void* p : {out, (const void*)dq, (const void*)dk, (const void*)dv})
     if (reinterpret_cast<uintptr_t>(p) & 15) return FM_UNSUPPORTED;
-  if (const size_t need = backward_floats(a) * sizeof(float)) {
+  if (const size_t need = backward_floats(a, dtype == DT_F32) * sizeof(float)) {
     if (!workspace || workspace_bytes < need) return FM_WORKSPACE_TOO_SMALL;
     if (reinterpret_cast<uintptr_t>(workspace) & 15) return FM_UNSUPPORTED;
   }
