@@ -271,8 +271,7 @@ __global__ __launch_bounds__(LPR < 256 ? 256 : LPR) void rms_backward_kernel(Rms
         t[e] = (S)dh, b[e] = (T)dh;
       }
       row_store<S, E, PAST>(static_cast<S*>(a.dres) + row * a.C, p + u * LPR, a.C, t);
-      if constexpr (!std::is_same<T, S>::value)
-        if (a.dx) row_store<T, E, PAST>(static_cast<T*>(a.dx) + row * a.C, p + u * LPR, a.C, b);
+      if (a.dx) row_store<T, E, PAST>(static_cast<T*>(a.dx) + row * a.C, p + u * LPR, a.C, b);
     }
   }
   if (!a.dw) return;
@@ -361,8 +360,7 @@ __global__ __launch_bounds__(256) void rms_backward_any_kernel(Rms a) {
       const float hh = h(c) * rstd;
       const float v = fmaf(rstd, fmaf(widen(dy[c]), one_weight<T>(a, c), -hh * s), dh ? widen(dh[c]) : 0.0f);
       static_cast<S*>(a.dres)[row * a.C + c] = (S)v;
-      if constexpr (!std::is_same<T, S>::value)
-        if (a.dx) static_cast<T*>(a.dx)[row * a.C + c] = (T)v;
+      if (a.dx) static_cast<T*>(a.dx)[row * a.C + c] = (T)v;
     }
   }
 }

@@ -665,8 +665,8 @@ int fm_rms_norm_forward(const void* x, long ld_x, const void* residual, long ld_
 /*
  * Its gradients, of the forward's x and residual: with hh = (x + residual) rstd and g = dy
  * gamma, dresidual = dh + rstd (g - hh mean(g hh)) in stream_dtype, dx the same in dtype
- * (NULL where the types are one and the caller takes dresidual), dgamma = the sum over
- * rows of dy hh (weight_dtype; NULL to leave it).  dh (stream_dtype; NULL for none) is the
+ * (NULL to leave it, as where the types are one and dresidual says the same), dgamma = the
+ * sum over rows of dy hh (weight_dtype; NULL to leave it).  dh (stream_dtype; NULL for none) is the
  * gradient that h has from elsewhere.  Either x or residual may be NULL: of an FP32 stream
  * the forward's h as the residual says the same and is one tensor less to read.
  * dx and dresidual are contiguous.  The workspace holds the row blocks' partial sums
