@@ -21,7 +21,7 @@ from __future__ import annotations
 
 import torch
 
-from .training import _DTYPES, _branch, _like, _on_gpu, _rows, _run, _scratch, _tensor
+from .training import _DTYPES, _branch, _like, _on_gpu, _rows, _run, _scratch, _sizes, _tensor
 
 __all__ = ["BLOCK", "linear", "quantize", "quantize_weight", "rms_norm"]
 
@@ -51,6 +51,7 @@ def quantize(x):
     x = _tensor("x", x)
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"x must have a last dimension, got shape {tuple(x.shape)}")
+    _sizes(x.shape[-1])
     device = _on_gpu(x=x)
     c = x.shape[-1]
     values = x.new_empty(x.shape, dtype=_VALUES)
@@ -68,6 +69,7 @@ def quantize_weight(weight):
     weight = _tensor("weight", weight)
     if weight.dim() != 2 or 0 in weight.shape:
         raise ValueError(f"weight must be [out, in], got shape {tuple(weight.shape)}")
+    _sizes(*weight.shape)
     device = _on_gpu(weight=weight)
     n, k = weight.shape
     values = weight.new_empty((n, k), dtype=_VALUES)
@@ -114,6 +116,7 @@ def linear(x, x_scale, weight, weight_scale, dtype: torch.dtype = torch.bfloat16
     (n, k), shape = weight.shape, x.shape
     if not shape or shape[-1] != k:
         raise ValueError(f"x must be [..., {k}] for weight {(n, k)}, got shape {tuple(shape)}")
+    _sizes(n, k)
     if k % 16:
         raise ValueError(f"the inputs of a projection must be a multiple of 16, got {k}")
     lead, blocks = shape[:-1], _blocks(k)
