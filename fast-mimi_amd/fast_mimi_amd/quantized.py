@@ -105,7 +105,7 @@ def linear(x, x_scale, weight, weight_scale, dtype: torch.dtype = torch.bfloat16
     ``x`` and ``x_scale`` are what :func:`quantize` or :func:`rms_norm` gave, ``weight`` and
     ``weight_scale`` what :func:`quantize_weight` did.  ``in`` must be a multiple of 16.
     """
-    given = x, weight
+    given = x, x_scale, weight, weight_scale
     x, weight = _tensor("x", x, (_VALUES,)), _tensor("weight", weight, (_VALUES,))
     _no_gradient(*given)
     x_scale, weight_scale = _tensor("x_scale", x_scale, (_SCALES,)), _tensor("weight_scale", weight_scale, (_SCALES,))
