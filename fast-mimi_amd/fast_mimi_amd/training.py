@@ -59,6 +59,7 @@ __all__ = [
 
 _DEFAULT_STREAM = "fast_mimi_amd.default_stream"
 _DTYPES = {torch.float32: nat.DTYPE_F32, torch.bfloat16: nat.DTYPE_BF16, torch.float16: nat.DTYPE_F16}
+_Parameter = torch.nn.Parameter
 # What may stand beside a type: itself, or FP32.
 _WIDER = {torch.float32: (torch.float32,), torch.bfloat16: (torch.bfloat16, torch.float32), torch.float16: (torch.float16, torch.float32)}
 
@@ -80,7 +81,7 @@ def _tensor(name: str, t, dtypes=tuple(_DTYPES)) -> torch.Tensor:
         raise TypeError(f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}, got {t.dtype}")
     if forward_ad._current_level >= 0:
         _reverse_mode(t)
-    if t.requires_grad:
+    if t.requires_grad or type(t) is _Parameter:  # a frozen one is a plain tensor to the kernels, not a subclass
         t = t.detach()
     return t.resolve_neg() if t.is_neg() else t
 
