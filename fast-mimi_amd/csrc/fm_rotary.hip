@@ -193,7 +193,7 @@ int fm_rotary(const void* q, long q_batch, long q_row, long q_head, int heads, c
               int positions_bytes, long first, int batch, int length, int head_dim, int rotated, int interleaved, float scale,
               int inverse, int dtype, void* q_out, void* k_out, hipStream_t stream) {
   if (batch < 0 || length < 0 || heads < 0 || kv_heads < 0 || head_dim <= 0 || rotated < 0 || rotated > head_dim || rotated % 2 ||
-      dtype < DT_F32 || dtype > DT_F16 || (positions && positions_bytes != 4 && positions_bytes != 8) || scale != scale)
+      dtype < DT_F32 || dtype > DT_F16 || (positions && positions_bytes != 4 && positions_bytes != 8) || !std::isfinite(scale))
     return FM_BAD_ARGUMENT;
   if (head_dim > 512 || (long)batch * length > 1 << 24 || (long)heads + kv_heads > 65535) return FM_UNSUPPORTED;
   if (batch == 0 || length == 0 || heads + kv_heads == 0) return FM_OK;

@@ -59,7 +59,7 @@ __all__ = [
 
 _DEFAULT_STREAM = "fast_mimi_amd.default_stream"
 _DTYPES = {torch.float32: nat.DTYPE_F32, torch.bfloat16: nat.DTYPE_BF16, torch.float16: nat.DTYPE_F16}
-_Parameter = torch.nn.Parameter
+_Parameter, _FLOAT_MAX = torch.nn.Parameter, torch.finfo(torch.float32).max
 # What may stand beside a type: itself, or FP32.
 _WIDER = {torch.float32: (torch.float32,), torch.bfloat16: (torch.bfloat16, torch.float32), torch.float16: (torch.float16, torch.float32)}
 
@@ -466,8 +466,8 @@ def _rotary_input(q, k, frequencies, positions, scale):
     if b * t > 1 << 24:
         raise ValueError(f"at most {1 << 24} positions in all, got {b * t}")
     scale = float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite, got {scale}")
+    if not abs(scale) <= _FLOAT_MAX:
+        raise ValueError(f"scale must be finite in FP32, got {scale}")
     return q, k, frequencies.contiguous(), positions, first, scale
 
 
