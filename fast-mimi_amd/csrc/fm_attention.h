@@ -535,7 +535,7 @@ FM_DEVICE void tile_barrier() {
 // the keys they see.
 template <int WQ, bool CROSS>
 struct Rows {
-  int b, kh, len, R, r, t, p, p_lo, p_hi, b_lo, k_lo, k_hi;
+  int b, kh, len, queries, R, r, t, p, p_lo, p_hi, b_lo, k_lo, k_hi;
   bool live;
   long row_index;  // into [B][T][H]
   FM_DEVICE Rows(const Attn& a, int wq, int lane) {
@@ -550,7 +550,7 @@ struct Rows {
     r = r0 + 32 * wq + (lane & 31);
     t = (int)fm_div(min(r, R - 1), a.by_g);
     p = past + t;
-    const int queries = CROSS && a.query_lengths ? min(max(a.query_lengths[b], 0), a.T) : a.T;
+    queries = CROSS && a.query_lengths ? min(max(a.query_lengths[b], 0), a.T) : a.T;
     live = r < R && (CROSS ? t < queries : p < len);
     row_index = ((long)b * a.T + t) * a.H + kh * a.G + (min(r, R - 1) - t * a.G);
     // The block's keys.
@@ -866,10 +866,13 @@ __global__ __launch_bounds__(256) void attention_join_kernel(Attn a) {
 // frames 12 / 13 / 13).  Rows of more keys with one large probability keep it (1.4 times at 0.3, 2.2
 // at 0.65): which they are is known after the pass only, and a second one for all
 // would be 12-24% of the backward (16 x 2500, window 250: 201 -> 230 us).
-// In a cross attention of few rows in all there may be little else: with 33 to 130 keys dQ of one to
-// four of them was at 1.2 times at the median of draws and up to 4 times, so those go over their
-// keys twice, whatever their number, where these are not cut (1 x 8 rows over 300, 8 heads of 64: backward 16 -> 19 us).
-constexpr int FEW_RESULTS = 512;
+// In a cross attention with few rows there may be little else: with 33 to 130 keys dQ of one to four of
+// them was at 1.2 times at the median of draws and up to 4 times.  So an item of up to EXACT_ROWS rows a key
+// head and EXACT_KEYS keys goes over these twice as well, in each part where they are cut: by its own lengths,
+// whatever else is in the batch.  Backward without / with it (us, 8 heads of 64): 1 x 8 rows over 300 keys 14.2 / 16.7, 64 x
+// 2 over 300 40.8 / 48, 20 over 200 in 3000, cut, 16.7 / 18.5.  For any number of rows it would be a tenth of long calls (up
+// to 320 keys, 8 x 2500 over 300: 99 / 111).
+constexpr int EXACT_ROWS = 64, EXACT_KEYS = 512;
 template <typename T, int DT, int WQ, int WK, bool CROSS>
 struct QueryGradient {
   template <bool SPLITS>
@@ -912,7 +915,11 @@ FM_DEVICE bool QueryGradient<T, DT, WQ, WK, CROSS>::run(const Attn& a, unsigned 
   auto load = [&](int i) {
     next.start(a, kp, vp, w.k_lo + i * L::KEYS, w.k_hi, lds + i % L::STAGES * 2 * L::TILE, wave, lane);
   };
-  if (begin < tiles) load(begin);
+  // With few keys (some row sees fewer than FEW) a first pass, over all of them, makes delta exact.
+  constexpr int FEW = 32;
+  const bool few = CROSS ? w.len < FEW || (w.queries * a.G <= EXACT_ROWS && w.len <= EXACT_KEYS) : min(w.b_lo + 1, a.window) < FEW;
+  bool first = sizeof(T) == 2 && begin < tiles && few;
+  if (begin < tiles) load(CROSS && first ? 0 : begin);
 
   typename G::Held q, g;
   const int head = w.kh * a.G + (min(w.r, w.R - 1) - w.t * a.G);
@@ -946,15 +953,12 @@ FM_DEVICE bool QueryGradient<T, DT, WQ, WK, CROSS>::run(const Attn& a, unsigned 
   float row_stats[2] = {lse, delta};
   arrive(row_stats);
   lse = row_stats[0], delta = row_stats[1];
-  // With few keys (some row sees fewer than FEW) a first pass makes delta exact.
-  constexpr int FEW = 32;
-  bool first = sizeof(T) == 2 && tiles > begin && (CROSS ? w.len : min(w.b_lo + 1, a.window)) < FEW;
-  if (CROSS && sizeof(T) == 2 && a.splits <= 1 && (long)a.B * a.T * a.H <= FEW_RESULTS) first = tiles > begin;
   for (;; first = false) {
-    for (int i = begin; i < tiles; ++i) {
+    const int end = CROSS && first ? all : tiles;
+    for (int i = CROSS && first ? 0 : begin; i < end; ++i) {
       tile_barrier();
       if constexpr (SPLITS) most = next.publish(lds, most);
-      if ((L::STAGES == 2 || SPLITS) && i + 1 < tiles) load(i + 1);
+      if ((L::STAGES == 2 || SPLITS) && i + 1 < end) load(i + 1);
       const unsigned char* kt = lds + i % L::STAGES * 2 * L::TILE;
   #pragma unroll
       for (int nb = 0; nb < L::NB; ++nb) {
@@ -992,7 +996,7 @@ FM_DEVICE bool QueryGradient<T, DT, WQ, WK, CROSS>::run(const Attn& a, unsigned 
         for (int e = 0; e < 16; ++e) rest += s[e];
         if (!first) G::template outer<true>(R::fresh(R::lds(kt) + row * R::PITCH + col_lane), s, acc);
       }
-      if (L::STAGES == 1 && !SPLITS && i + 1 < tiles) {
+      if (L::STAGES == 1 && !SPLITS && i + 1 < end) {
         tile_barrier();
         load(i + 1);
       }
@@ -1066,9 +1070,11 @@ constexpr bool HELD = sizeof(T) == 2 && DT == 128;
 // in two pieces; a block of that many rows is one or two tiles long (backward of 16 x
 // 13, 100 and 250 positions, never / up to 128 rows / up to 512: 13.0 / 13.4 / 13.4, 16.9 /
 // 17.7 / 17.8, 25.2 / 25.6 / 26.8 us; 16 x 2500 under a window of 100: 172 / 170 / 184).
-// So have cross attention's dV and dK of few keys in all (with 2 keys and 129 to 3000 queries up to
-// 1.8 times otherwise; 2 x 3000 over 16, 8 heads of 64: backward 24 -> 25 us).
-constexpr int FEW_ROWS = 128;
+// A cross attention's item has them in two pieces by its own lengths, however its rows are cut: up to FEW_ROWS
+// rows a key head, or FEW_KEYS keys (with 2 keys and 129 to 3000 queries up to 1.8 times otherwise; one
+// piece / two: 2 x 3000 over 16, 8 heads of 64, backward 22.1 / 23.1 us, 8 x 2500 over 64 47.6 / 50.7, 4 x 2000 over 60, 16 / 4
+// heads of 128, 67.6 / 70.8).
+constexpr int FEW_ROWS = 128, FEW_KEYS = 64;
 template <typename T, int DT, int WK, int WR, bool CROSS>
 struct KeyGradients {
   template <bool SPLITS>
@@ -1114,9 +1120,11 @@ FM_DEVICE bool KeyGradients<T, DT, WK, WR, CROSS>::run(const Attn& a, unsigned c
   const int p_hi = min((long)min(k0 + 32 * WK, len) - 1 + a.window - 1, (long)len - 1);
   int r_lo = (p_lo - past) * a.G, r_hi = (p_hi - past + 1) * a.G - 1;
   int tiles = k0 < len && p_hi >= p_lo ? (r_hi - r_lo) / ROWS + 1 : 0;
+  bool few = false;
   if constexpr (CROSS) {
     const int queries = a.query_lengths ? min(max(a.query_lengths[b], 0), a.T) : a.T;
     r_lo = 0, r_hi = queries * a.G - 1;
+    few = sizeof(T) == 2 && (r_hi < FEW_ROWS || len <= FEW_KEYS);
     tiles = k0 < len && r_hi >= 0 ? r_hi / ROWS + 1 : 0;
     if (a.splits > 1) {
       const int per = (tiles + a.splits - 1) / a.splits;
@@ -1125,7 +1133,7 @@ FM_DEVICE bool KeyGradients<T, DT, WK, WR, CROSS>::run(const Attn& a, unsigned c
       tiles = r_hi >= r_lo && tiles ? (r_hi - r_lo) / ROWS + 1 : 0;
     }
   }
-  const bool few = sizeof(T) == 2 && (r_hi - r_lo < FEW_ROWS || (CROSS && (long)a.B * a.S * a.KV <= FEW_RESULTS));
+  if (!CROSS) few = sizeof(T) == 2 && r_hi - r_lo < FEW_ROWS;
 
   const T* qp = static_cast<const T*>(a.q.p) + b * a.q.batch + kh * a.G * a.q.head;
   const T* gp = static_cast<const T*>(a.dout.p) + b * a.dout.batch + kh * a.G * a.dout.head;
