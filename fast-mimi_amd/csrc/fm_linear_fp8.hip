@@ -19,6 +19,8 @@
 
 #include "fm_common.h"
 
+#include <cstdio>
+
 namespace {
 
 typedef int intx8 __attribute__((ext_vector_type(8)));
@@ -354,23 +356,30 @@ __global__ __launch_bounds__(512) void linear_rows_kernel(Linear a) {
 // (us, few rows / 64 x 64 tiles: 1 x 4096 to 6144 8.1 / 9.9, 16 x 8192 to 2048 10.5 / 11.4, 32 x
 // 1008 to 1000 3.9 / 4.8, 32 x 4096 to 6144 14 / 11.9).
 //
+// Of the larger tiles those more than half of which hold results (the rule / 256 x 256 tiles, whose rounds the first
+// three fill: 65536 x 1024 to 64 14.3 / 18.6, to 128 16.6 / 21.3, 64 x 2048 to 65536 22.5 / 27.1; 20000 x 1024 to 64, 64 x 64 / 64
+// x 128, 5.7 / 7.3; just above half, 256 x 256 / 128 x 128, 129 x 2048 to 65536 30.8 / 36.5, 300 x 1024 to 65536 37.5 / 34.2).
+//
 // 256 x 256 tiles, one block to a CU, where their last round of 256 is nearly full: they
 // read the least per product (4096^3 60 us; 128 x 128 83, 64 x 128 96, 64 x 64 116).  Else
 // 128 x 128 (two to a CU) from 400 tiles on (1001 x 2048 to 8192 23.6; 64 x 128 28.1), 64
 // x 128 from 300 on (500 x 4096 to 6144 24.1; 128 x 128 26.6, 64 x 64 27.7), else 64 x 64
 // (256 x 2048 to 8192 11.6; 64 x 128 12.9), whose K is split, up to 512 blocks of eight or more of its
 // 128s: the parts go through memory (256 x 8192 to 2048, in 2 / 4 / 8: 19.8 / 17.2 / 21; 300 x
-// 1040 to 200, in 1 / 2: 5.1 / 6.4).  None was more than 8% behind the best of 20-40 tried at 20 sizes.
+// 1040 to 200, in 1 / 2: 5.1 / 6.4).  Of 40 sizes tried most were within 8% of the best of six plans; further behind
+// are rounds of 256 x 256 that are not as full (3000 x 8192 to 3000, 144 tiles: 113 us, 256 x 256 84; 16000 x 2048 to
+// 520, 189: 33 / 27) and 256 tiles of 64 x 64 that are split (1000 x 4096 to 1000, in 1 / 2: 12.1 / 17.6).
 struct LinearPlan {
   int bm, bn, splits;
 };
 LinearPlan linear_plan(long M, int N, int K) {
   if (M <= 16 || (M <= 32 && (long)N * K <= 1 << 21)) return {0, 0, 1};
   auto tiles = [&](int bm, int bn) { return (long)fm_ceil_div(M, bm) * fm_ceil_div(N, bn); };
+  auto full = [&](int bm, int bn) { return 2 * M * N > tiles(bm, bn) * bm * bn; };
   const long large = tiles(256, 256);
-  if (4 * large >= 3 * ((large + 255) / 256 * 256)) return {256, 256, 1};
-  if (tiles(128, 128) >= 400) return {128, 128, 1};
-  if (tiles(64, 128) >= 300) return {64, 128, 1};
+  if (full(256, 256) && 4 * large >= 3 * ((large + 255) / 256 * 256)) return {256, 256, 1};
+  if (full(128, 128) && tiles(128, 128) >= 400) return {128, 128, 1};
+  if (full(64, 128) && tiles(64, 128) >= 300) return {64, 128, 1};
   const long small = tiles(64, 64);
   return {64, 64, (int)std::max<long>(1, std::min<long>({512 / small, fm_ceil_div(K, 128) / 8, 8}))};
 }
@@ -402,6 +411,14 @@ size_t fm_linear_fp8_workspace_bytes(long rows, int in_features, int out_feature
   if (rows <= 0 || in_features <= 0 || out_features <= 0) return 0;
   const LinearPlan p = linear_plan(rows, out_features, in_features);
   return p.splits > 1 ? (size_t)p.splits * rows * out_features * sizeof(float) : 0;
+}
+
+int fm_linear_fp8_plan(long rows, int in_features, int out_features, char* buf, int size) {
+  if (!buf || size <= 0 || rows <= 0 || in_features <= 0 || out_features <= 0) return FM_BAD_ARGUMENT;
+  const LinearPlan p = linear_plan(rows, out_features, in_features);
+  if (p.bm == 0) snprintf(buf, (size_t)size, "linear_rows_kernel<%d>", rows <= 16 ? 1 : 2);
+  else snprintf(buf, (size_t)size, "linear_tile_kernel<%d, %d> splits=%d", p.bm, p.bn, p.splits);
+  return FM_OK;
 }
 
 int fm_linear_fp8(const void* x, const void* x_scales, const void* weight, const void* weight_scales, long rows,

@@ -109,6 +109,7 @@ _SIGNATURES = {
     "fm_quantize_rows": ([_P, _L, _L, _I, _I, _P, _P, _P], _I),
     "fm_quantize_weight": ([_P, _I, _I, _I, _P, _P, _P], _I),
     "fm_linear_fp8_workspace_bytes": ([_L, _I, _I], _S),
+    "fm_linear_fp8_plan": ([_L, _I, _I, ctypes.c_char_p, _I], _I),
     "fm_linear_fp8": ([_P, _P, _P, _P, _L, _I, _I, _I, _P, _P, _S, _P], _I),
     "fm_cross_attention_forward_workspace_bytes": ([_I, _I, _I, _I, _I, _I], _S),
     "fm_cross_attention_forward": ([_P, _L, _L, _L, _P, _L, _L, _L, _P, _L, _L, _L, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P, _P, _P, _S, _P], _I),
@@ -173,4 +174,11 @@ def last_gemm_plan() -> str:
     """Kernel, tiles and K splits of the last GEMM-engine call on this thread."""
     buf = ctypes.create_string_buffer(160)
     check(library().fm_gemm_last_plan(buf, len(buf)), "fm_gemm_last_plan")
+    return buf.value.decode()
+
+
+def linear_fp8_plan(rows: int, in_features: int, out_features: int) -> str:
+    """Kernel, tile and K splits of an 8-bit product of these sizes."""
+    buf = ctypes.create_string_buffer(80)
+    check(library().fm_linear_fp8_plan(rows, in_features, out_features, buf, len(buf)), "fm_linear_fp8_plan")
     return buf.value.decode()

@@ -758,10 +758,13 @@ int fm_quantize_weight(const void* weight, int out_features, int in_features, in
  * y 16-byte aligned, in_features a multiple of 16 up to 2^22, rows and out_features up to 2^24,
  * 2^40 results.  The workspace holds the parts of calls whose in_features are split over
  * blocks; NULL where its size is 0.
+ * fm_linear_fp8_plan writes the kernel, tile (rows, outputs) and K splits of such a call into
+ * `buf` (at most `size` bytes, NUL-terminated).  Host only, as the size is.
  * Stands beside fm_linear (nn.Linear of the transformer layers, model.py:1870-2061)
  * where a model over the codes is served in 8 bits.
  */
 size_t fm_linear_fp8_workspace_bytes(long rows, int in_features, int out_features);
+int fm_linear_fp8_plan(long rows, int in_features, int out_features, char* buf, int size);
 int fm_linear_fp8(const void* x, const void* x_scales, const void* weight,
                   const void* weight_scales, long rows, int in_features, int out_features,
                   int dtype, void* y, float* workspace, size_t workspace_bytes,
