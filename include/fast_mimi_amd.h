@@ -753,8 +753,8 @@ int fm_quantize_weight(const void* weight, int out_features, int in_features, in
  * y [rows][out_features] (dtype) = x weight^T of 8-bit x [rows][in_features] and weight
  * [out_features][in_features] with their scales (above): every product times both
  * powers of two, summed in FP32, rounded once.  For 16-bit results the matrix cores line up
- * eight products by their largest and drop what lies 2^-13 below it; FP32 results are sums of
- * exact products.  Values below 2^-126 with their scale may count as zero.  All contiguous, x, weight and
+ * eight neighbouring products by the largest and drop the bits that lie more than 2^-13 below its
+ * power of two, however small the sum comes out; FP32 results are sums of exact products.  Values below 2^-126 with their scale may count as zero.  All contiguous, x, weight and
  * y 16-byte aligned, in_features a multiple of 16 up to 2^22, rows and out_features up to 2^24,
  * 2^40 results.  The workspace holds the parts of calls whose in_features are split over
  * blocks; NULL where its size is 0.
