@@ -178,12 +178,8 @@ int cross_backward(Attn a, float* workspace, hipStream_t stream) {
   return (int)hipGetLastError();
 }
 
-int cross_check(const Attn& a, int dtype) {
-  if (const int status = check(a, dtype, true)) return status;
-  // A join has four rows to a block.
-  if (sequences(a) * std::max<long>((long)a.T * a.G, 2l * a.S) > 4l * INT_MAX) return FM_UNSUPPORTED;
-  return FM_OK;
-}
+// Joins need no limit of their own: only walks of fewer than 512 blocks, of 128 rows or keys at most, are cut.
+int cross_check(const Attn& a, int dtype) { return check(a, dtype, true); }
 
 Attn cross_sizes(int batch, int queries, int keys, int heads, int kv_heads, int head_dim, float scale) {
   Attn a{};
