@@ -446,8 +446,11 @@ __global__ __launch_bounds__(256) void quantize_weight_kernel(const T* w, int N,
 
 constexpr int MOST_CHANNELS = 1 << 26;
 constexpr long MOST_ROWS = 1 << 23;  // of a launch: a grid has at most 2^32 threads
-// Bytes of the stream from which on results go past the L2, whose eight parts hold 32 MB (bfloat16, through / past:
-// forward 40000 x 2048 93 / 70 us, 16000 x 2048 31 / 30, 40000 x 4096 with an FP32 stream 335 / 326).
+// Bytes of the stream from which on results go past the L2, whose eight parts hold 32 MB (through / past, us, inputs
+// that are not in the caches; in brackets with a product that reads y and a norm that reads h next.  bfloat16 x 4096:
+// 16 MB 11.9 / 11.6 (42 / 44), 32 MB 25.6 / 21.0 (74 / 73), 64 MB 48 / 48 (150 / 138), 256 MB 196 / 191 (489 / 472); with an
+// FP32 stream 24 MB 14.0 / 13.4 (46 / 45), 48 MB 33 / 25 (81 / 76), 128 MB 81 / 73 (204 / 191); backward 64 MB 65 / 58.  At 32 MB
+// and above nothing lost more than 3%, below it what reads y lost up to 6%).
 constexpr long PAST_FROM = 32l << 20;
 
 int rms_check(const Rms& a, int dtype, int stype, int wtype) {

@@ -111,7 +111,8 @@ def linear(x, x_scale, weight, weight_scale, dtype: torch.dtype = torch.bfloat16
     others that lie more than 2^-13 below its power of two (products down to 2^-6 of it keep all of theirs):
     2e-5 of the results' size with normal values, 1e-4 with values that spread over powers of two of 2^-4
     to 2^4.  That is a share of the products, not of their sum: where large ones cancel, it may be
-    all that is left.  FP32 results take about twice the time.
+    all that is left.  FP32 results take about twice the time, and want each value times its scale between
+    2^-126 and 2^128, as those of finite FP32 inputs are (to 3.29e38).
     """
     given = x, x_scale, weight, weight_scale
     x, weight = _tensor("x", x, (_VALUES,)), _tensor("weight", weight, (_VALUES,))

@@ -504,7 +504,7 @@ def rotary_forward(q, k, frequencies, positions=None, interleaved: bool = False,
     ``[batch, positions]``, or the first position (``None``: 0).
 
     Angles are formed in 64 bits, with what those round off beside them: positions up to 2^53 are
-    as exact as small ones.  At most 2^24 positions in all, heads of 512.
+    as exact as small ones.  At most 2^24 positions in all, 65535 heads of both, of up to 512 channels.
     """
     return _rotate(q, k, frequencies, positions, interleaved, scale, 0)
 

@@ -688,7 +688,8 @@ int fm_rms_norm_backward(const void* dy, long ld_dy, const void* x, long ld_x, c
  * per position.  positions holds [length] per batch item, positions_batch apart (0: the
  * same for all), of positions_bytes 4 or 8 (exact up to 2^53); NULL: first, first + 1, ...  inverse turns
  * back (the gradient).  q / k are strided (elements; channels adjacent), q_out / k_out
- * contiguous, other memory than q / k.  head_dim <= 512, batch * length <= 2^24.
+ * contiguous, other memory than q / k.  head_dim <= 512, batch * length <= 2^24,
+ * heads + kv_heads <= 65535.
  * Replaces MimiRotaryEmbedding and its use in MimiAttention (model.py:1484-1535, :1870-1961) where the
  * transformer is trained, with positions, pairings and frequencies of its own.
  */
@@ -754,7 +755,9 @@ int fm_quantize_weight(const void* weight, int out_features, int in_features, in
  * [out_features][in_features] with their scales (above): every product times both
  * powers of two, summed in FP32, rounded once.  For 16-bit results the matrix cores line up
  * eight neighbouring products by the largest and drop the bits that lie more than 2^-13 below its
- * power of two, however small the sum comes out; FP32 results are sums of exact products.  Values below 2^-126 with their scale may count as zero.  All contiguous, x, weight and
+ * power of two, however small the sum comes out; FP32 results are sums of exact products of
+ * bfloat16 values: of a value times its scale below 2^-126 bits may be lost, and from 2^128
+ * on it is infinite (fm_quantize_* give such only for inputs from 3.29e38 on).  All contiguous, x, weight and
  * y 16-byte aligned, in_features a multiple of 16 up to 2^22, rows and out_features up to 2^24,
  * 2^40 results.  The workspace holds the parts of calls whose in_features are split over
  * blocks; NULL where its size is 0.

@@ -135,6 +135,10 @@ def test_scales_reach_far(m, n, k, dtype):
 
     for by in (100, -100):
         assert torch.equal(qz.linear(x, moved(xs, by), w, moved(ws, -by), dtype), plain)
+    # FP32 results: within the range of a value times its scale.
+    exact = qz.linear(x, xs, w, ws, F32)
+    for by in (110, -110):
+        assert torch.equal(qz.linear(x, moved(xs, by), w, moved(ws, -by), F32), exact)
     if dtype == BF16:
         for by in (60, -60):
             assert torch.equal(qz.linear(x, moved(xs, by), w, ws, dtype).double(), plain.double() * 2.0 ** by)
