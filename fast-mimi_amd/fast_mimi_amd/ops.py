@@ -129,7 +129,7 @@ def op(entry: str):
 _dispatch_modes, _function_modes = torch._C._len_torch_dispatch_stack, torch._C._len_torch_function_stack
 _tracing, _functorch_level = torch._C._get_tracing_state, torch._C._functorch.peek_interpreter_stack
 _profiling = torch._C._autograd._profiler_enabled
-_raw_stream, _Tensor = getattr(torch._C, "_cuda_getCurrentRawStream", None), torch.Tensor
+_raw_stream, _Tensor, _Parameter = getattr(torch._C, "_cuda_getCurrentRawStream", None), torch.Tensor, torch.nn.Parameter
 
 _POINTERS = {entry: tuple(i for i, item in enumerate(spec.split()) if item[:3] in ("in:", "out", "res"))
              for entry, spec in SPECS.items()}
@@ -148,8 +148,8 @@ def _observed() -> bool:
 
 def call(entry: str, *args) -> None:
     """Run C-ABI entry point ``entry``: through its operator when something
-    observes operator calls or a tensor is not a plain one (a subclass, or
-    one that requires a gradient), else the C function itself on the current
+    observes operator calls or a tensor is not a plain one (a subclass but a
+    Parameter, or one that requires a gradient), else the C function itself on the current
     stream, which is all the operator's implementation does (the runtime
     resolves lazy negations where tensors come in).  A streamed 80 ms
     chunk is some 85 calls; the dispatcher's way took about 11 us of host time
@@ -161,7 +161,7 @@ def call(entry: str, *args) -> None:
             t = values[i]
             if t is None:
                 continue
-            if type(t) is not _Tensor or t.requires_grad:
+            if (type(t) is not _Tensor and type(t) is not _Parameter) or t.requires_grad:
                 break
             if device is None:
                 device = t.device

@@ -22,7 +22,7 @@ from __future__ import annotations
 
 import torch
 
-from .training import _DTYPES, _branch, _like, _on_gpu, _rows, _run, _scratch, _sizes, _tensor
+from .training import _DTYPES, _branch, _like, _on_gpu, _rows, _run, _scratch, _tensor, _too_large
 
 __all__ = ["BLOCK", "linear", "quantize", "quantize_weight", "rms_norm"]
 
@@ -32,7 +32,7 @@ _VALUES, _SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
 
 def _no_gradient(*inputs) -> None:
     for t in inputs:
-        if t is not None and isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled():
+        if isinstance(t, torch.Tensor) and t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("the 8-bit operators have no gradient: an input requires one (call them under torch.no_grad())")
 
 
@@ -52,7 +52,8 @@ def quantize(x):
     x = _tensor("x", x)
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"x must have a last dimension, got shape {tuple(x.shape)}")
-    _sizes(x.shape[-1])
+    if x.shape[-1] >> 31:
+        raise _too_large(x.shape[-1])
     device = _on_gpu(x=x)
     c = x.shape[-1]
     values = x.new_empty(x.shape, dtype=_VALUES)
@@ -70,9 +71,10 @@ def quantize_weight(weight):
     weight = _tensor("weight", weight)
     if weight.dim() != 2 or 0 in weight.shape:
         raise ValueError(f"weight must be [out, in], got shape {tuple(weight.shape)}")
-    _sizes(*weight.shape)
-    device = _on_gpu(weight=weight)
     n, k = weight.shape
+    if (n | k) >> 31:
+        raise _too_large(n, k)
+    device = _on_gpu(weight=weight)
     values = weight.new_empty((n, k), dtype=_VALUES)
     scales = weight.new_empty((_blocks(n), _blocks(k)), dtype=_SCALES)
     _run(device, "fm_quantize_weight", weight.contiguous(), n, k, _DTYPES[weight.dtype], values, scales)
@@ -125,7 +127,8 @@ def linear(x, x_scale, weight, weight_scale, dtype: torch.dtype = torch.bfloat16
     (n, k), shape = weight.shape, x.shape
     if not shape or shape[-1] != k:
         raise ValueError(f"x must be [..., {k}] for weight {(n, k)}, got shape {tuple(shape)}")
-    _sizes(n, k)
+    if (n | k) >> 31:
+        raise _too_large(n, k)
     if k % 16:
         raise ValueError(f"the inputs of a projection must be a multiple of 16, got {k}")
     lead, blocks = shape[:-1], _blocks(k)

@@ -59,7 +59,7 @@ __all__ = [
 
 _DEFAULT_STREAM = "fast_mimi_amd.default_stream"
 _DTYPES = {torch.float32: nat.DTYPE_F32, torch.bfloat16: nat.DTYPE_BF16, torch.float16: nat.DTYPE_F16}
-_Parameter, _FLOAT_MAX = torch.nn.Parameter, torch.finfo(torch.float32).max
+_FLOAT_MAX = torch.finfo(torch.float32).max
 # What may stand beside a type: itself, or FP32.
 _WIDER = {torch.float32: (torch.float32,), torch.bfloat16: (torch.bfloat16, torch.float32), torch.float16: (torch.float16, torch.float32)}
 
@@ -81,16 +81,15 @@ def _tensor(name: str, t, dtypes=tuple(_DTYPES)) -> torch.Tensor:
         raise TypeError(f"{name} must be {' or '.join(str(d).replace('torch.', '') for d in dtypes)}, got {t.dtype}")
     if forward_ad._current_level >= 0:
         _reverse_mode(t)
-    if t.requires_grad or type(t) is _Parameter:  # a frozen one is a plain tensor to the kernels, not a subclass
+    if t.requires_grad:
         t = t.detach()
     return t.resolve_neg() if t.is_neg() else t
 
 
-def _sizes(*sizes) -> None:
-    """Refuses what the entry points' 32-bit sizes cannot hold: it would arrive there as another size.  (Views of
-    one element, expanded, are that long at no cost.)"""
-    if max(sizes) > 0x7fffffff:
-        raise ValueError(f"sizes must be below 2^31, got {max(sizes)}")
+def _too_large(*sizes) -> ValueError:
+    """What the entry points' 32-bit sizes cannot hold (``(m | n) >> 31`` of any) would arrive there as another
+    size.  (Views of one element, expanded, are that long at no cost.)"""
+    return ValueError(f"sizes must be below 2^31, got {max(sizes)}")
 
 
 def _on_gpu(**tensors) -> torch.device:
@@ -203,7 +202,8 @@ def _norm_input(x, weight, bias):
     x = _tensor("x", x)
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"x must have a last dimension to normalise, got shape {tuple(x.shape)}")
-    _sizes(x.shape[-1])
+    if x.shape[-1] >> 31:
+        raise _too_large(x.shape[-1])
     weight, bias, wtype = _norm_weights(x, weight, bias)
     return x, weight, bias, wtype
 
@@ -283,7 +283,8 @@ def _branch(x, weight, residual, eps):
     shape = x.shape
     if not shape or not shape[-1]:
         raise ValueError(f"x must have a last dimension to normalise, got shape {tuple(shape)}")
-    _sizes(shape[-1])
+    if shape[-1] >> 31:
+        raise _too_large(shape[-1])
     if residual is not None:
         residual = _tensor("residual", residual, _WIDER[x.dtype])
         if residual.shape != shape:
@@ -343,7 +344,8 @@ def rms_norm_backward(grad, x, rstd, weight=None, residual=None, grad_h=None):
     shape = x.shape
     if not shape or not shape[-1] or grad.shape != shape:
         raise ValueError(f"grad must have x's shape {tuple(shape)}, got {tuple(grad.shape)}")
-    _sizes(shape[-1])
+    if shape[-1] >> 31:
+        raise _too_large(shape[-1])
     if residual is not None and residual.shape != shape:
         raise ValueError(f"residual must have x's shape {tuple(shape)}, got {tuple(residual.shape)}")
     if rstd.shape != shape[:-1] or not rstd.is_contiguous():
@@ -444,12 +446,14 @@ def _rotary_input(q, k, frequencies, positions, scale):
     for name, t in (("q", q), ("k", k)):
         if t is not None and t.dim() != 4:
             raise ValueError(f"{name} must be [batch, positions, heads, head_dim], got shape {tuple(t.shape)}")
-    b, t, _, d = q.shape
+    b, t, h, d = q.shape
+    kv = 0 if k is None else k.shape[2]
     if k is not None and (k.shape[:2] != (b, t) or k.shape[3] != d):
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} do not belong together")
     if not 0 < d <= 512:
         raise ValueError(f"head_dim must be from 1 to 512, got {d}")
-    _sizes(q.shape[2], 0 if k is None else k.shape[2])
+    if (h | kv) >> 31:
+        raise _too_large(h, kv)
     frequencies = _tensor("frequencies", frequencies, (torch.float64,))
     if frequencies.dim() != 1 or not 0 < 2 * frequencies.numel() <= d:
         raise ValueError(f"frequencies must be [pairs], at most {d // 2} for heads of {d}, got shape {tuple(frequencies.shape)}")
@@ -550,11 +554,12 @@ def _attention_operands(q, k, v, scale):
     for name, t in (("q", q), ("k", k), ("v", v)):
         if t.dim() != 4:
             raise ValueError(f"{name} must be [batch, positions, heads, head_dim], got shape {tuple(t.shape)}")
-    b, _, h, d = q.shape
+    b, t, h, d = q.shape
     s, kv = k.shape[1], k.shape[2]
     if k.shape != (b, s, kv, d) or v.shape != k.shape:
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
-    _sizes(b, q.shape[1], s, h)
+    if (b | t | s | h) >> 31:
+        raise _too_large(b, t, s, h)
     if h == 0 or kv == 0 or h % kv:
         raise ValueError(f"{h} query heads are not a multiple of {kv} key heads")
     unit = 4 if q.dtype == torch.float32 else 8
@@ -774,7 +779,8 @@ def _embedding_input(codes, table, scale):
         raise ValueError(f"table must be [codebooks, entries, dim], got shape {tuple(table.shape)}")
     if codes.shape[1] != table.shape[0]:
         raise ValueError(f"codes have {codes.shape[1]} codebooks, table {table.shape[0]}")
-    _sizes(*codes.shape, table.shape[2])
+    if max(*codes.shape, table.shape[2]) >> 31:
+        raise _too_large(*codes.shape, table.shape[2])
     if table.shape[1] > 32768:
         raise ValueError(f"a codebook may have at most 32768 entries, got {table.shape[1]}")
     scale = float(scale)

@@ -8,7 +8,6 @@ import torch
 
 from fast_mimi_amd import _native as nat
 from fast_mimi_amd import quantized as qz
-from fast_mimi_amd import training as tr
 
 X8, W8 = torch.zeros(4, 256).to(torch.float8_e4m3fn), torch.zeros(100, 256).to(torch.float8_e4m3fn)
 XS, WS = (torch.full((n, 2), 127, dtype=torch.uint8).view(torch.float8_e8m0fnu) for n in (4, 1))
@@ -22,12 +21,6 @@ def test_scales_that_require_a_gradient_are_refused(which):
         qz.linear(*args)
     with torch.no_grad(), pytest.raises(ValueError, match="ROCm GPU"):  # as far as a CPU goes
         qz.linear(*args)
-
-
-def test_frozen_parameters_are_plain_tensors():
-    frozen = torch.nn.Parameter(torch.ones(3), requires_grad=False)
-    got = tr._tensor("weight", frozen)
-    assert type(got) is torch.Tensor and got.data_ptr() == frozen.data_ptr()
 
 
 @pytest.mark.gpu
