@@ -13,9 +13,10 @@
 // long walk, it is cut, and the parts are joined in their order.
 //
 // Long calls are bound by the matrix cores and the exponentials beside them, dK / dV with heads of 128
-// by LDS reads: 2 x 4095 over 4001, 16 / 4 heads of 128, bfloat16: forward 303 us (890 TFLOP/s), dQ 484,
-// dK / dV 757.  2500 over up to 300 keys, 8 heads of 64, 8 items: 23, 41, 45 and the join 7 us.  A token over
-// 8000 keys by memory: 8 items, 16 / 4 heads of 64, float16, 66 MB in 14 us (4.7 TB/s), the join 4.
+// by LDS reads: 2 x 4095 over 4001, 16 / 4 heads of 128, bfloat16: forward 317 us (850 TFLOP/s), dQ 510,
+// dK / dV 771 (under the tracer; the whole pass 1500).  2500 over up to 300 keys, 8 heads of 64, 8 items: 25, 43, 50 and the
+// join 7 us (120).  FP32, 4 x 2048 over 1024, 8 / 4 heads of 128: 294, 473, 659 us (117, 109 and 104 TFLOP/s).  A token over
+// 8000 keys by memory: 8 items, 16 / 4 heads of 64, float16, 66 MB in 13.4 us (4.9 TB/s), the join 4.
 
 #include "fm_attention.h"
 

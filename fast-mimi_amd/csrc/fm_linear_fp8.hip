@@ -13,10 +13,10 @@
 // cancel.  FP32 results would lose bits by it, so those are summed from bfloat16 products, which are
 // exact: e4m3 times a power of two is a bfloat16, at half the matrix rate.
 //
-// Many rows are bound by the matrix cores and what feeds them: 8192^3 in 430 us (2560 TFLOP/s; up to 510 as the
-// clock goes, and 413 on another card), FP32 results 916; without its loads from memory it takes a tenth less.
-// Few rows are bound by latency and the weights' bytes: 1 x 4096 to 6144 7.4 us (25 MB), 32 x 8192 to 2048 6.3
-// and the join 2.7.
+// Many rows are bound by the matrix cores and what feeds them: 8192^3 in 413 to 437 us (2510 to 2660 TFLOP/s; up to
+// 520 as the clock goes), FP32 results 883; without its loads from memory it takes a tenth less.
+// Few rows are bound by latency and the weights' bytes: 1 x 4096 to 6144 6.5 us (25 MB; 8.4 under the tracer), 32 x 8192
+// to 2048 8.8 with the join.  (All in a queue of captured calls, bfloat16.)
 
 #include "fm_common.h"
 
@@ -354,20 +354,20 @@ __global__ __launch_bounds__(512) void linear_rows_kernel(Linear a) {
 // How a call runs.  Rows a block (0: the few-row kernel), columns a block, parts of K.
 //
 // Few rows up to 16, and up to 32 where the weights are 2 MB or less and latency is all
-// (us, few rows / 64 x 64 tiles: 1 x 4096 to 6144 8.1 / 9.9, 16 x 8192 to 2048 10.5 / 11.4, 32 x
-// 1008 to 1000 3.9 / 4.8, 32 x 4096 to 6144 14 / 11.9).
+// (us, few rows / the best of 64 x 64 tiles: 1 x 4096 to 6144 6.5 / 7.3, 16 x 8192 to 2048 9.6 / 8.5, 32 x
+// 1008 to 1000 3.3 / 4.3, 32 x 4096 to 6144 15.5 / 8.9).
 //
 // Of the larger tiles those more than half of which hold results (the rule / 256 x 256 tiles, whose rounds the first
 // three fill: 65536 x 1024 to 64 14.3 / 18.6, to 128 16.6 / 21.3, 64 x 2048 to 65536 22.5 / 27.1; 20000 x 1024 to 64, 64 x 64 / 64
 // x 128, 5.7 / 7.3; just above half, 256 x 256 / 128 x 128, 129 x 2048 to 65536 30.8 / 36.5, 300 x 1024 to 65536 37.5 / 34.2).
 //
 // 256 x 256 tiles, one block to a CU, where their last round of 256 is nearly full: they
-// read the least per product (4096^3 60 us; 128 x 128 83, 64 x 128 96, 64 x 64 116).  Else
-// 128 x 128 (two to a CU) from 400 tiles on (1001 x 2048 to 8192 23.6; 64 x 128 28.1), 64
-// x 128 from 300 on (500 x 4096 to 6144 24.1; 128 x 128 26.6, 64 x 64 27.7), else 64 x 64
-// (256 x 2048 to 8192 11.6; 64 x 128 12.9), whose K is split, up to 512 blocks of eight or more of its
-// 128s: the parts go through memory (256 x 8192 to 2048, in 2 / 4 / 8: 19.8 / 17.2 / 21; 300 x
-// 1040 to 200, in 1 / 2: 5.1 / 6.4).  Of 40 sizes tried most were within 8% of the best of six plans; further behind
+// read the least per product (4096^3 61 us; 128 x 128 79, 64 x 128 97, 64 x 64 129).  Else
+// 128 x 128 (two to a CU) from 400 tiles on (1001 x 2048 to 8192 22.0; 64 x 128 27.1), 64
+// x 128 from 300 on (500 x 4096 to 6144 23.5; 128 x 128 25.8, 64 x 64 27.1), else 64 x 64
+// (256 x 2048 to 8192 9.1; 64 x 128 8.7), whose K is split, up to 512 blocks of eight or more of its
+// 128s: the parts go through memory (256 x 8192 to 2048, in 2 / 4 / 8: 21.4 / 16.7 / 19.9; 300 x
+// 1040 to 200, in 1 / 2: 4.6 / 5.7).  Of 40 sizes tried most were within 8% of the best of six plans; further behind
 // are rounds of 256 x 256 that are not as full (3000 x 8192 to 3000, 144 tiles: 113 us, 256 x 256 84; 16000 x 2048 to
 // 520, 189: 33 / 27) and 256 tiles of 64 x 64 that are split (1000 x 4096 to 1000, in 1 / 2: 12.1 / 17.6).
 struct LinearPlan {

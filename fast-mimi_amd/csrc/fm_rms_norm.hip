@@ -13,8 +13,9 @@
 // it.  Rows start anywhere: 16-byte accesses need no alignment on this part, so
 // channels that are not whole vectors cost their last vector only.
 //
-// 40001 x 4096, bfloat16 on an FP32 stream: forward 326 us (6.0 TB/s), backward 465 (5.6; a large copy
-// reaches 4.9), the join 7; 1001 x 2048 bfloat16 in 8 bits 6; 13 x 512 FP32 2.9 and 5.8, by latency.
+// 40001 x 4096, bfloat16 on an FP32 stream: forward 327 us (6.0 TB/s), backward 460 (5.7; a large copy
+// reaches 4.9), the join 7; 1001 x 2048 bfloat16 in 8 bits 7; 13 x 512 FP32 2.6 and 6.0, by latency.  In 8 bits
+// as they are: rows 16000 x 2048 17 (5.9 TB/s), weights 8192 x 8192, once each, 105 (read twice, by single values).
 
 #include "fm_rows.h"
 
